@@ -26,6 +26,7 @@ lib = ctypes.CDLL(str(LIB_PATH))
 _i = ctypes.c_int
 _p = ctypes.c_void_p
 _sz = ctypes.c_size_t
+_d = ctypes.c_double
 
 
 class FnoConfig(ctypes.Structure):
@@ -78,6 +79,11 @@ _SIGNATURES = {
     "scx_clear_variants": ([], None),
     "scx_fno2d_workspace_size": ([ctypes.POINTER(FnoConfig)], _sz),
     "scx_fno2d_fwd": ([ctypes.POINTER(FnoConfig), ctypes.POINTER(FnoParams), _p, _p, _p, _sz, _p], _i),
+    "scx_grad_norm_workspace_size": ([_i], _sz),
+    "scx_grad_norm": ([_i, _p, _p, _p, _p, _p, _sz, _p], _i),
+    "scx_grad_clip": ([_i, _p, _p, _p, _d, _p, _p, _sz, _p], _i),
+    "scx_adam_workspace_size": ([_i], _sz),
+    "scx_adam_step": ([_i, _p, _p, _p, _p, _p, _p, _p, _d, _p, _d, _d, _d, _d, _i, _d, _p, _p, _p, _sz, _p], _i),
     "scx_ipc_handle_bytes": ([], _i),
     "scx_ipc_export": ([_p, _p, ctypes.POINTER(ctypes.c_ulonglong)], _i),
     "scx_ipc_import": ([_p, ctypes.POINTER(ctypes.c_void_p)], _i),

@@ -310,6 +310,53 @@ int scx_spectral_conv2d_fwd_noalloc(const float* x, const float* weights1, const
                                     int height, int width, int modes1, int modes2,
                                     scx_stream_t stream);
 
+/* Element types of the tensors below.  A complex64 tensor is given as SCX_FLOAT32 with twice
+ * its count. */
+#define SCX_FLOAT32 0
+#define SCX_BFLOAT16 1
+#define SCX_FLOAT16 2
+
+/* Global gradient norm over a list of tensors, and clipping by it.  No counterpart in the
+ * reference, whose training loop does not clip (fno_ns/train_official.py:56-154).
+ *   scx_grad_norm   *norm = sqrt(sum of squares of every element of every tensor)
+ *   scx_grad_clip   the same, then every element is multiplied by min(1, max_norm/(*norm + 1e-6))
+ * The arrays are host arrays of n_tensors entries (device address, element count, SCX_* type),
+ * read before the call returns; they travel as kernel parameters, so nothing is copied to the
+ * device and the call can be captured.  Tensors are dense runs of elements, aligned to their
+ * element size, of any count (0 included) and any mix of types; those of scx_grad_clip must not
+ * overlap.  Sums are held in 64 bits and added in a fixed order: results are bitwise repeatable
+ * on one device.  A norm that is not finite propagates (an infinite one scales by 0, so infinite
+ * elements become NaN; a NaN one makes every element NaN).  max_norm >= 0.
+ * norm: one float in device memory.  workspace: device memory of
+ * scx_grad_norm_workspace_size() bytes, 16-byte aligned, in use until the call's kernels end. */
+size_t scx_grad_norm_workspace_size(int n_tensors);
+int scx_grad_norm(int n_tensors, const void* const* tensors, const long long* counts,
+                  const int* dtypes, float* norm, void* workspace, size_t workspace_bytes,
+                  scx_stream_t stream);
+int scx_grad_clip(int n_tensors, void* const* tensors, const long long* counts, const int* dtypes,
+                  double max_norm, float* norm, void* workspace, size_t workspace_bytes,
+                  scx_stream_t stream);
+
+/* One Adam step over a list of tensors (the torch.optim.Adam of fno_ns/train_official.py:56-154),
+ * optionally with the gradients clipped on the way in: with norm != NULL, g is multiplied by
+ * min(1, max_norm/(N + 1e-6)) as it is read, N = the global norm of all gradients (left in
+ * *norm); the gradients themselves are not written.  given_norm (norm then NULL): clip by this
+ * float in device memory instead, the norm of a larger set (several lists, several ranks).
+ *   t = ++steps[i];  g' = c g (+ weight_decay p);  m = b1 m + (1-b1) g';  v = b2 v + (1-b2) g'^2
+ *   p = p (1 - lr weight_decay, where decoupled) - lr/(1-b1^t) m / (sqrt(v/(1-b2^t)) + eps)
+ * params and grads share their type and count per tensor; the moments are fp32 whatever that
+ * type is, and p is computed in fp32 and rounded once.  steps: one float in device memory per
+ * tensor (so a replayed graph advances).  lr_device: NULL, or one float in device memory that
+ * is read in place of lr.  Host arrays and addresses as above; params, moments and steps must
+ * not overlap one another.  workspace: scx_adam_workspace_size() bytes, 16-byte aligned. */
+size_t scx_adam_workspace_size(int n_tensors);
+int scx_adam_step(int n_tensors, void* const* params, const void* const* grads,
+                  float* const* exp_avgs, float* const* exp_avg_sqs, float* const* steps,
+                  const long long* counts, const int* dtypes, double lr, const float* lr_device,
+                  double beta1, double beta2, double eps, double weight_decay, int decoupled,
+                  double max_norm, const float* given_norm, float* norm, void* workspace,
+                  size_t workspace_bytes, scx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
