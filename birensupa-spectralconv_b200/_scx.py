@@ -49,6 +49,28 @@ class FnoParams(ctypes.Structure):
     ]
 
 
+class ResidualNormConfig(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_longlong), ("length", ctypes.c_longlong), ("channels", _i), ("channels_last", _i),
+        ("dtype", _i), ("weight_dtype", _i), ("kind", _i), ("gate_mode", _i), ("gate_act", _i), ("post_norm", _i),
+        ("pre_norm", _i), ("eps", ctypes.c_float), ("scale", ctypes.c_float),
+    ]
+
+
+class ResidualNormTensors(ctypes.Structure):
+    _fields_ = [
+        ("x", _p), ("y", _p), ("gate", _p), ("post_weight", _p), ("post_bias", _p), ("pre_weight", _p),
+        ("pre_bias", _p), ("scale", _p), ("r", _p), ("n", _p), ("stats", _p),
+    ]
+
+
+class ResidualNormGrads(ctypes.Structure):
+    _fields_ = [
+        ("dr", _p), ("dn", _p), ("dx", _p), ("dy", _p), ("dgate", _p), ("d_post_weight", _p), ("d_post_bias", _p),
+        ("d_pre_weight", _p), ("d_pre_bias", _p), ("d_scale", _p),
+    ]
+
+
 _SIGNATURES = {
     "scx_version": ([], _i),
     "scx_status_string": ([_i], ctypes.c_char_p),
@@ -84,6 +106,9 @@ _SIGNATURES = {
     "scx_grad_clip": ([_i, _p, _p, _p, _d, _p, _p, _sz, _p], _i),
     "scx_adam_workspace_size": ([_i], _sz),
     "scx_adam_step": ([_i, _p, _p, _p, _p, _p, _p, _p, _d, _p, _d, _d, _d, _d, _i, _d, _p, _p, _p, _sz, _p], _i),
+    "scx_residual_norm_fwd": ([_p, _p, _p], _i),
+    "scx_residual_norm_bwd_workspace_size": ([_p], _sz),
+    "scx_residual_norm_bwd": ([_p, _p, _p, _p, _sz, _p], _i),
     "scx_ipc_handle_bytes": ([], _i),
     "scx_ipc_export": ([_p, _p, ctypes.POINTER(ctypes.c_ulonglong)], _i),
     "scx_ipc_import": ([_p, ctypes.POINTER(ctypes.c_void_p)], _i),

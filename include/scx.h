@@ -357,6 +357,50 @@ int scx_adam_step(int n_tensors, void* const* params, const void* const* grads,
                   double max_norm, const float* given_norm, float* norm, void* workspace,
                   size_t workspace_bytes, scx_stream_t stream);
 
+/* The norms after and before a block, fused with the block's gate, residual scale and residual
+ * addition.  No counterpart in the reference, whose layers have no residual stream
+ * (fno_ns/model.py:87-134).  Per position, over its channels:
+ *   z = post(y),  r = x + scale act(gate) z,  n = pre(r)
+ *   post, pre: (v - mean) / sqrt(mean((v - mean)^2) + eps) * weight + bias; kind RMS: mean = 0
+ * Layouts: x, y, r, n (and a gate per element) are [batch][length][channels] (channels_last 1) or
+ * [batch][channels][length] (0); a gate per sample is [batch][channels]; weights, biases and the
+ * scale vector are [channels], of type weight_dtype (SCX_FLOAT32 or dtype).  Each may be NULL:
+ * weights and scale vector then are ones, biases zeros (at most 262144 channels); y NULL: r = x (t.r is not written), n =
+ * pre(x).  post_norm 0: z = y; pre_norm 0: no n.  The scale vector multiplies config.scale.
+ * Statistics and sums are fp32, and n is computed from the unrounded r.  stats (may be NULL in
+ * the forward): [4][batch*length] floats for the backward. */
+#define SCX_NORM_RMS 0
+#define SCX_NORM_LAYER 1
+#define SCX_GATE_NONE 0
+#define SCX_GATE_SAMPLE 1
+#define SCX_GATE_FULL 2
+#define SCX_ACT_NONE 0
+#define SCX_ACT_SIGMOID 1
+#define SCX_ACT_SILU 2
+typedef struct {
+    long long batch, length;
+    int channels, channels_last, dtype, weight_dtype, kind, gate_mode, gate_act, post_norm, pre_norm;
+    float eps, scale;
+} scx_residual_norm_config;
+typedef struct {
+    const void *x, *y, *gate, *post_weight, *post_bias, *pre_weight, *pre_bias, *scale;
+    void *r, *n;
+    float* stats;
+} scx_residual_norm_tensors;
+typedef struct {
+    const void *dr, *dn; /* gradients of r and n; either may be NULL (zero) */
+    void *dx, *dy, *dgate, *d_post_weight, *d_post_bias, *d_pre_weight, *d_pre_bias, *d_scale; /* NULL: not wanted */
+} scx_residual_norm_grads;
+int scx_residual_norm_fwd(const scx_residual_norm_config* config, const scx_residual_norm_tensors* t,
+                          scx_stream_t stream);
+/* Backward, from the forward's inputs and stats (t.r and t.n are not read).  workspace: device
+ * memory of scx_residual_norm_bwd_workspace_size() bytes, 16-byte aligned, in use until the
+ * call's kernels end; 0 on an invalid or empty configuration, for which the call is refused. */
+size_t scx_residual_norm_bwd_workspace_size(const scx_residual_norm_config* config);
+int scx_residual_norm_bwd(const scx_residual_norm_config* config, const scx_residual_norm_tensors* t,
+                          const scx_residual_norm_grads* g, void* workspace, size_t workspace_bytes,
+                          scx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
