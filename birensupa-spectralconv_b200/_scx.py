@@ -136,7 +136,8 @@ def check(status: int, what: str) -> None:
 
 
 def stream_of(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    return torch._C._cuda_getCurrentRawStream(index)  # the handle, without a Stream object around it
 
 
 def ptr(t: torch.Tensor) -> int:

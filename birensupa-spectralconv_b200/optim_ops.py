@@ -14,6 +14,7 @@ from __future__ import annotations
 import math
 from array import array
 from itertools import chain
+from operator import attrgetter
 
 import torch
 
@@ -45,25 +46,32 @@ def _overlaps_itself(t: torch.Tensor) -> bool:
     return False
 
 
+_dtype, _shape, _layout = attrgetter("dtype"), attrgetter("shape"), attrgetter("layout")
+_device_index, _is_contiguous = torch.Tensor.get_device, torch.Tensor.is_contiguous
+
+
 def _check_tensors(tensors: list, name: str) -> torch.device:
     """One CUDA device, strided layout, known element types."""
-    device = tensors[0].device
-    _check(device.type == "cuda", name, " must be CUDA tensors")
-    for t in tensors:
-        _check(t.layout is torch.strided, name, " must not be sparse")
-        _check(t.dtype in _CODES, name, " must be float32, bfloat16, float16 or complex64, got ", t.dtype)
-        _check(t.device == device, name, " must be on one device")
-    return device
+    index = tensors[0].get_device()
+    if index < 0 or set(map(_device_index, tensors)) != {index} or not _CODES.keys() >= set(map(_dtype, tensors)):
+        device = tensors[0].device
+        for t in tensors:
+            _check(t.device.type == "cuda", name, " must be CUDA tensors")
+            _check(t.dtype in _CODES, name, " must be float32, bfloat16, float16 or complex64, got ", t.dtype)
+            _check(t.device == device, name, " must be on one device")
+    _check(all([layout is torch.strided for layout in map(_layout, tensors)]), name, " must not be sparse")
+    return torch.device("cuda", index)
 
 
 def _pointers(tensors) -> array:
-    return array("Q", [t.data_ptr() for t in tensors])
+    return array("Q", map(torch.Tensor.data_ptr, tensors))
 
 
 def _described(tensors) -> tuple[array, array]:
     """(element counts, element types) of a list for the C calls."""
-    kinds = [_CODES[t.dtype] for t in tensors]
-    return (array("q", [t.numel() * k[1] for t, k in zip(tensors, kinds)]), array("i", [k[0] for k in kinds]))
+    kinds = [_CODES[d] for d in map(_dtype, tensors)]
+    return (array("q", [n * k[1] for n, k in zip(map(torch.Tensor.numel, tensors), kinds)]),
+            array("i", [k[0] for k in kinds]))
 
 
 def _address(values: array) -> int:
@@ -94,7 +102,8 @@ def grad_norm(tensors) -> torch.Tensor:
     if not tensors:
         return torch.tensor(0.0)
     device = _check_tensors(tensors, "tensors")
-    tensors = [t if t.is_contiguous() or _dense(t) else t.contiguous() for t in tensors]
+    if not all(map(_is_contiguous, tensors)):
+        tensors = [t if _dense(t) else t.contiguous() for t in tensors]
     pointers = _pointers(tensors)
     counts, kinds = _described(tensors)
     n = len(tensors)
@@ -118,7 +127,7 @@ def clip_grads_(grads, max_norm: float) -> torch.Tensor:
         return torch.tensor(0.0)
     device = _check_tensors(grads, "grads")
     flat = grads
-    if not all([g.is_contiguous() for g in grads]):
+    if not all(map(_is_contiguous, grads)):
         _check(not any(_overlaps_itself(g) for g in grads), "grads must not be expanded tensors")
         flat = [g if _dense(g) else g.contiguous() for g in grads]
     pointers = _pointers(flat)
@@ -149,6 +158,41 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
 def _same_layout(t: torch.Tensor, p: torch.Tensor) -> bool:
     return (t.is_contiguous() and p.is_contiguous()) or all(
         a == b for a, b, size in zip(t.stride(), p.stride(), p.shape) if size > 1)
+
+
+_MOMENTS = {torch.float32: torch.float32, torch.bfloat16: torch.float32, torch.float16: torch.float32,
+            torch.complex64: torch.complex64}
+
+
+def _checked_lists(params, grads, exp_avgs, exp_avg_sqs, steps, device: torch.device) -> list:
+    """Checks an Adam step's lists; returns the gradients, those of another layout than their
+    parameter's (or lazily conjugated or negated) copied to it."""
+    kinds, shapes = list(map(_dtype, params)), list(map(_shape, params))
+    moments = [_MOMENTS[k] for k in kinds]
+    _check(list(map(_dtype, grads)) == kinds and list(map(_shape, grads)) == shapes
+           and all([layout is torch.strided for layout in map(_layout, grads)]),
+           "a gradient must have its parameter's type and shape")
+    _check(list(map(_dtype, exp_avgs)) == moments and list(map(_dtype, exp_avg_sqs)) == moments
+           and list(map(_shape, exp_avgs)) == shapes and list(map(_shape, exp_avg_sqs)) == shapes,
+           "moments must be float32 (complex64 for a complex parameter), of their parameter's shape")
+    _check(set(map(_dtype, steps)) == {torch.float32} and set(map(torch.Tensor.numel, steps)) == {1},
+           "steps must be single float32 values")
+    _check(set(map(_device_index, chain(grads, exp_avgs, exp_avg_sqs, steps))) == {device.index},
+           "gradients, moments and steps must be on the params' device")
+    if torch.complex64 in kinds:
+        _check(not any(map(torch.Tensor.is_conj, chain(params, exp_avgs, exp_avg_sqs))),
+               "params and moments must not be conjugate views")
+    _check(not any(map(torch.Tensor.is_neg, chain(params, exp_avgs, exp_avg_sqs))),
+           "params and moments must not be negated views")
+    copied = [g.is_conj() or g.is_neg() for g in grads]
+    if not all(map(_is_contiguous, chain(params, grads, exp_avgs, exp_avg_sqs))):
+        for p, m, v in zip(params, exp_avgs, exp_avg_sqs):
+            _check(_dense(p) and _same_layout(m, p) and _same_layout(v, p),
+                   "params must be dense, and moments of their params' strides")
+        copied = [c or not _same_layout(g, p) for c, g, p in zip(copied, grads, params)]
+    if any(copied):
+        grads = [torch.empty_like(p).copy_(g) if c else g for c, g, p in zip(copied, grads, params)]
+    return grads
 
 
 @torch.no_grad()
@@ -194,26 +238,7 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     if total_norm is not None:
         _check(total_norm.dtype == torch.float32 and total_norm.numel() == 1 and total_norm.device == device,
                "total_norm must be one float32 value on the params' device")
-    for i, (p, g, m, v, t) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs, steps)):
-        _check(g.dtype == p.dtype and g.shape == p.shape and g.device == device and g.layout is torch.strided,
-               "a gradient must have its parameter's type, shape and device")
-        kind = torch.complex64 if p.dtype is torch.complex64 else torch.float32
-        _check(m.dtype is kind and v.dtype is kind and m.shape == p.shape and v.shape == p.shape
-               and m.device == device and v.device == device, "moments must be ", kind,
-               " of their parameter's shape and device")
-        _check(t.dtype is torch.float32 and t.numel() == 1 and t.device == device,
-               "steps must be single float32 values on the params' device")
-        if not (p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
-            _check(_dense(p) and _same_layout(m, p) and _same_layout(v, p),
-                   "params must be dense, and moments of their params' strides")
-            if not _same_layout(g, p):
-                grads[i] = torch.empty_like(p).copy_(g)
-        if p.dtype is torch.complex64:
-            _check(not (p.is_conj() or m.is_conj() or v.is_conj()), "params and moments must not be conjugate views")
-            if g.is_conj():
-                grads[i] = torch.empty_like(p).copy_(g)
-        if g.is_neg():
-            grads[i] = torch.empty_like(p).copy_(g)
+    grads = _checked_lists(params, grads, exp_avgs, exp_avg_sqs, steps, device)
     arrays = [_pointers(v) for v in (params, grads, exp_avgs, exp_avg_sqs, steps)]
     counts, kinds = _described(params)
     norm = torch.empty((), dtype=torch.float32, device=device) if clip and total_norm is None else None

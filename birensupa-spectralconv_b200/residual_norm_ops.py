@@ -112,49 +112,61 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *, pre_weight:
     Tensors that are not contiguous are copied first.  Statistics and sums are float32; r and n are
     rounded once, n from the unrounded r.
     """
-    _check(x.dim() >= 2, "x must have at least 2 dimensions, got ", tuple(x.shape))
-    _check(dim in (1, -1, x.dim() - 1), "dim must be 1 or -1, got ", dim)
+    shape, dtype, device = x.shape, x.dtype, x.device
+    rank = len(shape)
+    # the messages are only put together on failure: a single-token call is as long as its checks
+    if rank < 2:
+        _check(False, "x must have at least 2 dimensions, got ", tuple(shape))
+    if dim != 1 and dim != -1 and dim != rank - 1:
+        _check(False, "dim must be 1 or -1, got ", dim)
     _check(x.is_cuda, "x must be a CUDA tensor")
-    _check(x.dtype in _TYPES, "x must be float32, bfloat16 or float16, got ", x.dtype)
-    _check(kind in _KINDS, "kind must be 'rms' or 'layer', got ", kind)
-    _check(gate_activation in _ACTIVATIONS, "gate_activation must be 'none', 'sigmoid' or 'silu', got ", gate_activation)
+    if dtype not in _TYPES:
+        _check(False, "x must be float32, bfloat16 or float16, got ", dtype)
+    if kind not in _KINDS:
+        _check(False, "kind must be 'rms' or 'layer', got ", kind)
+    if gate_activation not in _ACTIVATIONS:
+        _check(False, "gate_activation must be 'none', 'sigmoid' or 'silu', got ", gate_activation)
     eps = float(eps)
-    _check(math.isfinite(eps) and eps >= 0.0, "eps must be finite and not negative, got ", eps)
-    _check(y is not None or (gate is None and scale is None and post_weight is None and post_bias is None),
-           "gate, scale, post_weight and post_bias need y")
+    if not 0.0 <= eps < math.inf:
+        _check(False, "eps must be finite and not negative, got ", eps)
+    last = dim != 1 or rank == 2
+    channels = shape[-1] if last else shape[1]
+    if not 0 < channels <= 262144:
+        _check(False, "x must have 1 to 262144 channels, got ", channels)
+    if y is None:
+        _check(gate is None and scale is None and post_weight is None and post_bias is None,
+               "gate, scale, post_weight and post_bias need y")
+        _check(pre_norm, "nothing to compute: no y and no pre_norm")
+    elif y.shape != shape or y.dtype != dtype or y.device != device:
+        _check(False, "y must have x's shape, type and device")
     _check(post_norm or (post_weight is None and post_bias is None), "post_weight and post_bias need post_norm")
     _check(pre_norm or (pre_weight is None and pre_bias is None), "pre_weight and pre_bias need pre_norm")
-    _check(y is not None or pre_norm, "nothing to compute: no y and no pre_norm")
-    last = dim != 1 or x.dim() == 2
-    channels = x.shape[-1] if last else x.shape[1]
-    _check(0 < channels <= 262144, "x must have 1 to 262144 channels, got ", channels)
-    batch = x.shape[0]
+    batch = shape[0]
     length = x.numel() // (batch * channels) if batch else 0
     number = 1.0
     if scale is not None and not isinstance(scale, torch.Tensor):
         number, scale = float(scale), None
-        _check(math.isfinite(number), "scale must be finite, got ", number)
-    if y is not None:
-        _check(y.shape == x.shape and y.dtype == x.dtype and y.device == x.device,
-               "y must have x's shape, type and device")
+        if not math.isfinite(number):
+            _check(False, "scale must be finite, got ", number)
     mode = 0
     if gate is not None:
-        _check(gate.dtype == x.dtype and gate.device == x.device, "gate must have x's type and device")
-        mode = 2 if gate.shape == x.shape else 1
-        _check(mode == 2 or tuple(gate.shape) == (batch, channels), "gate must have the shape of x or ",
-               (batch, channels), ", got ", tuple(gate.shape))
+        _check(gate.dtype == dtype and gate.device == device, "gate must have x's type and device")
+        mode = 2 if gate.shape == shape else 1
+        if mode == 1 and gate.shape != (batch, channels):
+            _check(False, "gate must have the shape of x or ", (batch, channels), ", got ", tuple(gate.shape))
     wide = None
     vectors = (post_weight, post_bias, pre_weight, pre_bias, scale)
     for v in vectors:
         if v is not None:
-            _check(v.dim() == 1 and v.shape[0] == channels and v.device == x.device,
-                   "weights, biases and scale must be [", channels, "] on x's device")
-            _check(v.dtype in (torch.float32, x.dtype) and wide in (None, v.dtype),
-                   "weights, biases and scale must all be float32 or all ", x.dtype)
-            wide = v.dtype
-    config = _scx.ResidualNormConfig(batch, length, channels, int(last), _TYPES[x.dtype],
+            if v.shape != (channels,) or v.device != device:
+                _check(False, "weights, biases and scale must be [", channels, "] on x's device")
+            if v.dtype is not wide:
+                _check(wide is None and (v.dtype is torch.float32 or v.dtype is dtype),
+                       "weights, biases and scale must all be float32 or all of x's type")
+                wide = v.dtype
+    config = _scx.ResidualNormConfig(batch, length, channels, last, _TYPES[dtype],
                                      _TYPES[wide or torch.float32], _KINDS[kind], mode,
-                                     _ACTIVATIONS[gate_activation], int(post_norm), int(pre_norm), eps, number)
+                                     _ACTIVATIONS[gate_activation], bool(post_norm), bool(pre_norm), eps, number)
     wanted = torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in (x, y, gate, *vectors)])
     args = [t if t is None or t.is_contiguous() else t.contiguous() for t in (x, y, gate, *vectors)]
     if wanted:
