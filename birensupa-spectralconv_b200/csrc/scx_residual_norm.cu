@@ -19,81 +19,16 @@
 //
 // A forward has to read x, y (and a gate per element) and write r, n; a backward has to read x, y,
 // gate, dr, dn and write dx, dy, dgate: about 3 operations per byte, bound by HBM.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <algorithm>
 #include <cmath>
-#include <cstdint>
 
 #include "scx.h"
 #include "scx_internal.h"
+#include "scx_residual_norm.cuh"
 
 namespace {
 
-enum : int { kF32 = 0, kBf16 = 1, kF16 = 2 };
-enum : int { kRms = 0, kLayer = 1 };
-enum : int { kGateNone = 0, kGateSample = 1, kGateFull = 2 };
-enum : int { kActNone = 0, kActSigmoid = 1, kActSilu = 2 };
-
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ void from_f32(float& o, float v) { o = v; }
-__device__ __forceinline__ void from_f32(__nv_bfloat16& o, float v) { o = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void from_f32(__half& o, float v) { o = __float2half_rn(v); }
-
-// A call's shapes, options and addresses, as a kernel parameter.
-struct Problem {
-    long long batch, length, positions;  // positions = batch * length
-    int channels;
-    int channels_last;
-    int kind, gate_mode, act;
-    int post, pre;  // whether the norm after the block, and the one before the next, is taken
-    int wide;       // weights are fp32 rather than the tensors' type
-    float eps, inv_c, scale;
-    const void *x, *y, *gate, *post_w, *post_b, *pre_w, *pre_b, *scale_w;
-    void *r, *n;
-    float* stats;  // [4][positions]: post mean, post rho, pre mean, pre rho
-    const void *dr, *dn;
-    void *dx, *dy, *dgate, *d_post_w, *d_post_b, *d_pre_w, *d_pre_b, *d_scale;
-    int sums;        // whether any gradient summed over positions is wanted
-    float* means;    // [2][positions]: mean(dn w'), mean(dn w' k)
-    float* partial;  // [blocks][kSums][channels]
-    float* items;    // [batch * chunks][channels]: sums of t z over a chunk of a sample's positions
-    int chunks;      // chunks of positions per sample
-    int parts;       // blocks that wrote partials
-};
-
-// Order of the sums over positions in `partial`.
-enum : int { kDPreW = 0, kDPreB = 1, kDPostW = 2, kDPostB = 3, kDScale = 4, kSums = 5 };
-
-template <typename T>
-__device__ __forceinline__ float weight(const void* w, int c, bool wide, float other) {
-    if (w == nullptr) return other;
-    return wide ? static_cast<const float*>(w)[c] : to_f32(static_cast<const T*>(w)[c]);
-}
-
-template <typename T>
-__device__ __forceinline__ void store_weight(void* w, int c, bool wide, float v) {
-    if (wide) static_cast<float*>(w)[c] = v;
-    else from_f32(static_cast<T*>(w)[c], v);
-}
-
-// act(g) and its derivative.
-__device__ __forceinline__ float activate(float g, int act, float& slope) {
-    if (act == kActNone) {
-        slope = 1.f;
-        return g;
-    }
-    const float s = 1.f / (1.f + expf(-g));
-    if (act == kActSilu) {
-        slope = s * (1.f + g * (1.f - s));
-        return g * s;
-    }
-    slope = s * (1.f - s);
-    return s;
-}
+using namespace scx_rn;
 
 // ---------------------------------------------------------------------------- any shape
 //
@@ -302,10 +237,8 @@ __global__ void __launch_bounds__(kAnyThreads) any_backward_kernel(const __grid_
     }
 }
 
-__device__ __forceinline__ long long chunk_begin(const Problem& p, int chunk) { return p.length * chunk / p.chunks; }
-
-// The sums over positions: a block takes one group of tc channels and a contiguous range of the
-// (sample, chunk) items; every item's sum of t z goes to `items`, the rest to `partial`.
+// The sums over positions: a block takes one group of tc channels and its share of the tiles (tp
+// positions of one sample each).
 template <typename T>
 __global__ void __launch_bounds__(kAnyThreads) any_sums_kernel(const __grid_constant__ Problem p, Split s) {
     __shared__ float red[kAnyThreads];
@@ -313,9 +246,7 @@ __global__ void __launch_bounds__(kAnyThreads) any_sums_kernel(const __grid_cons
     const int c = blockIdx.y * s.tc + at.c;
     const bool live = c < p.channels;
     const size_t sc = channel_stride(p);
-    const long long count = p.batch * p.chunks;
-    const long long from = count * blockIdx.x / gridDim.x, to = count * (blockIdx.x + 1) / gridDim.x;
-    auto over_positions = [&](float v) {  // the sum over the positions' threads, in thread at.p = 0
+    auto over_positions = [&](float v) {  // the sum over the positions' threads
         float* column = red + at.c * s.tp;
         __syncthreads();
         column[at.p] = v;
@@ -327,11 +258,13 @@ __global__ void __launch_bounds__(kAnyThreads) any_sums_kernel(const __grid_cons
         return column[0];
     };
     float sum[kSums] = {};
-    for (long long item = from; item < to; ++item) {
-        const long long sample = item / p.chunks;
-        const int chunk = static_cast<int>(item % p.chunks);
-        const long long begin = chunk_begin(p, chunk), end = chunk_begin(p, chunk + 1);
-        float tz = 0.f;
+    long long tile = tile_begin(p, blockIdx.x);
+    const long long last = tile_begin(p, blockIdx.x + 1);
+    while (tile < last) {
+        const long long sample = tile / p.tiles_per_sample;
+        const long long stop = min(last, (sample + 1) * p.tiles_per_sample);
+        const long long begin = (tile - sample * p.tiles_per_sample) * s.tp;
+        const long long end = min(p.length, (stop - sample * p.tiles_per_sample) * s.tp);
         for (long long l = begin + at.p; live && l < end; l += s.tp) {
             const long long q = sample * p.length + l;
             const size_t e = first_element(p, q) + c * sc;
@@ -345,16 +278,18 @@ __global__ void __launch_bounds__(kAnyThreads) any_sums_kernel(const __grid_cons
                 sum[kDPreW] = fmaf(dn, k, sum[kDPreW]);
                 sum[kDPreB] += dn;
             }
-            const float dz = t * v.scale * v.a;
-            sum[kDPostW] = fmaf(dz, v.h, sum[kDPostW]);
-            sum[kDPostB] += dz;
-            sum[kDScale] = fmaf(t * v.a, v.z, sum[kDScale]);
-            tz = fmaf(t, v.z, tz);
+            const float ta = p.slots ? t : t * v.a;
+            sum[kTah] = fmaf(ta, v.h, sum[kTah]);
+            sum[kTa] += ta;
         }
-        if (p.items) {
-            const float total = over_positions(tz);
-            if (live && at.p == 0) p.items[static_cast<size_t>(item) * p.channels + c] = total;
+        if (p.slots) {
+            for (int k = 0; k < 2; ++k) {
+                const float total = over_positions(sum[kTah + k]);
+                if (live && at.p == 0) slot_of(p, blockIdx.x, sample)[static_cast<size_t>(k) * p.channels + c] = total;
+                sum[kTah + k] = 0.f;
+            }
         }
+        tile = stop;
     }
     for (int k = 0; k < kSums; ++k) {
         const float total = over_positions(sum[k]);
@@ -365,47 +300,69 @@ __global__ void __launch_bounds__(kAnyThreads) any_sums_kernel(const __grid_cons
 
 // ---------------------------------------------------------------------------- the last sums
 
-// Adds the blocks' partials per channel (64-bit, in block order), and the items of each sample into
-// the gradient of its gate.  Grid (channels / 32, kSums + gate rows), block 32 x 8.
+constexpr int kFinishRows = 32;
+
+// Adds the blocks' partials per channel (in 64 bits and a fixed order), and the slots of each sample
+// into the gradient of its gate.  Grid (channels / 32, 2): the norm before the next block, then
+// the norm after the block, the scale and the gate.  Block 32 channels x kFinishRows.
 template <typename T>
-__global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Problem p) {
-    __shared__ double red[8][33];
+__global__ void __launch_bounds__(32 * kFinishRows) finish_kernel(const __grid_constant__ Problem p) {
+    __shared__ double red[2][kFinishRows][33];
+    grid_dep_wait();
     const int lane = threadIdx.x % 32, row = threadIdx.x / 32;
     const int c = blockIdx.x * 32 + lane;
-    if (blockIdx.y < kSums) {
-        void* const outs[kSums] = {p.d_pre_w, p.d_pre_b, p.d_post_w, p.d_post_b, p.d_scale};
-        void* out = outs[blockIdx.y];
-        if (out == nullptr) return;
-        double sum = 0.0;
-        if (c < p.channels)
-            for (int k = row; k < p.parts; k += 8)
-                sum += p.partial[(static_cast<size_t>(k) * kSums + blockIdx.y) * p.channels + c];
-        red[row][lane] = sum;
-        __syncthreads();
-        if (row == 0 && c < p.channels) {
-            for (int k = 1; k < 8; ++k) sum += red[k][lane];
-            if (blockIdx.y == kDScale) sum *= p.scale;
-            store_weight<T>(out, c, p.wide, static_cast<float>(sum));
+    const bool live = c < p.channels;
+    const bool second = blockIdx.y == 1;
+    const float w = live ? weight<T>(p.post_w, c, p.wide, 1.f) : 0.f, b = live ? weight<T>(p.post_b, c, p.wide, 0.f) : 0.f;
+    const float scale = p.scale * (live ? weight<T>(p.scale_w, c, p.wide, 1.f) : 0.f);
+    double s0 = 0.0, s1 = 0.0;
+    if (live && second && p.slots) {
+        for (long long s = row; s < p.batch; s += kFinishRows) {
+            double th = 0.0, t = 0.0;
+            const long long to = block_of_tile(p, (s + 1) * p.tiles_per_sample - 1);
+            for (long long k = block_of_tile(p, s * p.tiles_per_sample); k <= to; ++k) {
+                const float* slot = slot_of(p, k, s);
+                th += slot[c];
+                t += slot[static_cast<size_t>(p.channels) + c];
+            }
+            const size_t g = static_cast<size_t>(s) * p.channels + c;
+            float slope;
+            const float a = activate(to_f32(static_cast<const T*>(p.gate)[g]), p.act, slope);
+            if (p.dgate)
+                from_f32(static_cast<T*>(p.dgate)[g], static_cast<float>(w * th + b * t) * scale * slope);
+            s0 += a * th;
+            s1 += a * t;
         }
-        return;
+    } else if (live) {
+        const float* from = p.partial + static_cast<size_t>(second ? kTah : kDPreW) * p.channels + c;
+#pragma unroll 4
+        for (int k = row; k < p.parts; k += kFinishRows) {
+            const float* at = from + static_cast<size_t>(k) * kSums * p.channels;
+            s0 += at[0];
+            s1 += at[p.channels];
+        }
     }
-    if (c >= p.channels || p.items == nullptr) return;
-    const float scale = p.scale * weight<T>(p.scale_w, c, p.wide, 1.f);
-    for (long long b = (static_cast<long long>(blockIdx.y) - kSums) * 8 + row; b < p.batch;
-         b += (static_cast<long long>(gridDim.y) - kSums) * 8) {
-        double sum = 0.0;
-        for (int k = 0; k < p.chunks; ++k) sum += p.items[(static_cast<size_t>(b) * p.chunks + k) * p.channels + c];
-        const size_t g = static_cast<size_t>(b) * p.channels + c;
-        float slope;
-        activate(to_f32(static_cast<const T*>(p.gate)[g]), p.act, slope);
-        from_f32(static_cast<T*>(p.dgate)[g], static_cast<float>(sum) * scale * slope);
+    red[0][row][lane] = s0;
+    red[1][row][lane] = s1;
+    __syncthreads();
+    if (row != 0 || !live) return;
+    for (int k = 1; k < kFinishRows; ++k) {
+        s0 += red[0][k][lane];
+        s1 += red[1][k][lane];
+    }
+    if (!second) {
+        if (p.d_pre_w) store_weight<T>(p.d_pre_w, c, p.wide, static_cast<float>(s0));
+        if (p.d_pre_b) store_weight<T>(p.d_pre_b, c, p.wide, static_cast<float>(s1));
+    } else {
+        if (p.d_post_w) store_weight<T>(p.d_post_w, c, p.wide, static_cast<float>(scale * s0));
+        if (p.d_post_b) store_weight<T>(p.d_post_b, c, p.wide, static_cast<float>(scale * s1));
+        if (p.d_scale) store_weight<T>(p.d_scale, c, p.wide, static_cast<float>(p.scale * (w * s0 + b * s1)));
     }
 }
 
 // ---------------------------------------------------------------------------- host side
 
 constexpr int kMaxChannels = 1 << 18;  // keeps every grid within its limits
-constexpr int kMaxParts = 512;  // blocks along the positions in the sums
 
 Split split_for(const Problem& p) {
     if (!p.channels_last) return {32, kAnyThreads / 32};
@@ -418,28 +375,21 @@ Split sums_split_for(const Problem& p) {
     return p.channels_last ? Split{kAnyThreads / 32, 32} : Split{32, kAnyThreads / 32};
 }
 
-// Chunks per sample: enough items to give every block work, none shorter than 32 positions.
-int chunks_for(long long batch, long long length) {
-    const long long want = (kMaxParts + batch - 1) / batch;
-    return static_cast<int>(std::max(1LL, std::min(want, length / 32)));
-}
-
 size_t align256(size_t b) { return (b + 255) / 256 * 256; }
 
 struct Layout {
-    size_t means, partial, items, total;
+    size_t means, partial, slots, total;
 };
 
 Layout layout_of(const scx_residual_norm_config& c) {
     const size_t positions = static_cast<size_t>(c.batch) * static_cast<size_t>(c.length);
-    const int chunks = chunks_for(c.batch, c.length);
     Layout l;
     l.means = 0;
     l.partial = align256(positions * 2 * sizeof(float));
-    l.items = l.partial + align256(static_cast<size_t>(kMaxParts) * kSums * c.channels * sizeof(float));
-    l.total = l.items + (c.gate_mode == kGateSample
-                             ? align256(static_cast<size_t>(c.batch) * chunks * c.channels * sizeof(float))
-                             : 0);
+    l.slots = l.partial + align256(static_cast<size_t>(max_parts(c.channels)) * kSums * c.channels * sizeof(float));
+    l.total = l.slots;
+    if (c.gate_mode == kGateSample)
+        l.total += align256((static_cast<size_t>(max_parts(c.channels)) + static_cast<size_t>(c.batch)) * 2 * c.channels * sizeof(float));
     return l;
 }
 
@@ -487,6 +437,16 @@ Problem problem_of(const scx_residual_norm_config& c, const scx_residual_norm_te
     p.r = t.r;
     p.n = t.n;
     p.stats = t.stats;
+    // the same memory under a simpler description: one position per sample makes the layouts and the
+    // gates one; without a gate per sample, tokens do not know of samples
+    if (p.length == 1) {
+        p.channels_last = 1;
+        if (p.gate_mode == kGateSample) p.gate_mode = kGateFull;
+    }
+    if (p.channels_last && p.gate_mode != kGateSample) {
+        p.batch = 1;
+        p.length = p.positions;
+    }
     return p;
 }
 
@@ -504,25 +464,33 @@ int grid_for(long long work) {
 
 template <typename T>
 cudaError_t forward(const Problem& p, cudaStream_t s) {
+    const cudaError_t e = p.channels_last ? token_forward<T>(p, s) : field_forward<T>(p, s);
+    if (e != cudaErrorNotSupported) return e;
     const Split split = split_for(p);
     any_forward_kernel<T><<<grid_for((p.positions + split.tp - 1) / split.tp), kAnyThreads, 0, s>>>(p, split);
     return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t backward(Problem& p, cudaStream_t s) {
+cudaError_t any_backward(Problem& p, cudaStream_t s) {
     const Split split = split_for(p);
     any_backward_kernel<T><<<grid_for((p.positions + split.tp - 1) / split.tp), kAnyThreads, 0, s>>>(p, split);
-    cudaError_t e = cudaGetLastError();
+    const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || !p.sums) return e;
     const Split sums = sums_split_for(p);
-    p.parts = static_cast<int>(std::min<long long>(kMaxParts, p.batch * p.chunks));
+    p.tiles_per_sample = (p.length + sums.tp - 1) / sums.tp;
+    p.tiles = p.batch * p.tiles_per_sample;
+    p.parts = static_cast<int>(std::min<long long>(std::min(max_parts(p.channels), 512), p.tiles));
     any_sums_kernel<T><<<dim3(p.parts, (p.channels + sums.tc - 1) / sums.tc), kAnyThreads, 0, s>>>(p, sums);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    const int gates = p.items ? static_cast<int>(std::min<long long>(1024, (p.batch + 7) / 8)) : 0;
-    finish_kernel<T><<<dim3((p.channels + 31) / 32, kSums + gates), 256, 0, s>>>(p);
     return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t backward(Problem& p, cudaStream_t s) {
+    cudaError_t e = p.channels_last ? token_backward<T>(p, s) : field_backward<T>(p, s);
+    if (e == cudaErrorNotSupported) e = any_backward<T>(p, s);
+    if (e != cudaSuccess || !p.sums) return e;
+    return scx::launch_chained(finish_kernel<T>, dim3((p.channels + 31) / 32, 2), dim3(32 * kFinishRows), 0, s, p);
 }
 
 }  // namespace
@@ -578,9 +546,9 @@ extern "C" int scx_residual_norm_bwd(const scx_residual_norm_config* cfg, const 
     char* ws = static_cast<char*>(workspace);
     p.means = reinterpret_cast<float*>(ws + l.means);
     p.partial = reinterpret_cast<float*>(ws + l.partial);
-    p.chunks = chunks_for(cfg->batch, cfg->length);
-    if (p.gate_mode == kGateSample && p.dgate) p.items = reinterpret_cast<float*>(ws + l.items);
-    p.sums = p.items || p.d_post_w || p.d_post_b || p.d_pre_w || p.d_pre_b || p.d_scale;
+    const bool of_y = p.d_post_w || p.d_post_b || p.d_scale || (p.gate_mode == kGateSample && p.dgate);
+    if (p.gate_mode == kGateSample && of_y) p.slots = reinterpret_cast<float*>(ws + l.slots);
+    p.sums = of_y || p.d_pre_w || p.d_pre_b;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     try {
         if (cfg->dtype == kF32) return backward<float>(p, s);

@@ -1,0 +1,141 @@
+// What the residual-norm kernels share: a call's description, loads and stores by type, the gate's
+// activation, and how a backward's blocks split the positions.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include <cuda_runtime.h>
+
+namespace scx_rn {
+
+enum : int { kF32 = 0, kBf16 = 1, kF16 = 2 };
+enum : int { kRms = 0, kLayer = 1 };
+enum : int { kGateNone = 0, kGateSample = 1, kGateFull = 2 };
+enum : int { kActNone = 0, kActSigmoid = 1, kActSilu = 2 };
+
+// A call's shapes, options and addresses, as a kernel parameter.
+struct Problem {
+    long long batch, length, positions;  // positions = batch * length
+    int channels;
+    int channels_last;
+    int kind, gate_mode, act;
+    int post, pre;  // whether the norm after the block, and the one before the next, is taken
+    int wide;       // weights are fp32 rather than the tensors' type
+    float eps, inv_c, scale;
+    const void *x, *y, *gate, *post_w, *post_b, *pre_w, *pre_b, *scale_w;
+    void *r, *n;
+    float* stats;  // [4][positions]: post mean, post rho, pre mean, pre rho
+    const void *dr, *dn;
+    void *dx, *dy, *dgate, *d_post_w, *d_post_b, *d_pre_w, *d_pre_b, *d_scale;
+    int sums;        // whether any gradient summed over positions is wanted
+    float* means;    // [2][positions]: mean(dn w'), mean(dn w' k); any-shape kernels only
+    float* partial;  // [parts][kSums][channels]
+    float* slots;    // [parts + batch][2][channels], with a gate per sample whose sums are wanted
+    long long tiles, tiles_per_sample;  // a tile: some positions of one sample
+    int parts;                          // blocks that share the tiles
+};
+
+// The sums over positions that a backward's blocks leave per channel.  With a = act(gate):
+//   dw' = sum dn k, db' = sum dn, and from A = sum t a h, B = sum t a:
+//   dw = scale A, db = scale B, dscale = w A + b B (z = w h + b), dgate of a sample, whose a is
+//   constant, from sum t h and sum t over its positions.
+// With a gate per sample the last two are kept per sample, without a, in `slots`.
+enum : int { kDPreW = 0, kDPreB = 1, kTah = 2, kTa = 3, kSums = 4 };
+
+// Block b of a backward takes the tiles [tile_begin(b), tile_begin(b + 1)), in order.
+__host__ __device__ __forceinline__ long long tile_begin(const Problem& p, long long b) {
+    return p.tiles * b / p.parts;
+}
+
+// The block that has tile t: the largest b with tile_begin(b) <= t.
+__host__ __device__ __forceinline__ long long block_of_tile(const Problem& p, long long t) {
+    return ((t + 1) * p.parts - 1) / p.tiles;
+}
+
+// Where block b keeps its sums over its positions of sample s: b + s grows by one with either, so
+// no two (block, sample) pairs that meet share a slot.
+__device__ __forceinline__ float* slot_of(const Problem& p, long long b, long long s) {
+    return p.slots + static_cast<size_t>(b + s) * 2 * p.channels;
+}
+
+__device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ void from_f32(float& o, float v) { o = v; }
+__device__ __forceinline__ void from_f32(__nv_bfloat16& o, float v) { o = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void from_f32(__half& o, float v) { o = __float2half_rn(v); }
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+    T v[V];
+};
+
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> load_vec(const void* p, size_t e) {
+    return *reinterpret_cast<const Vec<T, V>*>(static_cast<const T*>(p) + e);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(void* p, size_t e, const Vec<T, V>& v) {
+    *reinterpret_cast<Vec<T, V>*>(static_cast<T*>(p) + e) = v;
+}
+
+template <typename T>
+__device__ __forceinline__ float weight(const void* w, int c, bool wide, float other) {
+    if (w == nullptr) return other;
+    return wide ? static_cast<const float*>(w)[c] : to_f32(static_cast<const T*>(w)[c]);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_weight(void* w, int c, bool wide, float v) {
+    if (wide) static_cast<float*>(w)[c] = v;
+    else from_f32(static_cast<T*>(w)[c], v);
+}
+
+// act(g) and its derivative.
+__device__ __forceinline__ float activate(float g, int act, float& slope) {
+    if (act == kActNone) {
+        slope = 1.f;
+        return g;
+    }
+    const float s = 1.f / (1.f + expf(-g));
+    if (act == kActSilu) {
+        slope = s * (1.f + g * (1.f - s));
+        return g * s;
+    }
+    slope = s * (1.f - s);
+    return s;
+}
+
+__device__ __forceinline__ float activate(float g, int act) {
+    float slope;
+    return activate(g, act, slope);
+}
+
+// Launchers of the kernels that keep a position's channels in registers.  They return
+// cudaErrorNotSupported, without a launch, for a problem they do not take.  The backward ones set
+// p.tiles, p.tiles_per_sample and p.parts for the sums that follow.
+template <typename T>
+cudaError_t field_forward(const Problem& p, cudaStream_t s);
+template <typename T>
+cudaError_t field_backward(Problem& p, cudaStream_t s);
+template <typename T>
+cudaError_t token_forward(const Problem& p, cudaStream_t s);
+template <typename T>
+cudaError_t token_backward(Problem& p, cudaStream_t s);
+
+// Most blocks that share a backward's tiles; bounds `partial` to 64 MB at any channel count.
+inline int max_parts(int channels) {
+    const int n = (1 << 22) / channels;
+    return n < 16 ? 16 : n > 1024 ? 1024 : n;
+}
+
+inline bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+}  // namespace scx_rn
