@@ -98,13 +98,16 @@ __device__ __forceinline__ void store_weight(void* w, int c, bool wide, float v)
     else from_f32(static_cast<T*>(w)[c], v);
 }
 
+// 1 / (1 + exp(-g)) to about 4 units in the last place.
+__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.f, 1.f + expf(-g)); }
+
 // act(g) and its derivative.
 __device__ __forceinline__ float activate(float g, int act, float& slope) {
     if (act == kActNone) {
         slope = 1.f;
         return g;
     }
-    const float s = 1.f / (1.f + expf(-g));
+    const float s = sigmoid(g);
     if (act == kActSilu) {
         slope = s * (1.f + g * (1.f - s));
         return g * s;
@@ -116,6 +119,72 @@ __device__ __forceinline__ float activate(float g, int act, float& slope) {
 __device__ __forceinline__ float activate(float g, int act) {
     float slope;
     return activate(g, act, slope);
+}
+
+// The same over a thread's values, the choice made once.
+template <int N>
+__device__ __forceinline__ void activate_all(float (&g)[N], int act) {
+    if (act == kActSilu) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] *= sigmoid(g[i]);
+    } else if (act == kActSigmoid) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] = sigmoid(g[i]);
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void activate_all(float (&g)[N], float (&slope)[N], int act) {
+    if (act == kActSilu) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float s = sigmoid(g[i]);
+            g[i] *= s;
+            slope[i] = fmaf(g[i], 1.f - s, s);
+        }
+    } else if (act == kActSigmoid) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            g[i] = sigmoid(g[i]);
+            slope[i] = g[i] * (1.f - g[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) slope[i] = 1.f;
+    }
+}
+
+// What a kernel's code depends on: whether there is a block's output, and a gate of which form.
+enum Mode : int { kNoBlock = 0, kPlain = 1, kSample = 2, kFull = 3 };
+
+inline int mode_of(const Problem& p) {
+    return p.y == nullptr ? kNoBlock : p.gate_mode == kGateNone ? kPlain : p.gate_mode == kGateSample ? kSample : kFull;
+}
+
+// A thread's copies from global to its own slots in shared memory, ahead of their use: they need no
+// registers while in flight, and no barrier, since nobody else reads the slots.  `live` false
+// fills with zeros.  Copies are of 4, 8 or 16 bytes; narrower vectors (kCopied false) are loaded
+// when they are used.
+template <typename V>
+constexpr bool kCopied = sizeof(V) >= 4;
+
+template <typename V>
+__device__ __forceinline__ void copy_async(V* to, const void* from, bool live) {
+    const unsigned dst = static_cast<unsigned>(__cvta_generic_to_shared(to));
+    const int bytes = live ? static_cast<int>(sizeof(V)) : 0;
+    if constexpr (sizeof(V) == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
+    else if constexpr (sizeof(V) == 8)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
+    else if constexpr (sizeof(V) == 4)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // Launchers of the kernels that keep a position's channels in registers.  They return

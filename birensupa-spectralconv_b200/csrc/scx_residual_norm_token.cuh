@@ -1,0 +1,554 @@
+// The residual-norm kernels for tokens, [position][channels]: a position's channels are neighbours,
+// so 4 to 512 threads take one position, each NV vectors of VEC channels, and every tensor is read
+// once: the values of the next positions are copied into the thread's own slots in shared memory
+// while this one's are in registers.  A thread keeps its channels from position to position, with
+// their weights, and in the backward their sums, in registers.  Statistics are sums over a
+// position's threads, by shuffles within a warp and through shared memory across warps.
+#pragma once
+
+#include <algorithm>
+
+#include "scx_internal.h"
+#include "scx_residual_norm.cuh"
+
+namespace scx_rn {
+namespace {
+
+constexpr int kMaxThreads = 512;
+constexpr int kAhead = 2;  // positions whose copies are under way while one is computed
+constexpr int kPartBytes = 2 * kMaxThreads / 32 * sizeof(float2);
+
+// A block of blockDim threads takes blockDim / tpr positions, tpr threads (a power of two) each.
+struct Team {
+    int tpr, me, row, rows;
+    float2* part;  // [2][warps]
+
+    __device__ __forceinline__ Team(int threads, float2* shared)
+        : tpr(threads), me(threadIdx.x % threads), row(threadIdx.x / threads), rows(blockDim.x / threads), part(shared) {}
+
+    // Sums over the position's threads, the same bits in all of them.  `turn` alternates between
+    // calls, so that one barrier per call is enough.
+    __device__ __forceinline__ float2 sum(float a, float b, int& turn) {
+        for (int o = min(tpr, 32) / 2; o > 0; o >>= 1) {
+            a += __shfl_xor_sync(0xffffffffu, a, o);
+            b += __shfl_xor_sync(0xffffffffu, b, o);
+        }
+        if (tpr <= 32) return make_float2(a, b);
+        float2* now = part + turn * (kMaxThreads / 32);
+        turn ^= 1;
+        if (threadIdx.x % 32 == 0) now[threadIdx.x / 32] = make_float2(a, b);
+        __syncthreads();
+        const int warps = tpr / 32;
+        const float2* mine = now + row * warps;
+        float2 s = mine[0];
+        for (int w = 1; w < warps; ++w) {
+            s.x += mine[w].x;
+            s.y += mine[w].y;
+        }
+        return s;
+    }
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void weights(const void* w, int c, bool live, bool wide, float other, float (&out)[VEC]) {
+    if (w == nullptr || !live) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) out[i] = other;
+    } else if (wide) {
+        constexpr int kPer = VEC < 4 ? VEC : 4;
+#pragma unroll
+        for (int i = 0; i < VEC; i += kPer) {
+            const Vec<float, kPer> v = load_vec<float, kPer>(w, c + i);
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) out[i + k] = v.v[k];
+        }
+    } else {
+        const Vec<T, VEC> v = load_vec<T, VEC>(w, c);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) out[i] = to_f32(v.v[i]);
+    }
+}
+
+// Mean and 1 / sqrt(variance + eps) of a position's values; vectors that do not exist hold zeros.
+template <int VEC, int NV>
+__device__ __forceinline__ float2 statistics(const Problem& p, Team& team, const float (&v)[NV * VEC],
+                                             const bool (&on)[NV], int& turn) {
+    float mean = 0.f, s = 0.f;
+    if (p.kind == kLayer) {
+#pragma unroll
+        for (int i = 0; i < NV * VEC; ++i) s += v[i];
+        mean = team.sum(s, 0.f, turn).x * p.inv_c;
+        s = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (on[j]) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) s = fmaf(v[j * VEC + i] - mean, v[j * VEC + i] - mean, s);
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV * VEC; ++i) s = fmaf(v[i], v[i], s);
+    }
+    return make_float2(mean, 1.f / sqrtf(fmaf(team.sum(s, 0.f, turn).x, p.inv_c, p.eps)));
+}
+
+// The weights of a thread's channels, the scale taken into those of the norm after the block.
+template <typename T, int VEC, int NV>
+struct Weights {
+    float w[NV * VEC], b[NV * VEC], w2[NV * VEC];
+
+    __device__ __forceinline__ Weights(const Problem& p, const Team& team, bool block) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * team.tpr + team.me) * VEC;
+            const bool live = c < p.channels;
+            float v[VEC];
+            if (block) {
+                float scale[VEC];
+                weights<T, VEC>(p.scale_w, c, live, p.wide, 1.f, scale);
+                weights<T, VEC>(p.post ? p.post_w : nullptr, c, live, p.wide, 1.f, v);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) w[j * VEC + i] = p.scale * scale[i] * v[i];
+                weights<T, VEC>(p.post ? p.post_b : nullptr, c, live, p.wide, 0.f, v);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) b[j * VEC + i] = p.scale * scale[i] * v[i];
+            }
+            weights<T, VEC>(p.pre_w, c, live, p.wide, 1.f, v);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) w2[j * VEC + i] = v[i];
+        }
+    }
+};
+
+// A thread's slots for one tensor of one position, and how it fills and reads them.
+template <typename T, int VEC, int NV>
+struct Slots {
+    using E = Vec<T, VEC>;
+
+    static __device__ __forceinline__ void fetch(E* slot, const void* from, size_t row, const Team& team, int channels,
+                                                 bool here) {
+        if constexpr (kCopied<E>) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int c = (j * team.tpr + team.me) * VEC;
+                const bool live = here && c < channels;
+                copy_async(slot + j * blockDim.x, static_cast<const T*>(from) + (live ? row + c : 0), live);
+            }
+        }
+    }
+
+    static __device__ __forceinline__ void read(const E* slot, const void* from, size_t row, const Team& team,
+                                                int channels, bool here, float (&out)[NV * VEC]) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            E v{};
+            if constexpr (kCopied<E>) {
+                v = slot[j * blockDim.x];
+            } else {
+                const int c = (j * team.tpr + team.me) * VEC;
+                if (here && c < channels) v = load_vec<T, VEC>(from, row + c);
+            }
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) out[j * VEC + i] = to_f32(v.v[i]);
+        }
+    }
+
+    static __device__ __forceinline__ void store(void* to, size_t row, const Team& team, int channels, bool here,
+                                                 const float (&v)[NV * VEC]) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * team.tpr + team.me) * VEC;
+            E o;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) from_f32(o.v[i], v[j * VEC + i]);
+            if (here && c < channels) store_vec<T, VEC>(to, row + c, o);
+        }
+    }
+};
+
+__host__ __device__ constexpr int forward_tensors(int mode) { return mode == kNoBlock ? 1 : mode == kPlain ? 2 : 3; }
+__host__ __device__ constexpr int backward_tensors(int mode) { return mode == kNoBlock ? 3 : mode == kPlain ? 4 : 5; }
+
+// A gate per sample is read like one per element, from the sample's row: kSample and kFull are one
+// mode here.
+template <typename T, int VEC, int NV, int MODE>
+__global__ void __launch_bounds__(kMaxThreads) token_forward_kernel(const __grid_constant__ Problem p, int tpr) {
+    using F = Slots<T, VEC, NV>;
+    constexpr int N = NV * VEC, kTensors = forward_tensors(MODE);
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    auto* part = reinterpret_cast<float2*>(dynamic);
+    Team team(tpr, part);
+    const int channels = p.channels;
+    const long long groups = (p.positions + team.rows - 1) / team.rows;
+    auto* slots = reinterpret_cast<typename F::E*>(dynamic + kPartBytes) + threadIdx.x;
+    auto slot = [&](int ring, int tensor) { return slots + (ring * kTensors + tensor) * NV * blockDim.x; };
+    auto gate_row = [&](long long q) {
+        return static_cast<size_t>(p.gate_mode == kGateSample ? q / p.length : q) * channels;
+    };
+    auto fetch = [&](long long group, int ring) {
+        if (group < groups) {
+            const long long q = group * team.rows + team.row;
+            const bool here = q < p.positions;
+            const size_t row = static_cast<size_t>(q) * channels;
+            F::fetch(slot(ring, 0), p.x, row, team, channels, here);
+            if constexpr (MODE != kNoBlock) F::fetch(slot(ring, 1), p.y, row, team, channels, here);
+            if constexpr (MODE == kFull) F::fetch(slot(ring, 2), p.gate, here ? gate_row(q) : 0, team, channels, here);
+        }
+        copy_commit();
+    };
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) fetch(blockIdx.x + static_cast<long long>(k) * gridDim.x, k);
+    const Weights<T, VEC, NV> weight_of(p, team, MODE != kNoBlock);
+    bool on[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) on[j] = (j * tpr + team.me) * VEC < channels;
+    int turn = 0, ring = 0;
+    for (long long group = blockIdx.x; group < groups; group += gridDim.x) {
+        const long long q = group * team.rows + team.row;
+        const bool here = q < p.positions;
+        const size_t row = static_cast<size_t>(q) * channels;
+        const int next = ring + kAhead >= kAhead + 1 ? ring - 1 : ring + kAhead;
+        fetch(group + static_cast<long long>(kAhead) * gridDim.x, next);
+        copy_wait<kAhead>();
+        float r[N];
+        float2 st = make_float2(0.f, 1.f), st2 = st;
+        F::read(slot(ring, 0), p.x, row, team, channels, here, r);
+        if constexpr (MODE != kNoBlock) {
+            float h[N], a[N];
+            F::read(slot(ring, 1), p.y, row, team, channels, here, h);
+            if constexpr (MODE == kFull) {
+                F::read(slot(ring, 2), p.gate, here ? gate_row(q) : 0, team, channels, here, a);
+                activate_all(a, p.act);
+            }
+            if (p.post) st = statistics<VEC, NV>(p, team, h, on, turn);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float z = fmaf((h[i] - st.x) * st.y, weight_of.w[i], weight_of.b[i]);
+                r[i] = MODE == kPlain ? r[i] + z : fmaf(a[i], z, r[i]);
+            }
+            // vectors past the last channel hold -mean rho w + b: back to zero for the next statistic
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (!on[j]) {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) r[j * VEC + i] = 0.f;
+                }
+            F::store(p.r, row, team, channels, here, r);
+        }
+        if (p.pre) {
+            st2 = statistics<VEC, NV>(p, team, r, on, turn);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                float b[VEC];
+                weights<T, VEC>(p.pre_b, (j * tpr + team.me) * VEC, on[j], p.wide, 0.f, b);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i)
+                    r[j * VEC + i] = fmaf((r[j * VEC + i] - st2.x) * st2.y, weight_of.w2[j * VEC + i], b[i]);
+            }
+            F::store(p.n, row, team, channels, here, r);
+        }
+        if (p.stats && team.me == 0 && here) {
+            p.stats[q] = st.x;
+            p.stats[p.positions + q] = st.y;
+            p.stats[2 * p.positions + q] = st2.x;
+            p.stats[3 * p.positions + q] = st2.y;
+        }
+        ring = ring == kAhead ? 0 : ring + 1;
+    }
+    copy_wait<0>();
+}
+
+// Sums over a block's positions: the rows' threads of one channel are added through shared memory in
+// row order.  Every thread of the block calls it.
+template <int VEC, int NV>
+__device__ void store_sums(const Problem& p, const Team& team, float* shared, const float (&sum)[NV * VEC], float* out) {
+    if (team.rows > 1) {
+        __syncthreads();
+        const int width = team.tpr * VEC * NV;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) shared[team.row * width + (j * team.tpr + team.me) * VEC + i] = sum[j * VEC + i];
+        __syncthreads();
+        for (int c = threadIdx.x; c < p.channels; c += blockDim.x) {
+            float s = 0.f;
+            for (int r = 0; r < team.rows; ++r) s += shared[r * width + c];
+            out[c] = s;
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (j * team.tpr + team.me) * VEC;
+        if (c >= p.channels) continue;
+        Vec<float, VEC> o;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o.v[i] = sum[j * VEC + i];
+        if (p.channels % 4 == 0) {  // every array of the workspace then starts on 16 bytes
+#pragma unroll
+            for (int i = 0; i < VEC; i += (VEC < 4 ? VEC : 4))
+                *reinterpret_cast<Vec<float, (VEC < 4 ? VEC : 4)>*>(out + c + i) =
+                    *reinterpret_cast<const Vec<float, (VEC < 4 ? VEC : 4)>*>(o.v + i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+                if (c + i < p.channels) out[c + i] = o.v[i];
+        }
+    }
+}
+
+template <typename T, int VEC, int NV, int MODE>
+__global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __grid_constant__ Problem p, int tpr) {
+    using F = Slots<T, VEC, NV>;
+    constexpr int N = NV * VEC, kTensors = backward_tensors(MODE);
+    // the tensors' places in a ring slot
+    constexpr int kX = 0, kDn = 1, kDr = 2, kY = 3, kGate = 4;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    auto* part = reinterpret_cast<float2*>(dynamic);
+    grid_dep_launch();
+    Team team(tpr, part);
+    const int channels = p.channels;
+    auto* slots = reinterpret_cast<typename F::E*>(dynamic + kPartBytes) + threadIdx.x;
+    auto slot = [&](int ring, int tensor) { return slots + (ring * kTensors + tensor) * NV * blockDim.x; };
+    const long long first = tile_begin(p, blockIdx.x), last = tile_begin(p, blockIdx.x + 1);
+    const bool samples = p.tiles_per_sample != p.tiles;  // otherwise no division
+    struct At {
+        long long sample, q;
+        bool here;
+    };
+    auto at_of = [&](long long tile) {
+        const long long sample = samples ? tile / p.tiles_per_sample : 0;
+        const long long l = (tile - sample * p.tiles_per_sample) * team.rows + team.row;
+        return At{sample, sample * p.length + l, l < p.length};
+    };
+    auto fetch = [&](long long tile, int ring) {
+        if (tile < last) {
+            const At at = at_of(tile);
+            const size_t row = static_cast<size_t>(at.q) * channels;
+            if (p.dn) {
+                F::fetch(slot(ring, kX), p.x, row, team, channels, at.here);
+                F::fetch(slot(ring, kDn), p.dn, row, team, channels, at.here);
+            }
+            if (p.dr) F::fetch(slot(ring, kDr), p.dr, row, team, channels, at.here);
+            if constexpr (MODE != kNoBlock) F::fetch(slot(ring, kY), p.y, row, team, channels, at.here);
+            if constexpr (MODE == kFull)
+                F::fetch(slot(ring, kGate), p.gate,
+                         p.gate_mode == kGateSample ? static_cast<size_t>(at.sample) * channels : row, team, channels,
+                         at.here);
+        }
+        copy_commit();
+    };
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) fetch(first + k, k);
+    const Weights<T, VEC, NV> weight_of(p, team, MODE != kNoBlock);
+    float dw2[N] = {}, db2[N] = {}, tah[N] = {}, ta[N] = {};
+    int turn = 0, ring = 0;
+    for (long long tile = first; tile < last; ++tile) {
+        const At at = at_of(tile);
+        const size_t row = static_cast<size_t>(at.q) * channels;
+        const size_t gate_row = p.gate_mode == kGateSample ? static_cast<size_t>(at.sample) * channels : row;
+        float mean = 0.f, rho = 0.f, mean2 = 0.f, rho2 = 0.f;
+        if (at.here) {
+            mean = p.post ? p.stats[at.q] : 0.f;
+            rho = p.post ? p.stats[p.positions + at.q] : 1.f;
+            if (p.dn) {
+                mean2 = p.stats[2 * p.positions + at.q];
+                rho2 = p.stats[3 * p.positions + at.q];
+            }
+        }
+        fetch(tile + kAhead, ring == 0 ? kAhead : ring - 1);
+        copy_wait<kAhead>();
+        float h[N], a[N], k[N], g[N];
+        if constexpr (MODE != kNoBlock) {
+            F::read(slot(ring, kY), p.y, row, team, channels, at.here, h);
+#pragma unroll
+            for (int i = 0; i < N; ++i) h[i] = (h[i] - mean) * rho;
+            if constexpr (MODE == kFull) {
+                F::read(slot(ring, kGate), p.gate, gate_row, team, channels, at.here, a);
+                activate_all(a, p.act);
+            }
+        }
+        if (p.dn) {
+            F::read(slot(ring, kX), p.x, row, team, channels, at.here, k);
+            F::read(slot(ring, kDn), p.dn, row, team, channels, at.here, g);  // zeros where there is no channel
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if constexpr (MODE != kNoBlock) {
+                    const float z = fmaf(h[i], weight_of.w[i], weight_of.b[i]);
+                    k[i] = MODE == kPlain ? k[i] + z : fmaf(a[i], z, k[i]);
+                }
+                k[i] = (k[i] - mean2) * rho2;
+                dw2[i] = fmaf(g[i], k[i], dw2[i]);
+                db2[i] += g[i];
+                g[i] *= weight_of.w2[i];
+                s0 += g[i];
+                s1 = fmaf(g[i], k[i], s1);
+            }
+            const float2 m = team.sum(s0, s1, turn);
+            const float m1 = p.kind == kLayer ? m.x * p.inv_c : 0.f, m2 = m.y * p.inv_c;
+#pragma unroll
+            for (int i = 0; i < N; ++i) g[i] = rho2 * (g[i] - m1 - k[i] * m2);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) g[i] = 0.f;
+        }
+        if (p.dr) {
+            F::read(slot(ring, kDr), p.dr, row, team, channels, at.here, k);
+#pragma unroll
+            for (int i = 0; i < N; ++i) g[i] += k[i];
+        }
+        // g: the gradient of r; back to zero where there is no channel
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if ((j * tpr + team.me) * VEC >= channels) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) g[j * VEC + i] = 0.f;
+            }
+        if (p.dx) F::store(p.dx, row, team, channels, at.here, g);
+        if constexpr (MODE != kNoBlock) {
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float v = MODE == kPlain ? g[i] : g[i] * a[i];
+                const float kept = p.slots ? g[i] : v;
+                tah[i] = fmaf(kept, h[i], tah[i]);
+                ta[i] += kept;
+                k[i] = v * weight_of.w[i];
+                s0 += k[i];
+                s1 = fmaf(k[i], h[i], s1);
+            }
+            if (MODE == kFull && p.dgate && p.gate_mode == kGateFull) {
+                // the gate again, for its slope: registers are what this kernel is short of
+                float slope[N];
+                F::read(slot(ring, kGate), p.gate, gate_row, team, channels, at.here, a);
+                activate_all(a, slope, p.act);
+#pragma unroll
+                for (int i = 0; i < N; ++i) a[i] = g[i] * fmaf(h[i], weight_of.w[i], weight_of.b[i]) * slope[i];
+                F::store(p.dgate, row, team, channels, at.here, a);
+            }
+            if (p.dy) {
+                if (p.post) {
+                    const float2 m = team.sum(s0, s1, turn);
+                    const float m3 = p.kind == kLayer ? m.x * p.inv_c : 0.f, m4 = m.y * p.inv_c;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) k[i] = rho * (k[i] - m3 - h[i] * m4);
+                }
+                F::store(p.dy, row, team, channels, at.here, k);
+            }
+            if (p.slots && (tile + 1 == last || (tile + 1) % p.tiles_per_sample == 0)) {
+                // this ring slot has been read, and its next copies are kAhead positions away: the sums
+                // of several rows meet in the space behind the ring
+                float* meet = reinterpret_cast<float*>(slots - threadIdx.x + (kAhead + 1) * kTensors * NV * blockDim.x);
+                float* to = slot_of(p, blockIdx.x, at.sample);
+                store_sums<VEC, NV>(p, team, meet, tah, to);
+                store_sums<VEC, NV>(p, team, meet, ta, to + channels);
+#pragma unroll
+                for (int i = 0; i < N; ++i) tah[i] = ta[i] = 0.f;
+            }
+        }
+        ring = ring == kAhead ? 0 : ring + 1;
+    }
+    copy_wait<0>();
+    if (!p.sums) return;
+    float* meet = reinterpret_cast<float*>(slots - threadIdx.x + (kAhead + 1) * kTensors * NV * blockDim.x);
+    float* out = p.partial + static_cast<size_t>(blockIdx.x) * kSums * channels;
+    store_sums<VEC, NV>(p, team, meet, dw2, out + static_cast<size_t>(kDPreW) * channels);
+    store_sums<VEC, NV>(p, team, meet, db2, out + static_cast<size_t>(kDPreB) * channels);
+    store_sums<VEC, NV>(p, team, meet, tah, out + static_cast<size_t>(kTah) * channels);
+    store_sums<VEC, NV>(p, team, meet, ta, out + static_cast<size_t>(kTa) * channels);
+}
+
+// Threads per position: a power of two that covers the channels.
+int team_for(int channels, int per_thread) {
+    int tpr = 4;
+    while (tpr * per_thread < channels) tpr *= 2;
+    return tpr;
+}
+
+template <typename T, int VEC, int NV, int MODE>
+cudaError_t forward_as(const Problem& p, cudaStream_t s) {
+    const int tpr = team_for(p.channels, VEC * NV);
+    const int threads = std::max(128, tpr), rows = threads / tpr;
+    const long long groups = (p.positions + rows - 1) / rows;
+    const size_t smem = kPartBytes + (kAhead + 1) * forward_tensors(MODE) * NV * sizeof(Vec<T, VEC>) * threads;
+    int per_sm = 0;
+    const cudaError_t e =
+        scx::prepare_kernel(reinterpret_cast<const void*>(token_forward_kernel<T, VEC, NV, MODE>), smem, threads, &per_sm);
+    if (e != cudaSuccess) return e;
+    const int grid = static_cast<int>(std::min<long long>(groups, static_cast<long long>(per_sm) * scx::num_sms()));
+    token_forward_kernel<T, VEC, NV, MODE><<<grid, threads, smem, s>>>(p, tpr);
+    return cudaGetLastError();
+}
+
+template <typename T, int VEC, int NV, int MODE>
+cudaError_t backward_as(Problem& p, cudaStream_t s) {
+    const int tpr = team_for(p.channels, VEC * NV);
+    const int threads = std::max(128, tpr), rows = threads / tpr;
+    const size_t smem = kPartBytes + (kAhead + 1) * backward_tensors(MODE) * NV * sizeof(Vec<T, VEC>) * threads +
+                        (rows > 1 ? sizeof(float) * threads * VEC * NV : 0);
+    int per_sm = 0;
+    const cudaError_t e =
+        scx::prepare_kernel(reinterpret_cast<const void*>(token_backward_kernel<T, VEC, NV, MODE>), smem, threads, &per_sm);
+    if (e != cudaSuccess) return e;
+    p.tiles_per_sample = (p.length + rows - 1) / rows;
+    p.tiles = p.batch * p.tiles_per_sample;
+    p.parts = static_cast<int>(std::min<long long>(std::min(max_parts(p.channels), per_sm * scx::num_sms()), p.tiles));
+    token_backward_kernel<T, VEC, NV, MODE><<<p.parts, threads, smem, s>>>(p, tpr);
+    return cudaGetLastError();
+}
+
+// Whether rows can be moved by 16-byte accesses: whole vectors per row, every base aligned.
+template <typename T>
+bool vectors_fit(const Problem& p) {
+    const void* all[] = {p.x, p.y, p.gate_mode != kGateNone ? p.gate : nullptr, p.r, p.n, p.dr, p.dn, p.dx, p.dy,
+                         p.gate_mode == kGateFull ? p.dgate : nullptr, p.post_w, p.post_b, p.pre_w, p.pre_b, p.scale_w};
+    for (const void* a : all)
+        if (!aligned(a, 16)) return false;
+    return p.channels % (16 / static_cast<int>(sizeof(T))) == 0;
+}
+
+template <typename T, int MODE>
+cudaError_t forward_in(const Problem& p, cudaStream_t s) {
+    constexpr int VEC = 16 / static_cast<int>(sizeof(T));
+    if (vectors_fit<T>(p)) {
+        if (p.channels <= VEC * kMaxThreads) return forward_as<T, VEC, 1, MODE>(p, s);
+        if (p.channels <= 2 * VEC * kMaxThreads) return forward_as<T, VEC, 2, MODE>(p, s);
+        return cudaErrorNotSupported;
+    }
+    if (p.channels <= 4 * kMaxThreads) return forward_as<T, 1, 4, MODE>(p, s);
+    return cudaErrorNotSupported;
+}
+
+template <typename T, int MODE>
+cudaError_t backward_in(Problem& p, cudaStream_t s) {
+    constexpr int VEC = 16 / static_cast<int>(sizeof(T));
+    if (vectors_fit<T>(p)) {
+        if (p.channels <= VEC * kMaxThreads) return backward_as<T, VEC, 1, MODE>(p, s);
+        return cudaErrorNotSupported;
+    }
+    if (p.channels <= 4 * kMaxThreads) return backward_as<T, 1, 4, MODE>(p, s);
+    return cudaErrorNotSupported;
+}
+
+}  // namespace
+
+template <typename T>
+cudaError_t token_forward(const Problem& p, cudaStream_t s) {
+    switch (mode_of(p)) {
+        case kNoBlock: return forward_in<T, kNoBlock>(p, s);
+        case kPlain: return forward_in<T, kPlain>(p, s);
+        default: return forward_in<T, kFull>(p, s);
+    }
+}
+
+template <typename T>
+cudaError_t token_backward(Problem& p, cudaStream_t s) {
+    switch (mode_of(p)) {
+        case kNoBlock: return backward_in<T, kNoBlock>(p, s);
+        case kPlain: return backward_in<T, kPlain>(p, s);
+        default: return backward_in<T, kFull>(p, s);
+    }
+}
+
+}  // namespace scx_rn
