@@ -319,8 +319,8 @@ __global__ void __launch_bounds__(32 * kFinishRows) finish_kernel(const __grid_c
     if (live && second && p.slots) {
         for (long long s = row; s < p.batch; s += kFinishRows) {
             double th = 0.0, t = 0.0;
-            const long long to = block_of_tile(p, (s + 1) * p.tiles_per_sample - 1);
-            for (long long k = block_of_tile(p, s * p.tiles_per_sample); k <= to; ++k) {
+            const long long to = part_of_tile(p, (s + 1) * p.tiles_per_sample - 1);
+            for (long long k = part_of_tile(p, s * p.tiles_per_sample); k <= to; ++k) {
                 const float* slot = slot_of(p, k, s);
                 th += slot[c];
                 t += slot[static_cast<size_t>(p.channels) + c];
@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(32 * kFinishRows) finish_kernel(const __grid_c
     } else if (live) {
         const float* from = p.partial + static_cast<size_t>(second ? kTah : kDPreW) * p.channels + c;
 #pragma unroll 4
-        for (int k = row; k < p.parts; k += kFinishRows) {
+        for (int k = row; k < p.partials; k += kFinishRows) {
             const float* at = from + static_cast<size_t>(k) * kSums * p.channels;
             s0 += at[0];
             s1 += at[p.channels];
@@ -481,6 +481,7 @@ cudaError_t any_backward(Problem& p, cudaStream_t s) {
     p.tiles_per_sample = (p.length + sums.tp - 1) / sums.tp;
     p.tiles = p.batch * p.tiles_per_sample;
     p.parts = static_cast<int>(std::min<long long>(std::min(max_parts(p.channels), 512), p.tiles));
+    p.partials = p.parts;
     any_sums_kernel<T><<<dim3(p.parts, (p.channels + sums.tc - 1) / sums.tc), kAnyThreads, 0, s>>>(p, sums);
     return cudaGetLastError();
 }

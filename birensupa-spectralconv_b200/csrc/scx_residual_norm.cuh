@@ -32,10 +32,11 @@ struct Problem {
     void *dx, *dy, *dgate, *d_post_w, *d_post_b, *d_pre_w, *d_pre_b, *d_scale;
     int sums;        // whether any gradient summed over positions is wanted
     float* means;    // [2][positions]: mean(dn w'), mean(dn w' k); any-shape kernels only
-    float* partial;  // [parts][kSums][channels]
+    float* partial;  // [partials][kSums][channels]
     float* slots;    // [parts + batch][2][channels], with a gate per sample whose sums are wanted
     long long tiles, tiles_per_sample;  // a tile: some positions of one sample
-    int parts;                          // blocks that share the tiles
+    int parts;                          // blocks or warps that share the tiles
+    int partials;                       // rows of `partial`
 };
 
 // The sums over positions that a backward's blocks leave per channel.  With a = act(gate):
@@ -45,18 +46,18 @@ struct Problem {
 // With a gate per sample the last two are kept per sample, without a, in `slots`.
 enum : int { kDPreW = 0, kDPreB = 1, kTah = 2, kTa = 3, kSums = 4 };
 
-// Block b of a backward takes the tiles [tile_begin(b), tile_begin(b + 1)), in order.
+// Part b of a backward (a block, or a warp) takes the tiles [tile_begin(b), tile_begin(b + 1)), in order.
 __host__ __device__ __forceinline__ long long tile_begin(const Problem& p, long long b) {
     return p.tiles * b / p.parts;
 }
 
-// The block that has tile t: the largest b with tile_begin(b) <= t.
-__host__ __device__ __forceinline__ long long block_of_tile(const Problem& p, long long t) {
+// The part that has tile t: the largest b with tile_begin(b) <= t.
+__host__ __device__ __forceinline__ long long part_of_tile(const Problem& p, long long t) {
     return ((t + 1) * p.parts - 1) / p.tiles;
 }
 
-// Where block b keeps its sums over its positions of sample s: b + s grows by one with either, so
-// no two (block, sample) pairs that meet share a slot.
+// Where part b keeps its sums over its positions of sample s: b + s grows by one with either, so
+// no two (part, sample) pairs that meet share a slot.
 __device__ __forceinline__ float* slot_of(const Problem& p, long long b, long long s) {
     return p.slots + static_cast<size_t>(b + s) * 2 * p.channels;
 }
@@ -84,6 +85,34 @@ __device__ __forceinline__ Vec<T, V> load_vec(const void* p, size_t e) {
 template <typename T, int V>
 __device__ __forceinline__ void store_vec(void* p, size_t e, const Vec<T, V>& v) {
     *reinterpret_cast<Vec<T, V>*>(static_cast<T*>(p) + e) = v;
+}
+
+// Two fp32 values at once: sm_100a has packed fp32 arithmetic, which halves the instructions of
+// these kernels' inner loops (the token kernels in bf16 are bound by them).
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+
+__device__ __forceinline__ float2 unpack(float a, float b) { return make_float2(a, b); }
+__device__ __forceinline__ float2 unpack(__nv_bfloat16 a, __nv_bfloat16 b) {
+    return make_float2(__bfloat162float(a), __bfloat162float(b));
+}
+__device__ __forceinline__ float2 unpack(__half a, __half b) { return make_float2(__half2float(a), __half2float(b)); }
+
+__device__ __forceinline__ void pack(float& a, float& b, float2 v) {
+    a = v.x;
+    b = v.y;
+}
+__device__ __forceinline__ void pack(__nv_bfloat16& a, __nv_bfloat16& b, float2 v) {
+    const __nv_bfloat162 o = __floats2bfloat162_rn(v.x, v.y);
+    a = o.x;
+    b = o.y;
+}
+__device__ __forceinline__ void pack(__half& a, __half& b, float2 v) {
+    const __half2 o = __floats2half2_rn(v.x, v.y);
+    a = __low2half(o);
+    b = __high2half(o);
 }
 
 template <typename T>
@@ -121,36 +150,39 @@ __device__ __forceinline__ float activate(float g, int act) {
     return activate(g, act, slope);
 }
 
-// The same over a thread's values, the choice made once.
-template <int N>
-__device__ __forceinline__ void activate_all(float (&g)[N], int act) {
+// act over a thread's pairs, the choice made once.
+template <int P>
+__device__ __forceinline__ void activate_all(float2 (&g)[P], int act) {
     if (act == kActSilu) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) g[i] *= sigmoid(g[i]);
+        for (int i = 0; i < P; ++i) g[i] = mul2(g[i], make_float2(sigmoid(g[i].x), sigmoid(g[i].y)));
     } else if (act == kActSigmoid) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) g[i] = sigmoid(g[i]);
+        for (int i = 0; i < P; ++i) g[i] = make_float2(sigmoid(g[i].x), sigmoid(g[i].y));
     }
 }
 
-template <int N>
-__device__ __forceinline__ void activate_all(float (&g)[N], float (&slope)[N], int act) {
+// The same and the derivative.
+template <int P>
+__device__ __forceinline__ void activate_all(float2 (&g)[P], float2 (&slope)[P], int act) {
+    if (act == kActNone) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) slope[i] = both(1.f);
+        return;
+    }
     if (act == kActSilu) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float s = sigmoid(g[i]);
-            g[i] *= s;
-            slope[i] = fmaf(g[i], 1.f - s, s);
-        }
-    } else if (act == kActSigmoid) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            g[i] = sigmoid(g[i]);
-            slope[i] = g[i] * (1.f - g[i]);
+        for (int i = 0; i < P; ++i) {
+            const float2 s = make_float2(sigmoid(g[i].x), sigmoid(g[i].y));
+            g[i] = mul2(g[i], s);
+            slope[i] = fma2(g[i], make_float2(1.f - s.x, 1.f - s.y), s);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) slope[i] = 1.f;
+        for (int i = 0; i < P; ++i) {
+            g[i] = make_float2(sigmoid(g[i].x), sigmoid(g[i].y));
+            slope[i] = mul2(g[i], make_float2(1.f - g[i].x, 1.f - g[i].y));
+        }
     }
 }
 
@@ -199,10 +231,10 @@ cudaError_t token_forward(const Problem& p, cudaStream_t s);
 template <typename T>
 cudaError_t token_backward(Problem& p, cudaStream_t s);
 
-// Most blocks that share a backward's tiles; bounds `partial` to 64 MB at any channel count.
+// Most parts that share a backward's tiles; bounds `partial` to 64 MB at any channel count.
 inline int max_parts(int channels) {
     const int n = (1 << 22) / channels;
-    return n < 16 ? 16 : n > 1024 ? 1024 : n;
+    return n < 16 ? 16 : n > 4096 ? 4096 : n;
 }
 
 inline bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }

@@ -2,14 +2,21 @@
 // `length` elements apart, so a warp takes neighbouring positions of a few channels, and a block's
 // warps together all channels of a tile of positions.
 //
-// A thread has V neighbouring positions (one access) of kEpt channels, and every tensor is read
-// once: the next tile's values are copied into the thread's own slots in shared memory while this
-// tile's are in registers.  A warp's 32 lanes are 32/LC positions x LC channel groups; LC > 1
-// serves channel counts that would take more than 16 warps.  A statistic is a sum over a
-// position's channel groups: each group leaves its part in shared memory, one thread per position
-// adds them and leaves the result.  The layer kind's variance is not taken from sums of squares: a
-// group leaves its mean and its sum of squares about it, and the parts are joined about the common
-// mean.
+// A thread has V neighbouring positions (one access) of EPT channels, 8 values for V = 4, and every
+// tensor is read once: the next tile's values are copied into the thread's own slots in shared
+// memory while this tile's are in registers.  A warp's 32 lanes are 32/LC positions x LC channel
+// groups: LC = 2 keeps accesses of 16 bytes and warps of 4 channels, larger LC serves channel counts
+// that would take more than 16 warps.  A statistic is a sum over a position's channels: within the
+// thread, over the warp's channel groups by shuffles, and over the warps through shared memory,
+// where a few threads per position add the warps' parts.  The layer kind's variance is not taken from
+// sums of squares: a warp leaves its mean and its sum of squares about it, and the parts are joined
+// about the common mean.
+//
+// Other splits that were measured on a 16 x 64 x 256 x 256 fp32 field with a gate per element, forward
+// and backward: a thread per column of channels (no barriers, but two columns in registers leave 8
+// warps per SM: 284 us and 2.1 ms); every thread adding all warps' parts itself (one barrier instead
+// of two, but shared memory saturates: 452 and 558 us); 8-byte accesses, V = 2 and EPT = 4
+// (296 and 526 us).
 #pragma once
 
 #include <algorithm>
@@ -21,21 +28,24 @@ namespace scx_rn {
 namespace {
 
 constexpr int kMaxWarps = 16;
-constexpr int kEpt = 4;  // channels per thread
 enum : int { kPostW = 0, kPostB = 1, kPreW = 2, kPreB = 3, kVectors = 4 };
 
-template <int V, int LC>
+template <int V, int EPT, int LC>
 struct Shape {
-    static constexpr int kGroups = kMaxWarps * LC;  // most channel groups of a block
-    static constexpr int kPos = 32 / LC * V;        // positions of a tile
-    static constexpr int kChannels = kGroups * kEpt;
+    static constexpr int kPos = 32 / LC * V;         // positions of a tile
+    static constexpr int kPerWarp = EPT * LC;        // channels of a warp
+    static constexpr int kChannels = kMaxWarps * kPerWarp;
+    static constexpr int kPitch = kPos + 8;          // float2 per row: neighbouring rows on other banks
+    static constexpr int kPairs = EPT * V / 2;       // of a thread's values
+    static constexpr int kSpots = V == 1 ? 1 : V / 2;  // pairs of a thread's positions
+    static constexpr int kAcc = V == 1 ? EPT / 2 : EPT;
 };
 
-template <int V, int LC>
+template <int V, int EPT, int LC>
 struct alignas(16) Shared {
-    using S = Shape<V, LC>;
+    using S = Shape<V, EPT, LC>;
     float vec[kVectors][S::kChannels];
-    float2 part[S::kGroups][S::kPos];
+    float2 part[kMaxWarps][S::kPitch];
     float2 stat[S::kPos];
 };
 
@@ -55,95 +65,187 @@ __device__ void load_vectors(SH& sh, const Problem& p, int channels) {
 }
 
 struct Where {
-    int group, groups, pos, c0, mine;  // mine: the thread's channels that exist
+    int warp, warps, pos, c0, mine, of_warp;  // mine, of_warp: channels that exist
+    bool first;                               // of the warp's channel groups
 };
 
-template <int LC>
+template <int V, int EPT, int LC>
 __device__ __forceinline__ Where where(const Problem& p) {
+    constexpr int kLanes = 32 / LC;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int group = warp * LC + lane / (32 / LC);
-    return {group, static_cast<int>(blockDim.x) / 32 * LC, lane % (32 / LC), group * kEpt,
-            max(0, min(kEpt, p.channels - group * kEpt))};
+    const int c0 = warp * EPT * LC + lane / kLanes * EPT;
+    return {warp, static_cast<int>(blockDim.x) / 32, lane % kLanes, c0, max(0, min(EPT, p.channels - c0)),
+            max(0, min(EPT * LC, p.channels - warp * EPT * LC)), lane < kLanes};
 }
 
-// Mean and 1 / sqrt(variance + eps) over the channels of each of a thread's V positions; `keep`
-// (may be null) receives them per position.  Every thread of the block calls it.
-template <int V, int LC>
-__device__ __forceinline__ void statistics(Shared<V, LC>& sh, const Problem& p, const float (&v)[kEpt * V],
-                                           const Where& at, float (&mean)[V], float (&rho)[V], float* keep,
-                                           int live_pos) {
+// A thread's values lie in pairs: two positions of one channel (V = 4: pairs 2j and 2j + 1 are channel
+// j's), or two channels at one position (V = 1: pair i is channels 2i and 2i + 1).  Numbers per
+// position come as pairs too, kSpots of them; for V = 1 the same number twice.
+template <int V, int EPT>
+struct Pairs {
+    static constexpr int kCount = EPT * V / 2, kSpots = V == 1 ? 1 : V / 2;
+
+    static __device__ __forceinline__ int spot(int i) { return V == 1 ? 0 : i % kSpots; }
+    static __device__ __forceinline__ float2 channels(const float* of, int i) {
+        return V == 1 ? make_float2(of[2 * i], of[2 * i + 1]) : both(of[i / kSpots]);
+    }
+    // sums over the thread's channels, per position
+    static __device__ __forceinline__ void sum(const float2 (&v)[kCount], float2 (&s)[kSpots]) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        float m = 0.f, s = 0.f;
-        if (p.kind == kLayer) {  // channels that do not exist hold zeros
+        for (int q = 0; q < kSpots; ++q) s[q] = v[q];
 #pragma unroll
-            for (int j = 0; j < kEpt; ++j) m += v[j * V + i];
-            m = at.mine ? m / static_cast<float>(at.mine) : 0.f;
+        for (int i = kSpots; i < kCount; ++i) s[spot(i)] = add2(s[spot(i)], v[i]);
+        if (V == 1) s[0] = both(s[0].x + s[0].y);
+    }
+};
+
+// Sums over the warp's channel groups.
+template <int LC>
+__device__ __forceinline__ float2 sum_groups(float2 v) {
 #pragma unroll
-            for (int j = 0; j < kEpt; ++j) {
-                const float d = j < at.mine ? v[j * V + i] - m : 0.f;
-                s = fmaf(d, d, s);
-            }
+    for (int o = 16; o >= 32 / LC && LC > 1; o >>= 1) {
+        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+    return v;
+}
+
+// Joins two numbers per position and warp: f(thread's share, shares per position, read) runs on a few
+// threads per position, read(w) being warp w's numbers, and its result comes back to every thread's
+// positions in a and b.  Every thread of the block calls it.
+template <int V, int EPT, int LC, typename F>
+__device__ __forceinline__ void join(Shared<V, EPT, LC>& sh, const Where& at, float2 (&a)[Pairs<V, EPT>::kSpots],
+                                     float2 (&b)[Pairs<V, EPT>::kSpots], F f) {
+    using S = Shape<V, EPT, LC>;
+    if (at.first) {
+        float2* to = &sh.part[at.warp][at.pos * V];
+        if constexpr (V == 1) {
+            to[0] = make_float2(a[0].x, b[0].x);
         } else {
 #pragma unroll
-            for (int j = 0; j < kEpt; ++j) s = fmaf(v[j * V + i], v[j * V + i], s);
+            for (int q = 0; q < S::kSpots; ++q)
+                *reinterpret_cast<float4*>(to + 2 * q) = make_float4(a[q].x, b[q].x, a[q].y, b[q].y);
         }
-        sh.part[at.group][at.pos * V + i] = make_float2(m, s);
     }
     __syncthreads();
-    for (int q = threadIdx.x; q < Shape<V, LC>::kPos; q += blockDim.x) {
-        float m = 0.f, s = 0.f;
-        if (p.kind == kLayer) {
-            for (int g = 0; g < at.groups; ++g)
-                m = fmaf(static_cast<float>(max(0, min(kEpt, p.channels - g * kEpt))), sh.part[g][q].x, m);
-            m *= p.inv_c;
-            for (int g = 0; g < at.groups; ++g) {
-                const float2 a = sh.part[g][q];
-                const float d = a.x - m;
-                s += fmaf(static_cast<float>(max(0, min(kEpt, p.channels - g * kEpt))) * d, d, a.y);
+    // whole warps take part or not: f shuffles
+    const int lane = static_cast<int>(threadIdx.x % 32);
+    auto one = [&](int q, int share, int shares) {
+        const bool here = q < S::kPos;
+        const float2 r = f(share, shares, here ? q : 0, here && share == 0, [&](int w) { return sh.part[w][here ? q : 0]; });
+        if (here && share == 0) sh.stat[q] = r;
+    };
+    if (S::kPos >= 8 && static_cast<int>(blockDim.x) >= 4 * S::kPos) {  // a warp: 8 positions x 4 shares
+        if (at.warp < S::kPos / 8) one(at.warp * 8 + lane % 8, lane / 8, 4);
+    } else {
+        for (int q0 = at.warp * 32; q0 < S::kPos; q0 += at.warps * 32) one(q0 + lane, 0, 1);
+    }
+    __syncthreads();
+    const float2* from = &sh.stat[at.pos * V];
+    if constexpr (V == 1) {
+        a[0] = both(from[0].x);
+        b[0] = both(from[0].y);
+    } else {
+#pragma unroll
+        for (int s = 0; s < S::kSpots; ++s) {
+            const float4 v = *reinterpret_cast<const float4*>(from + 2 * s);
+            a[s] = make_float2(v.x, v.z);
+            b[s] = make_float2(v.y, v.w);
+        }
+    }
+}
+
+// Sums over the four shares of a position.
+__device__ __forceinline__ float sum_shares(float v, int shares) {
+    if (shares == 4) {
+        v += __shfl_xor_sync(0xffffffffu, v, 8);
+        v += __shfl_xor_sync(0xffffffffu, v, 16);
+    }
+    return v;
+}
+
+// Rho = 1 / sqrt(variance + eps) and -mean rho over the channels of a thread's positions, so that the
+// normalised value is v rho - mean rho; `keep` (may be null) receives mean and rho per position.
+template <int V, int EPT, int LC>
+__device__ __forceinline__ void statistics(Shared<V, EPT, LC>& sh, const Problem& p,
+                                           const float2 (&v)[Pairs<V, EPT>::kCount], const Where& at,
+                                           float2 (&rho)[Pairs<V, EPT>::kSpots], float2 (&shift)[Pairs<V, EPT>::kSpots],
+                                           float* keep, int live_pos) {
+    using P = Pairs<V, EPT>;
+    constexpr int kPerWarp = EPT * LC;
+    float2 d[P::kCount];
+    const bool layer = p.kind == kLayer;
+    if (layer) {  // channels that do not exist hold zeros
+        P::sum(v, shift);
+        const float2 inv = both(at.of_warp ? 1.f / static_cast<float>(at.of_warp) : 0.f);
+#pragma unroll
+        for (int q = 0; q < P::kSpots; ++q) shift[q] = mul2(sum_groups<LC>(shift[q]), inv);
+#pragma unroll
+        for (int i = 0; i < P::kCount; ++i) {
+            const float2 m = shift[P::spot(i)];
+            d[i] = add2(v[i], make_float2(-m.x, -m.y));
+            if (V == 1) {
+                if (2 * i >= at.mine) d[i].x = 0.f;
+                if (2 * i + 1 >= at.mine) d[i].y = 0.f;
+            } else if (i / P::kSpots >= at.mine) {
+                d[i] = both(0.f);
+            }
+            d[i] = mul2(d[i], d[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < P::kCount; ++i) d[i] = mul2(v[i], v[i]);
+#pragma unroll
+        for (int q = 0; q < P::kSpots; ++q) shift[q] = both(0.f);
+    }
+    P::sum(d, rho);
+#pragma unroll
+    for (int q = 0; q < P::kSpots; ++q) rho[q] = sum_groups<LC>(rho[q]);
+    join<V, EPT, LC>(sh, at, shift, rho, [&](int share, int shares, int q, bool store, auto part) {
+        float mean = 0.f, sum = 0.f;
+        if (layer) {
+            for (int w = share; w < at.warps; w += shares)
+                mean = fmaf(static_cast<float>(min(kPerWarp, p.channels - w * kPerWarp)), part(w).x, mean);
+            mean = sum_shares(mean, shares) * p.inv_c;
+            for (int w = share; w < at.warps; w += shares) {
+                const float2 e = part(w);
+                const float off = e.x - mean;
+                sum += fmaf(static_cast<float>(min(kPerWarp, p.channels - w * kPerWarp)) * off, off, e.y);
             }
         } else {
 #pragma unroll 4
-            for (int g = 0; g < at.groups; ++g) s += sh.part[g][q].y;
+            for (int w = share; w < at.warps; w += shares) sum += part(w).y;
         }
-        const float r = 1.f / sqrtf(fmaf(s, p.inv_c, p.eps));
-        sh.stat[q] = make_float2(m, r);
-        if (keep != nullptr && q < live_pos) {
-            keep[q] = m;
+        const float r = rsqrtf(fmaf(sum_shares(sum, shares), p.inv_c, p.eps));
+        if (store && keep != nullptr && q < live_pos) {
+            keep[q] = mean;
             keep[p.positions + q] = r;
         }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const float2 a = sh.stat[at.pos * V + i];
-        mean[i] = a.x;
-        rho[i] = a.y;
-    }
+        return make_float2(-mean * r, r);
+    });
 }
 
-// Means over the channels of two products, per position; every thread of the block calls it.
-template <int V, int LC>
-__device__ __forceinline__ void two_means(Shared<V, LC>& sh, const Problem& p, const Where& at, float2 (&mean)[V]) {
+// The negatives of the means over the channels of two products, given as sums over the thread's
+// channels per position; the first is zero in the RMS kind.
+template <int V, int EPT, int LC>
+__device__ __forceinline__ void two_means(Shared<V, EPT, LC>& sh, const Problem& p, const Where& at,
+                                          float2 (&m1)[Pairs<V, EPT>::kSpots], float2 (&m2)[Pairs<V, EPT>::kSpots]) {
+    const bool layer = p.kind == kLayer;
 #pragma unroll
-    for (int i = 0; i < V; ++i) sh.part[at.group][at.pos * V + i] = mean[i];
-    __syncthreads();
-    for (int q = threadIdx.x; q < Shape<V, LC>::kPos; q += blockDim.x) {
-        float a = 0.f, b = 0.f;
-#pragma unroll 4
-        for (int g = 0; g < at.groups; ++g) {
-            a += sh.part[g][q].x;
-            b += sh.part[g][q].y;
-        }
-        sh.stat[q] = make_float2(p.kind == kLayer ? a * p.inv_c : 0.f, b * p.inv_c);
+    for (int q = 0; q < Pairs<V, EPT>::kSpots; ++q) {
+        if (layer) m1[q] = sum_groups<LC>(m1[q]);
+        m2[q] = sum_groups<LC>(m2[q]);
     }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < V; ++i) mean[i] = sh.stat[at.pos * V + i];
+    join<V, EPT, LC>(sh, at, m1, m2, [&](int share, int shares, int, bool, auto part) {
+        float2 s = both(0.f);
+#pragma unroll 4
+        for (int w = share; w < at.warps; w += shares) s = add2(s, part(w));
+        return make_float2(layer ? -sum_shares(s.x, shares) * p.inv_c : 0.f, -sum_shares(s.y, shares) * p.inv_c);
+    });
 }
 
 // Where a tile lies, for one thread.
-template <int V, int LC>
+template <int V, int EPT, int LC>
 struct Tile {
     int sample, l0;
     bool live;    // whether the thread's positions exist
@@ -152,7 +254,7 @@ struct Tile {
     __device__ __forceinline__ Tile(const Problem& p, const Where& at, int tile) {
         const int ts = static_cast<int>(p.tiles_per_sample);
         sample = tile / ts;
-        l0 = (tile - sample * ts) * Shape<V, LC>::kPos;
+        l0 = (tile - sample * ts) * Shape<V, EPT, LC>::kPos;
         const int l = l0 + at.pos * V;
         live = l < static_cast<int>(p.length);
         base = (static_cast<size_t>(sample) * p.channels + at.c0) * p.length + l;
@@ -160,73 +262,80 @@ struct Tile {
 };
 
 // A thread's slots for one tensor of one tile, and how it fills and reads them.
-template <typename T, int V>
+template <typename T, int V, int EPT>
 struct Slots {
     using E = Vec<T, V>;
+    using P = Pairs<V, EPT>;
 
     static __device__ __forceinline__ void fetch(E* slot, const void* from, size_t base, size_t stride, int end) {
         if constexpr (kCopied<E>) {
 #pragma unroll
-            for (int j = 0; j < kEpt; ++j)
+            for (int j = 0; j < EPT; ++j)
                 copy_async(slot + j * blockDim.x, static_cast<const T*>(from) + (j < end ? base + j * stride : 0), j < end);
         }
     }
 
     static __device__ __forceinline__ void read(const E* slot, const void* from, size_t base, size_t stride, int end,
-                                                float (&out)[kEpt * V]) {
+                                                float2 (&out)[P::kCount]) {
+        E v[EPT];
 #pragma unroll
-        for (int j = 0; j < kEpt; ++j) {
-            E v{};
-            if constexpr (kCopied<E>) v = slot[j * blockDim.x];
-            else if (j < end) v = load_vec<T, V>(from, base + j * stride);
-#pragma unroll
-            for (int i = 0; i < V; ++i) out[j * V + i] = to_f32(v.v[i]);
+        for (int j = 0; j < EPT; ++j) {
+            v[j] = E{};
+            if constexpr (kCopied<E>) v[j] = slot[j * blockDim.x];
+            else if (j < end) v[j] = load_vec<T, V>(from, base + j * stride);
         }
+#pragma unroll
+        for (int i = 0; i < P::kCount; ++i) {
+            if constexpr (V == 1) out[i] = unpack(v[2 * i].v[0], v[2 * i + 1].v[0]);
+            else out[i] = unpack(v[i / P::kSpots].v[i % P::kSpots * 2], v[i / P::kSpots].v[i % P::kSpots * 2 + 1]);
+        }
+    }
+
+    static __device__ __forceinline__ void store(void* to, size_t base, size_t stride, int end,
+                                                 const float2 (&v)[P::kCount]) {
+        E o[EPT];
+#pragma unroll
+        for (int i = 0; i < P::kCount; ++i) {
+            if constexpr (V == 1) pack(o[2 * i].v[0], o[2 * i + 1].v[0], v[i]);
+            else pack(o[i / P::kSpots].v[i % P::kSpots * 2], o[i / P::kSpots].v[i % P::kSpots * 2 + 1], v[i]);
+        }
+#pragma unroll
+        for (int j = 0; j < EPT; ++j)
+            if (j < end) store_vec<T, V>(to, base + j * stride, o[j]);
     }
 };
 
-template <typename T, int V>
-__device__ __forceinline__ void store_all(void* to, size_t base, size_t stride, int end, const float (&v)[kEpt * V]) {
-#pragma unroll
-    for (int j = 0; j < kEpt; ++j) {
-        Vec<T, V> o;
-#pragma unroll
-        for (int i = 0; i < V; ++i) from_f32(o.v[i], v[j * V + i]);
-        if (j < end) store_vec<T, V>(to, base + j * stride, o);
-    }
-}
-
 // act(gate) of a thread's channels, the gate being one value per sample and channel.
-template <typename T, int V>
-__device__ __forceinline__ void sample_gate(const Problem& p, const Where& at, int sample, float (&a)[kEpt * V]) {
-    float g[kEpt];
+template <typename T, int V, int EPT>
+__device__ __forceinline__ void sample_gate(const Problem& p, const Where& at, int sample,
+                                            float2 (&a)[Pairs<V, EPT>::kCount]) {
+    float g[EPT];
 #pragma unroll
-    for (int j = 0; j < kEpt; ++j)
-        g[j] = j < at.mine ? to_f32(static_cast<const T*>(p.gate)[static_cast<size_t>(sample) * p.channels + at.c0 + j]) : 0.f;
-    activate_all(g, p.act);
+    for (int j = 0; j < EPT; ++j)
+        g[j] = j < at.mine ? activate(to_f32(static_cast<const T*>(
+                                          p.gate)[static_cast<size_t>(sample) * p.channels + at.c0 + j]), p.act)
+                           : 0.f;
 #pragma unroll
-    for (int j = 0; j < kEpt; ++j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) a[j * V + i] = g[j];
+    for (int i = 0; i < Pairs<V, EPT>::kCount; ++i) a[i] = Pairs<V, EPT>::channels(g, i);
 }
 
 __host__ __device__ constexpr int forward_tensors(int mode) { return mode == kNoBlock ? 1 : mode == kFull ? 3 : 2; }
 
-template <typename T, int V, int LC, int MODE>
+template <typename T, int V, int EPT, int LC, int MODE>
 __global__ void __launch_bounds__(kMaxWarps * 32, 2) field_forward_kernel(const __grid_constant__ Problem p) {
-    using S = Shape<V, LC>;
-    using F = Slots<T, V>;
+    using F = Slots<T, V, EPT>;
+    using P = Pairs<V, EPT>;
     extern __shared__ __align__(16) unsigned char dynamic[];
-    auto& sh = *reinterpret_cast<Shared<V, LC>*>(dynamic);
-    const Where at = where<LC>(p);
+    auto& sh = *reinterpret_cast<Shared<V, EPT, LC>*>(dynamic);
+    const Where at = where<V, EPT, LC>(p);
     const size_t stride = static_cast<size_t>(p.length);
     const int tiles = static_cast<int>(p.tiles);
     constexpr int kTensors = forward_tensors(MODE);
     auto* slots = reinterpret_cast<typename F::E*>(dynamic + sizeof(sh)) + threadIdx.x;
-    auto slot = [&](int turn, int tensor) { return slots + (turn * kTensors + tensor) * kEpt * blockDim.x; };
+    auto slot = [&](int turn, int tensor) { return slots + (turn * kTensors + tensor) * EPT * blockDim.x; };
     auto fetch = [&](int tile, int turn) {
         if (tile < tiles) {
-            const Tile<V, LC> t(p, at, tile);
+            const Tile<V, EPT, LC> t(p, at, tile);
             const int end = t.live ? at.mine : 0;
             F::fetch(slot(turn, 0), p.x, t.base, stride, end);
             if constexpr (MODE != kNoBlock) F::fetch(slot(turn, 1), p.y, t.base, stride, end);
@@ -235,51 +344,75 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) field_forward_kernel(const 
         copy_commit();
     };
     fetch(blockIdx.x, 0);
-    load_vectors<T>(sh, p, at.groups * kEpt);
+    load_vectors<T>(sh, p, at.warps * EPT * LC);
     int turn = 0;
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
-        const Tile<V, LC> t(p, at, tile);
+        const Tile<V, EPT, LC> t(p, at, tile);
         const int end = t.live ? at.mine : 0;
         const size_t q0 = static_cast<size_t>(t.sample) * p.length + t.l0;
-        const int live_pos = min(S::kPos, static_cast<int>(p.length) - t.l0);
+        const int live_pos = static_cast<int>(p.length) - t.l0;
         fetch(tile + gridDim.x, turn ^ 1);
         copy_wait<1>();
-        float r[kEpt * V], mean[V], rho[V];
+        float2 r[P::kCount], rho[P::kSpots], shift[P::kSpots];
         F::read(slot(turn, 0), p.x, t.base, stride, end, r);
         if constexpr (MODE != kNoBlock) {
-            float h[kEpt * V], a[kEpt * V];
+            float2 h[P::kCount], a[P::kCount];
             F::read(slot(turn, 1), p.y, t.base, stride, end, h);
             if constexpr (MODE == kFull) F::read(slot(turn, 2), p.gate, t.base, stride, end, a);
             if (p.post) {
-                statistics<V, LC>(sh, p, h, at, mean, rho, p.stats ? p.stats + q0 : nullptr, live_pos);
+                statistics<V, EPT, LC>(sh, p, h, at, rho, shift, p.stats ? p.stats + q0 : nullptr, live_pos);
 #pragma unroll
-                for (int j = 0; j < kEpt * V; ++j) h[j] = (h[j] - mean[j % V]) * rho[j % V];
+                for (int i = 0; i < P::kCount; ++i) h[i] = fma2(h[i], rho[P::spot(i)], shift[P::spot(i)]);
             }
             if constexpr (MODE == kFull) activate_all(a, p.act);
-            if constexpr (MODE == kSample) sample_gate<T, V>(p, at, t.sample, a);
+            if constexpr (MODE == kSample) sample_gate<T, V, EPT>(p, at, t.sample, a);
 #pragma unroll
-            for (int j = 0; j < kEpt; ++j) {
-                const float w = sh.vec[kPostW][at.c0 + j], b = sh.vec[kPostB][at.c0 + j];
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float z = fmaf(h[j * V + i], w, b);
-                    r[j * V + i] = MODE == kPlain ? r[j * V + i] + z : fmaf(a[j * V + i], z, r[j * V + i]);
-                }
+            for (int i = 0; i < P::kCount; ++i) {
+                const float2 z = fma2(h[i], P::channels(&sh.vec[kPostW][at.c0], i), P::channels(&sh.vec[kPostB][at.c0], i));
+                r[i] = MODE == kPlain ? add2(r[i], z) : fma2(a[i], z, r[i]);
             }
-            store_all<T, V>(p.r, t.base, stride, end, r);
+            F::store(p.r, t.base, stride, end, r);
         }
         if (!p.pre) continue;
-        statistics<V, LC>(sh, p, r, at, mean, rho, p.stats ? p.stats + 2 * p.positions + q0 : nullptr, live_pos);
+        statistics<V, EPT, LC>(sh, p, r, at, rho, shift, p.stats ? p.stats + 2 * p.positions + q0 : nullptr, live_pos);
 #pragma unroll
-        for (int j = 0; j < kEpt; ++j) {
-            const float w = sh.vec[kPreW][at.c0 + j], b = sh.vec[kPreB][at.c0 + j];
-#pragma unroll
-            for (int i = 0; i < V; ++i) r[j * V + i] = fmaf((r[j * V + i] - mean[i]) * rho[i], w, b);
-        }
-        store_all<T, V>(p.n, t.base, stride, end, r);
+        for (int i = 0; i < P::kCount; ++i)
+            r[i] = fma2(fma2(r[i], rho[P::spot(i)], shift[P::spot(i)]), P::channels(&sh.vec[kPreW][at.c0], i),
+                        P::channels(&sh.vec[kPreB][at.c0], i));
+        F::store(p.n, t.base, stride, end, r);
     }
     copy_wait<0>();
 }
+
+// The forward's statistics of a thread's positions; zero rho where there is no position.  They are
+// loaded a tile ahead, like the tensors.
+template <int V>
+struct Saved {
+    static constexpr int kSpots = V == 1 ? 1 : V / 2;
+    float2 mean[kSpots], rho[kSpots], mean2[kSpots], rho2[kSpots];
+
+    template <typename TILE>
+    __device__ __forceinline__ void load(const Problem& p, const TILE& t, int pos) {
+#pragma unroll
+        for (int s = 0; s < kSpots; ++s) mean[s] = rho[s] = mean2[s] = rho2[s] = both(0.f);
+        if (!t.live) return;
+        const float* st = p.stats + static_cast<size_t>(t.sample) * p.length + t.l0 + pos * V;
+        const size_t row = static_cast<size_t>(p.positions);
+#pragma unroll
+        for (int s = 0; s < kSpots; ++s) {
+            const int b = V == 1 ? 0 : 1;
+            rho[s] = both(1.f);
+            if (p.post) {
+                mean[s] = make_float2(st[2 * s], st[2 * s + b]);
+                rho[s] = make_float2(st[row + 2 * s], st[row + 2 * s + b]);
+            }
+            if (p.dn) {
+                mean2[s] = make_float2(st[2 * row + 2 * s], st[2 * row + 2 * s + b]);
+                rho2[s] = make_float2(st[3 * row + 2 * s], st[3 * row + 2 * s + b]);
+            }
+        }
+    }
+};
 
 // Adds v over the lanes that share this lane's channel group.
 template <int LC>
@@ -292,22 +425,24 @@ __device__ __forceinline__ float sum_positions(float v) {
 // Tensors a backward reads: x, y, dn, dr, and a gate per element.
 __host__ __device__ constexpr int backward_tensors(int mode) { return mode == kFull ? 5 : 4; }
 
-template <typename T, int V, int LC, int MODE>
+template <typename T, int V, int EPT, int LC, int MODE>
 __global__ void __launch_bounds__(kMaxWarps * 32) field_backward_kernel(const __grid_constant__ Problem p) {
-    using F = Slots<T, V>;
-    constexpr int N = kEpt * V;
+    using F = Slots<T, V, EPT>;
+    using P = Pairs<V, EPT>;
+    using TILE = Tile<V, EPT, LC>;
+    constexpr int N = P::kCount, kSpots = P::kSpots, kAcc = Shape<V, EPT, LC>::kAcc;
     extern __shared__ __align__(16) unsigned char dynamic[];
-    auto& sh = *reinterpret_cast<Shared<V, LC>*>(dynamic);
+    auto& sh = *reinterpret_cast<Shared<V, EPT, LC>*>(dynamic);
     grid_dep_launch();
-    const Where at = where<LC>(p);
+    const Where at = where<V, EPT, LC>(p);
     const size_t stride = static_cast<size_t>(p.length);
     constexpr int kTensors = backward_tensors(MODE);
     auto* slots = reinterpret_cast<typename F::E*>(dynamic + sizeof(sh)) + threadIdx.x;
-    auto slot = [&](int turn, int tensor) { return slots + (turn * kTensors + tensor) * kEpt * blockDim.x; };
+    auto slot = [&](int turn, int tensor) { return slots + (turn * kTensors + tensor) * EPT * blockDim.x; };
     const int first = static_cast<int>(tile_begin(p, blockIdx.x)), last = static_cast<int>(tile_begin(p, blockIdx.x + 1));
     auto fetch = [&](int tile, int turn) {
         if (tile < last) {
-            const Tile<V, LC> t(p, at, tile);
+            const TILE t(p, at, tile);
             const int end = t.live ? at.mine : 0;
             if constexpr (MODE != kNoBlock) F::fetch(slot(turn, 1), p.y, t.base, stride, end);
             if (p.dn) {
@@ -320,123 +455,122 @@ __global__ void __launch_bounds__(kMaxWarps * 32) field_backward_kernel(const __
         copy_commit();
     };
     fetch(first, 0);
-    load_vectors<T>(sh, p, at.groups * kEpt);
+    Saved<V> ahead;
+    if (first < last) ahead.load(p, TILE(p, at, first), at.pos);
+    load_vectors<T>(sh, p, at.warps * EPT * LC);
     int turn = 0;
-    float sum[kSums][kEpt] = {};
-    for (int tile = first; tile < last; ++tile, turn ^= 1) {
-        const Tile<V, LC> t(p, at, tile);
-        const int end = t.live ? at.mine : 0;
-        float mean[V], rho[V], mean2[V], rho2[V];
-        {
-            const float* st = p.stats + static_cast<size_t>(t.sample) * p.length + t.l0 + at.pos * V;
+    // sums over positions: per channel (V = 4: to be added over the pair), or per pair of channels
+    float2 sum[kSums][kAcc];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                mean[i] = t.live && p.post ? st[i] : 0.f;
-                rho[i] = t.live ? (p.post ? st[p.positions + i] : 1.f) : 0.f;
-                mean2[i] = t.live && p.dn ? st[2 * p.positions + i] : 0.f;
-                rho2[i] = t.live && p.dn ? st[3 * p.positions + i] : 0.f;
-            }
+    for (int k = 0; k < kSums; ++k)
+#pragma unroll
+        for (int i = 0; i < kAcc; ++i) sum[k][i] = both(0.f);
+    auto acc = [](int i) { return V == 1 ? i : i / kSpots; };
+    auto of_channel = [&](int kind, int j) {
+        return V == 1 ? (j % 2 ? sum[kind][j / 2].y : sum[kind][j / 2].x) : sum[kind][j % kAcc].x + sum[kind][j % kAcc].y;
+    };
+    for (int tile = first; tile < last; ++tile, turn ^= 1) {
+        const TILE t(p, at, tile);
+        const int end = t.live ? at.mine : 0;
+        float2 rho[kSpots], shift[kSpots], rho2[kSpots], shift2[kSpots];
+#pragma unroll
+        for (int s = 0; s < kSpots; ++s) {
+            rho[s] = ahead.rho[s];
+            rho2[s] = ahead.rho2[s];
+            shift[s] = make_float2(-ahead.mean[s].x * rho[s].x, -ahead.mean[s].y * rho[s].y);
+            shift2[s] = make_float2(-ahead.mean2[s].x * rho2[s].x, -ahead.mean2[s].y * rho2[s].y);
         }
         fetch(tile + 1, turn ^ 1);
+        if (tile + 1 < last) ahead.load(p, TILE(p, at, tile + 1), at.pos);
         copy_wait<1>();
-        float h[N], a[N], slope[N], k[N], g[N];
+        float2 h[N], a[N], slope[N], k[N], g[N];
         if constexpr (MODE != kNoBlock) {
             F::read(slot(turn, 1), p.y, t.base, stride, end, h);
 #pragma unroll
-            for (int j = 0; j < N; ++j) h[j] = (h[j] - mean[j % V]) * rho[j % V];
+            for (int i = 0; i < N; ++i) h[i] = fma2(h[i], rho[P::spot(i)], shift[P::spot(i)]);
             if constexpr (MODE == kFull) {
                 F::read(slot(turn, 4), p.gate, t.base, stride, end, a);
                 activate_all(a, slope, p.act);
             }
-            if constexpr (MODE == kSample) sample_gate<T, V>(p, at, t.sample, a);
+            if constexpr (MODE == kSample) sample_gate<T, V, EPT>(p, at, t.sample, a);
         }
-        float2 m[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) m[i] = make_float2(0.f, 0.f);
         if (p.dn) {
             F::read(slot(turn, 0), p.x, t.base, stride, end, k);
             F::read(slot(turn, 2), p.dn, t.base, stride, end, g);
+            float2 gk[N], m1[kSpots], m2[kSpots];
 #pragma unroll
-            for (int j = 0; j < kEpt; ++j) {
-                const float w = sh.vec[kPostW][at.c0 + j], b = sh.vec[kPostB][at.c0 + j], w2 = sh.vec[kPreW][at.c0 + j];
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const int e = j * V + i;
-                    if constexpr (MODE != kNoBlock) {
-                        const float z = fmaf(h[e], w, b);
-                        k[e] = MODE == kPlain ? k[e] + z : fmaf(a[e], z, k[e]);
-                    }
-                    k[e] = (k[e] - mean2[i]) * rho2[i];
-                    sum[kDPreW][j] = fmaf(g[e], k[e], sum[kDPreW][j]);
-                    sum[kDPreB][j] += g[e];
-                    g[e] *= w2;
-                    m[i].x += g[e];
-                    m[i].y = fmaf(g[e], k[e], m[i].y);
+            for (int i = 0; i < N; ++i) {
+                if constexpr (MODE != kNoBlock) {
+                    const float2 z =
+                        fma2(h[i], P::channels(&sh.vec[kPostW][at.c0], i), P::channels(&sh.vec[kPostB][at.c0], i));
+                    k[i] = MODE == kPlain ? add2(k[i], z) : fma2(a[i], z, k[i]);
                 }
+                k[i] = fma2(k[i], rho2[P::spot(i)], shift2[P::spot(i)]);
+                sum[kDPreW][acc(i)] = fma2(g[i], k[i], sum[kDPreW][acc(i)]);
+                sum[kDPreB][acc(i)] = add2(sum[kDPreB][acc(i)], g[i]);
+                g[i] = mul2(g[i], P::channels(&sh.vec[kPreW][at.c0], i));
+                gk[i] = mul2(g[i], k[i]);
             }
-            two_means<V, LC>(sh, p, at, m);
+            P::sum(g, m1);
+            P::sum(gk, m2);
+            two_means<V, EPT, LC>(sh, p, at, m1, m2);
 #pragma unroll
-            for (int e = 0; e < N; ++e) g[e] = rho2[e % V] * (g[e] - m[e % V].x - k[e] * m[e % V].y);
+            for (int i = 0; i < N; ++i)
+                g[i] = mul2(rho2[P::spot(i)], add2(fma2(k[i], m2[P::spot(i)], g[i]), m1[P::spot(i)]));
         } else {
 #pragma unroll
-            for (int e = 0; e < N; ++e) g[e] = 0.f;
+            for (int i = 0; i < N; ++i) g[i] = both(0.f);
         }
         if (p.dr) {
             F::read(slot(turn, 3), p.dr, t.base, stride, end, k);
 #pragma unroll
-            for (int e = 0; e < N; ++e) g[e] += k[e];
+            for (int i = 0; i < N; ++i) g[i] = add2(g[i], k[i]);
         }
         // g: the gradient of r
-        if (p.dx) store_all<T, V>(p.dx, t.base, stride, end, g);
+        if (p.dx) F::store(p.dx, t.base, stride, end, g);
         if constexpr (MODE != kNoBlock) {
+            float2 kh[N];
 #pragma unroll
-            for (int i = 0; i < V; ++i) m[i] = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int j = 0; j < kEpt; ++j) {
-                const float w = sh.vec[kPostW][at.c0 + j];
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const int e = j * V + i;
-                    const float ta = MODE == kPlain ? g[e] : g[e] * a[e];
-                    const float v = MODE == kSample ? g[e] : ta;
-                    sum[kTah][j] = fmaf(v, h[e], sum[kTah][j]);
-                    sum[kTa][j] += v;
-                    k[e] = ta * w;
-                    m[i].x += k[e];
-                    m[i].y = fmaf(k[e], h[e], m[i].y);
-                }
+            for (int i = 0; i < N; ++i) {
+                const float2 ta = MODE == kPlain ? g[i] : mul2(g[i], a[i]);
+                const float2 v = MODE == kSample ? g[i] : ta;
+                sum[kTah][acc(i)] = fma2(v, h[i], sum[kTah][acc(i)]);
+                sum[kTa][acc(i)] = add2(sum[kTa][acc(i)], v);
+                k[i] = mul2(ta, P::channels(&sh.vec[kPostW][at.c0], i));
+                kh[i] = mul2(k[i], h[i]);
             }
             if (MODE == kFull && p.dgate) {
-                float o[N];
 #pragma unroll
-                for (int j = 0; j < kEpt; ++j) {
-                    const float w = sh.vec[kPostW][at.c0 + j], b = sh.vec[kPostB][at.c0 + j];
-#pragma unroll
-                    for (int i = 0; i < V; ++i)
-                        o[j * V + i] = g[j * V + i] * fmaf(h[j * V + i], w, b) * slope[j * V + i];
-                }
-                store_all<T, V>(p.dgate, t.base, stride, end, o);
+                for (int i = 0; i < N; ++i)
+                    a[i] = mul2(mul2(g[i], slope[i]),
+                                fma2(h[i], P::channels(&sh.vec[kPostW][at.c0], i), P::channels(&sh.vec[kPostB][at.c0], i)));
+                F::store(p.dgate, t.base, stride, end, a);
             }
             if (p.dy) {
                 if (p.post) {
-                    two_means<V, LC>(sh, p, at, m);
+                    float2 m1[kSpots], m2[kSpots];
+                    P::sum(k, m1);
+                    P::sum(kh, m2);
+                    two_means<V, EPT, LC>(sh, p, at, m1, m2);
 #pragma unroll
-                    for (int e = 0; e < N; ++e) k[e] = rho[e % V] * (k[e] - m[e % V].x - h[e] * m[e % V].y);
+                    for (int i = 0; i < N; ++i)
+                        k[i] = mul2(rho[P::spot(i)], add2(fma2(h[i], m2[P::spot(i)], k[i]), m1[P::spot(i)]));
                 }
-                store_all<T, V>(p.dy, t.base, stride, end, k);
+                F::store(p.dy, t.base, stride, end, k);
             }
             if (MODE == kSample && p.slots &&
-                (tile + 1 == last || t.l0 + Shape<V, LC>::kPos >= static_cast<int>(p.length))) {
+                (tile + 1 == last || t.l0 + Shape<V, EPT, LC>::kPos >= static_cast<int>(p.length))) {
                 float* to = slot_of(p, blockIdx.x, t.sample);
 #pragma unroll
-                for (int j = 0; j < kEpt; ++j) {
+                for (int j = 0; j < EPT; ++j) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float total = sum_positions<LC>(sum[kTah + i][j]);
+                        const float total = sum_positions<LC>(of_channel(kTah + i, j));
                         if (at.pos == 0 && j < at.mine) to[static_cast<size_t>(i) * p.channels + at.c0 + j] = total;
-                        sum[kTah + i][j] = 0.f;
                     }
                 }
+#pragma unroll
+                for (int i = 0; i < kAcc; ++i) sum[kTah][i] = sum[kTa][i] = both(0.f);
             }
         }
     }
@@ -445,8 +579,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32) field_backward_kernel(const __
 #pragma unroll
     for (int i = 0; i < kSums; ++i) {
 #pragma unroll
-        for (int j = 0; j < kEpt; ++j) {
-            const float total = sum_positions<LC>(sum[i][j]);
+        for (int j = 0; j < EPT; ++j) {
+            const float total = sum_positions<LC>(of_channel(i, j));
             if (at.pos == 0 && j < at.mine)
                 p.partial[(static_cast<size_t>(blockIdx.x) * kSums + i) * p.channels + at.c0 + j] = total;
         }
@@ -454,48 +588,50 @@ __global__ void __launch_bounds__(kMaxWarps * 32) field_backward_kernel(const __
 }
 
 // Sets the tiles of a shape; false where their count or a position does not fit the kernels' int.
-template <int V, int LC>
+template <typename S>
 bool set_tiles(Problem& p) {
-    constexpr int kPos = Shape<V, LC>::kPos;
-    p.tiles_per_sample = (p.length + kPos - 1) / kPos;
+    p.tiles_per_sample = (p.length + S::kPos - 1) / S::kPos;
     p.tiles = p.batch * p.tiles_per_sample;
     return p.tiles < (1LL << 30) && p.length < (1LL << 30);
 }
 
-template <int LC>
+template <typename S>
 int threads_for(int channels) {
-    return (channels + kEpt * LC - 1) / (kEpt * LC) * 32;
+    return (channels + S::kPerWarp - 1) / S::kPerWarp * 32;
 }
 
-template <typename T, int V, int LC, int MODE>
+template <typename T, int V, int EPT, int LC, int MODE>
 cudaError_t forward_as(Problem p, cudaStream_t s) {
-    if (!set_tiles<V, LC>(p)) return cudaErrorNotSupported;
-    const int threads = threads_for<LC>(p.channels);
-    const size_t smem = sizeof(Shared<V, LC>) +
-                        (kCopied<Vec<T, V>> ? 2 * forward_tensors(MODE) * kEpt * sizeof(Vec<T, V>) * threads : 0);
+    using S = Shape<V, EPT, LC>;
+    if (!set_tiles<S>(p)) return cudaErrorNotSupported;
+    const int threads = threads_for<S>(p.channels);
+    const size_t smem = sizeof(Shared<V, EPT, LC>) +
+                        (kCopied<Vec<T, V>> ? 2 * forward_tensors(MODE) * EPT * sizeof(Vec<T, V>) * threads : 0);
     int per_sm = 0;
-    const cudaError_t e =
-        scx::prepare_kernel(reinterpret_cast<const void*>(field_forward_kernel<T, V, LC, MODE>), smem, threads, &per_sm);
+    const cudaError_t e = scx::prepare_kernel(reinterpret_cast<const void*>(field_forward_kernel<T, V, EPT, LC, MODE>),
+                                              smem, threads, &per_sm);
     if (e != cudaSuccess) return e;
     const int grid = static_cast<int>(std::min<long long>(p.tiles, static_cast<long long>(per_sm) * scx::num_sms()));
-    field_forward_kernel<T, V, LC, MODE><<<grid, threads, smem, s>>>(p);
+    field_forward_kernel<T, V, EPT, LC, MODE><<<grid, threads, smem, s>>>(p);
     return cudaGetLastError();
 }
 
-template <typename T, int V, int LC, int MODE>
+template <typename T, int V, int EPT, int LC, int MODE>
 cudaError_t backward_as(Problem& p, cudaStream_t s) {
+    using S = Shape<V, EPT, LC>;
     Problem q = p;
-    if (!set_tiles<V, LC>(q)) return cudaErrorNotSupported;
-    const int threads = threads_for<LC>(p.channels);
-    const size_t smem = sizeof(Shared<V, LC>) +
-                        (kCopied<Vec<T, V>> ? 2 * backward_tensors(MODE) * kEpt * sizeof(Vec<T, V>) * threads : 0);
+    if (!set_tiles<S>(q)) return cudaErrorNotSupported;
+    const int threads = threads_for<S>(p.channels);
+    const size_t smem = sizeof(Shared<V, EPT, LC>) +
+                        (kCopied<Vec<T, V>> ? 2 * backward_tensors(MODE) * EPT * sizeof(Vec<T, V>) * threads : 0);
     int per_sm = 0;
-    const cudaError_t e =
-        scx::prepare_kernel(reinterpret_cast<const void*>(field_backward_kernel<T, V, LC, MODE>), smem, threads, &per_sm);
+    const cudaError_t e = scx::prepare_kernel(reinterpret_cast<const void*>(field_backward_kernel<T, V, EPT, LC, MODE>),
+                                              smem, threads, &per_sm);
     if (e != cudaSuccess) return e;
     q.parts = static_cast<int>(std::min<long long>(std::min(max_parts(p.channels), per_sm * scx::num_sms()), q.tiles));
+    q.partials = q.parts;
     p = q;
-    field_backward_kernel<T, V, LC, MODE><<<p.parts, threads, smem, s>>>(p);
+    field_backward_kernel<T, V, EPT, LC, MODE><<<p.parts, threads, smem, s>>>(p);
     return cudaGetLastError();
 }
 
@@ -511,29 +647,27 @@ bool vectors_fit(const Problem& p) {
 
 template <typename T, int MODE>
 cudaError_t forward_in(const Problem& p, cudaStream_t s) {
-    constexpr int kPer = kEpt * kMaxWarps;  // channels of a block at LC = 1
-    if (vectors_fit<T, 2>(p)) {
-        if (p.channels <= kPer) return forward_as<T, 2, 1, MODE>(p, s);
-        if (p.channels <= 2 * kPer) return forward_as<T, 2, 2, MODE>(p, s);
-        if (p.channels <= 8 * kPer) return forward_as<T, 2, 8, MODE>(p, s);
+    if (vectors_fit<T, 4>(p)) {
+        if (p.channels <= 64) return forward_as<T, 4, 2, 2, MODE>(p, s);
+        if (p.channels <= 128) return forward_as<T, 4, 2, 4, MODE>(p, s);
+        if (p.channels <= 512) return forward_as<T, 4, 2, 16, MODE>(p, s);
         return cudaErrorNotSupported;
     }
-    if (p.channels <= kPer) return forward_as<T, 1, 1, MODE>(p, s);
-    if (p.channels <= 4 * kPer) return forward_as<T, 1, 4, MODE>(p, s);
+    if (p.channels <= 64) return forward_as<T, 1, 4, 1, MODE>(p, s);
+    if (p.channels <= 256) return forward_as<T, 1, 4, 4, MODE>(p, s);
     return cudaErrorNotSupported;
 }
 
 template <typename T, int MODE>
 cudaError_t backward_in(Problem& p, cudaStream_t s) {
-    constexpr int kPer = kEpt * kMaxWarps;
-    if (vectors_fit<T, 2>(p)) {
-        if (p.channels <= kPer) return backward_as<T, 2, 1, MODE>(p, s);
-        if (p.channels <= 2 * kPer) return backward_as<T, 2, 2, MODE>(p, s);
-        if (p.channels <= 8 * kPer) return backward_as<T, 2, 8, MODE>(p, s);
+    if (vectors_fit<T, 4>(p)) {
+        if (p.channels <= 64) return backward_as<T, 4, 2, 2, MODE>(p, s);
+        if (p.channels <= 128) return backward_as<T, 4, 2, 4, MODE>(p, s);
+        if (p.channels <= 512) return backward_as<T, 4, 2, 16, MODE>(p, s);
         return cudaErrorNotSupported;
     }
-    if (p.channels <= kPer) return backward_as<T, 1, 1, MODE>(p, s);
-    if (p.channels <= 4 * kPer) return backward_as<T, 1, 4, MODE>(p, s);
+    if (p.channels <= 64) return backward_as<T, 1, 4, 1, MODE>(p, s);
+    if (p.channels <= 256) return backward_as<T, 1, 4, 4, MODE>(p, s);
     return cudaErrorNotSupported;
 }
 

@@ -26,26 +26,38 @@ struct Team {
     __device__ __forceinline__ Team(int threads, float2* shared)
         : tpr(threads), me(threadIdx.x % threads), row(threadIdx.x / threads), rows(blockDim.x / threads), part(shared) {}
 
-    // Sums over the position's threads, the same bits in all of them.  `turn` alternates between
-    // calls, so that one barrier per call is enough.
-    __device__ __forceinline__ float2 sum(float a, float b, int& turn) {
-        for (int o = min(tpr, 32) / 2; o > 0; o >>= 1) {
-            a += __shfl_xor_sync(0xffffffffu, a, o);
-            b += __shfl_xor_sync(0xffffffffu, b, o);
+    // Sums over the position's threads, the same bits in all of them.  Across warps every warp adds
+    // the warps' parts itself; `turn` alternates between calls, so that one barrier per call is
+    // enough.
+    template <int K>
+    __device__ __forceinline__ void sum(float (&v)[K], int& turn) {
+        if (tpr < 32) {
+            for (int o = tpr / 2; o > 0; o >>= 1) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+            }
+            return;
         }
-        if (tpr <= 32) return make_float2(a, b);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+        }
+        if (tpr == 32) return;
         float2* now = part + turn * (kMaxThreads / 32);
         turn ^= 1;
-        if (threadIdx.x % 32 == 0) now[threadIdx.x / 32] = make_float2(a, b);
+        if (threadIdx.x % 32 == 0) now[threadIdx.x / 32] = make_float2(v[0], v[K - 1]);
         __syncthreads();
-        const int warps = tpr / 32;
-        const float2* mine = now + row * warps;
-        float2 s = mine[0];
-        for (int w = 1; w < warps; ++w) {
-            s.x += mine[w].x;
-            s.y += mine[w].y;
+        const int warps = tpr / 32;  // 2, 4, 8 or 16; the 16 lanes that hold more parts than there are hold zeros
+        const int lane = threadIdx.x % 16;
+        const float2 s = lane < warps ? now[row * warps + lane] : make_float2(0.f, 0.f);
+        v[0] = s.x;
+        v[K - 1] = s.y;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
         }
-        return s;
     }
 };
 
@@ -69,54 +81,74 @@ __device__ __forceinline__ void weights(const void* w, int c, bool live, bool wi
     }
 }
 
+// A thread's values lie in pairs of neighbours of its NV * VEC channels.
+template <int P>
+__device__ __forceinline__ float sum_of(const float2 (&v)[P]) {
+    float2 s = v[0];
+#pragma unroll
+    for (int i = 1; i < P; ++i) s = add2(s, v[i]);
+    return s.x + s.y;
+}
+
 // Mean and 1 / sqrt(variance + eps) of a position's values; vectors that do not exist hold zeros.
 template <int VEC, int NV>
-__device__ __forceinline__ float2 statistics(const Problem& p, Team& team, const float (&v)[NV * VEC],
+__device__ __forceinline__ float2 statistics(const Problem& p, Team& team, const float2 (&v)[NV * VEC / 2],
                                              const bool (&on)[NV], int& turn) {
-    float mean = 0.f, s = 0.f;
+    constexpr int P = NV * VEC / 2;
+    float mean = 0.f, s[1];
+    float2 d[P];
     if (p.kind == kLayer) {
+        s[0] = sum_of(v);
+        team.sum(s, turn);
+        mean = s[0] * p.inv_c;
 #pragma unroll
-        for (int i = 0; i < NV * VEC; ++i) s += v[i];
-        mean = team.sum(s, 0.f, turn).x * p.inv_c;
-        s = 0.f;
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-            if (on[j]) {
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) s = fmaf(v[j * VEC + i] - mean, v[j * VEC + i] - mean, s);
-            }
+        for (int i = 0; i < P; ++i) {
+            d[i] = add2(v[i], both(-mean));
+            if (!on[2 * i / VEC]) d[i].x = 0.f;
+            if (!on[(2 * i + 1) / VEC]) d[i].y = 0.f;
+            d[i] = mul2(d[i], d[i]);
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < NV * VEC; ++i) s = fmaf(v[i], v[i], s);
+        for (int i = 0; i < P; ++i) d[i] = mul2(v[i], v[i]);
     }
-    return make_float2(mean, 1.f / sqrtf(fmaf(team.sum(s, 0.f, turn).x, p.inv_c, p.eps)));
+    s[0] = sum_of(d);
+    team.sum(s, turn);
+    return make_float2(mean, rsqrtf(fmaf(s[0], p.inv_c, p.eps)));
+}
+
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void weight_pairs(const void* w, const Problem& p, const Team& team, float other,
+                                             float2 (&out)[NV * VEC / 2]) {
+    float v[NV][VEC];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (j * team.tpr + team.me) * VEC;
+        weights<T, VEC>(w, c, c < p.channels, p.wide, other, v[j]);
+    }
+#pragma unroll
+    for (int i = 0; i < NV * VEC / 2; ++i) out[i] = make_float2(v[2 * i / VEC][2 * i % VEC], v[(2 * i + 1) / VEC][(2 * i + 1) % VEC]);
 }
 
 // The weights of a thread's channels, the scale taken into those of the norm after the block.
 template <typename T, int VEC, int NV>
 struct Weights {
-    float w[NV * VEC], b[NV * VEC], w2[NV * VEC];
+    float2 w[NV * VEC / 2], b[NV * VEC / 2], w2[NV * VEC / 2];
 
     __device__ __forceinline__ Weights(const Problem& p, const Team& team, bool block) {
+        if (block) {
+            float2 scale[NV * VEC / 2];
+            weight_pairs<T, VEC, NV>(p.scale_w, p, team, 1.f, scale);
+            weight_pairs<T, VEC, NV>(p.post ? p.post_w : nullptr, p, team, 1.f, w);
+            weight_pairs<T, VEC, NV>(p.post ? p.post_b : nullptr, p, team, 0.f, b);
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int c = (j * team.tpr + team.me) * VEC;
-            const bool live = c < p.channels;
-            float v[VEC];
-            if (block) {
-                float scale[VEC];
-                weights<T, VEC>(p.scale_w, c, live, p.wide, 1.f, scale);
-                weights<T, VEC>(p.post ? p.post_w : nullptr, c, live, p.wide, 1.f, v);
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) w[j * VEC + i] = p.scale * scale[i] * v[i];
-                weights<T, VEC>(p.post ? p.post_b : nullptr, c, live, p.wide, 0.f, v);
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) b[j * VEC + i] = p.scale * scale[i] * v[i];
+            for (int i = 0; i < NV * VEC / 2; ++i) {
+                scale[i] = mul2(scale[i], both(p.scale));
+                w[i] = mul2(w[i], scale[i]);
+                b[i] = mul2(b[i], scale[i]);
             }
-            weights<T, VEC>(p.pre_w, c, live, p.wide, 1.f, v);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) w2[j * VEC + i] = v[i];
         }
+        weight_pairs<T, VEC, NV>(p.pre_w, p, team, 1.f, w2);
     }
 };
 
@@ -138,33 +170,46 @@ struct Slots {
     }
 
     static __device__ __forceinline__ void read(const E* slot, const void* from, size_t row, const Team& team,
-                                                int channels, bool here, float (&out)[NV * VEC]) {
+                                                int channels, bool here, float2 (&out)[NV * VEC / 2]) {
+        E v[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            E v{};
+            v[j] = E{};
             if constexpr (kCopied<E>) {
-                v = slot[j * blockDim.x];
+                v[j] = slot[j * blockDim.x];
             } else {
                 const int c = (j * team.tpr + team.me) * VEC;
-                if (here && c < channels) v = load_vec<T, VEC>(from, row + c);
+                if (here && c < channels) v[j] = load_vec<T, VEC>(from, row + c);
             }
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) out[j * VEC + i] = to_f32(v.v[i]);
         }
+#pragma unroll
+        for (int i = 0; i < NV * VEC / 2; ++i)
+            out[i] = unpack(v[2 * i / VEC].v[2 * i % VEC], v[(2 * i + 1) / VEC].v[(2 * i + 1) % VEC]);
     }
 
     static __device__ __forceinline__ void store(void* to, size_t row, const Team& team, int channels, bool here,
-                                                 const float (&v)[NV * VEC]) {
+                                                 const float2 (&v)[NV * VEC / 2]) {
+        E o[NV];
+#pragma unroll
+        for (int i = 0; i < NV * VEC / 2; ++i)
+            pack(o[2 * i / VEC].v[2 * i % VEC], o[(2 * i + 1) / VEC].v[(2 * i + 1) % VEC], v[i]);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = (j * team.tpr + team.me) * VEC;
-            E o;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) from_f32(o.v[i], v[j * VEC + i]);
-            if (here && c < channels) store_vec<T, VEC>(to, row + c, o);
+            if (here && c < channels) store_vec<T, VEC>(to, row + c, o[j]);
         }
     }
 };
+
+// Zeros where there is no channel.
+template <int VEC, int NV>
+__device__ __forceinline__ void clear_dead(float2 (&v)[NV * VEC / 2], const bool (&on)[NV]) {
+#pragma unroll
+    for (int i = 0; i < NV * VEC / 2; ++i) {
+        if (!on[2 * i / VEC]) v[i].x = 0.f;
+        if (!on[(2 * i + 1) / VEC]) v[i].y = 0.f;
+    }
+}
 
 __host__ __device__ constexpr int forward_tensors(int mode) { return mode == kNoBlock ? 1 : mode == kPlain ? 2 : 3; }
 __host__ __device__ constexpr int backward_tensors(int mode) { return mode == kNoBlock ? 3 : mode == kPlain ? 4 : 5; }
@@ -174,7 +219,7 @@ __host__ __device__ constexpr int backward_tensors(int mode) { return mode == kN
 template <typename T, int VEC, int NV, int MODE>
 __global__ void __launch_bounds__(kMaxThreads) token_forward_kernel(const __grid_constant__ Problem p, int tpr) {
     using F = Slots<T, VEC, NV>;
-    constexpr int N = NV * VEC, kTensors = forward_tensors(MODE);
+    constexpr int N = NV * VEC / 2, kTensors = forward_tensors(MODE);
     extern __shared__ __align__(16) unsigned char dynamic[];
     auto* part = reinterpret_cast<float2*>(dynamic);
     Team team(tpr, part);
@@ -210,41 +255,32 @@ __global__ void __launch_bounds__(kMaxThreads) token_forward_kernel(const __grid
         const int next = ring + kAhead >= kAhead + 1 ? ring - 1 : ring + kAhead;
         fetch(group + static_cast<long long>(kAhead) * gridDim.x, next);
         copy_wait<kAhead>();
-        float r[N];
-        float2 st = make_float2(0.f, 1.f), st2 = st;
+        float2 r[N], st = make_float2(0.f, 1.f), st2 = st;
         F::read(slot(ring, 0), p.x, row, team, channels, here, r);
         if constexpr (MODE != kNoBlock) {
-            float h[N], a[N];
+            float2 h[N], a[N];
             F::read(slot(ring, 1), p.y, row, team, channels, here, h);
             if constexpr (MODE == kFull) {
                 F::read(slot(ring, 2), p.gate, here ? gate_row(q) : 0, team, channels, here, a);
                 activate_all(a, p.act);
             }
             if (p.post) st = statistics<VEC, NV>(p, team, h, on, turn);
+            const float2 rho = both(st.y), shift = both(-st.x * st.y);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float z = fmaf((h[i] - st.x) * st.y, weight_of.w[i], weight_of.b[i]);
-                r[i] = MODE == kPlain ? r[i] + z : fmaf(a[i], z, r[i]);
+                const float2 z = fma2(fma2(h[i], rho, shift), weight_of.w[i], weight_of.b[i]);
+                r[i] = MODE == kPlain ? add2(r[i], z) : fma2(a[i], z, r[i]);
             }
-            // vectors past the last channel hold -mean rho w + b: back to zero for the next statistic
-#pragma unroll
-            for (int j = 0; j < NV; ++j)
-                if (!on[j]) {
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) r[j * VEC + i] = 0.f;
-                }
             F::store(p.r, row, team, channels, here, r);
+            clear_dead<VEC, NV>(r, on);
         }
         if (p.pre) {
             st2 = statistics<VEC, NV>(p, team, r, on, turn);
+            const float2 rho = both(st2.y), shift = both(-st2.x * st2.y);
+            float2 b[N];
+            weight_pairs<T, VEC, NV>(p.pre_b, p, team, 0.f, b);
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                float b[VEC];
-                weights<T, VEC>(p.pre_b, (j * tpr + team.me) * VEC, on[j], p.wide, 0.f, b);
-#pragma unroll
-                for (int i = 0; i < VEC; ++i)
-                    r[j * VEC + i] = fmaf((r[j * VEC + i] - st2.x) * st2.y, weight_of.w2[j * VEC + i], b[i]);
-            }
+            for (int i = 0; i < N; ++i) r[i] = fma2(fma2(r[i], rho, shift), weight_of.w2[i], b[i]);
             F::store(p.n, row, team, channels, here, r);
         }
         if (p.stats && team.me == 0 && here) {
@@ -261,14 +297,20 @@ __global__ void __launch_bounds__(kMaxThreads) token_forward_kernel(const __grid
 // Sums over a block's positions: the rows' threads of one channel are added through shared memory in
 // row order.  Every thread of the block calls it.
 template <int VEC, int NV>
-__device__ void store_sums(const Problem& p, const Team& team, float* shared, const float (&sum)[NV * VEC], float* out) {
+__device__ void store_sums(const Problem& p, const Team& team, float* shared, const float2 (&sum)[NV * VEC / 2], float* out) {
+    float v[NV * VEC];
+#pragma unroll
+    for (int i = 0; i < NV * VEC / 2; ++i) {
+        v[2 * i] = sum[i].x;
+        v[2 * i + 1] = sum[i].y;
+    }
     if (team.rows > 1) {
         __syncthreads();
         const int width = team.tpr * VEC * NV;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) shared[team.row * width + (j * team.tpr + team.me) * VEC + i] = sum[j * VEC + i];
+            for (int i = 0; i < VEC; ++i) shared[team.row * width + (j * team.tpr + team.me) * VEC + i] = v[j * VEC + i];
         __syncthreads();
         for (int c = threadIdx.x; c < p.channels; c += blockDim.x) {
             float s = 0.f;
@@ -277,22 +319,17 @@ __device__ void store_sums(const Problem& p, const Team& team, float* shared, co
         }
         return;
     }
+    constexpr int kPer = VEC < 4 ? VEC : 4;  // VEC >= 4 divides the channels, so `out` starts on 16 bytes
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int c = (j * team.tpr + team.me) * VEC;
         if (c >= p.channels) continue;
-        Vec<float, VEC> o;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o.v[i] = sum[j * VEC + i];
-        if (p.channels % 4 == 0) {  // every array of the workspace then starts on 16 bytes
+        for (int i = 0; i < VEC; i += kPer) {
+            Vec<float, kPer> o;
 #pragma unroll
-            for (int i = 0; i < VEC; i += (VEC < 4 ? VEC : 4))
-                *reinterpret_cast<Vec<float, (VEC < 4 ? VEC : 4)>*>(out + c + i) =
-                    *reinterpret_cast<const Vec<float, (VEC < 4 ? VEC : 4)>*>(o.v + i);
-        } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i)
-                if (c + i < p.channels) out[c + i] = o.v[i];
+            for (int k = 0; k < kPer; ++k) o.v[k] = v[j * VEC + i + k];
+            store_vec<float, kPer>(out, c + i, o);
         }
     }
 }
@@ -300,7 +337,7 @@ __device__ void store_sums(const Problem& p, const Team& team, float* shared, co
 template <typename T, int VEC, int NV, int MODE>
 __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __grid_constant__ Problem p, int tpr) {
     using F = Slots<T, VEC, NV>;
-    constexpr int N = NV * VEC, kTensors = backward_tensors(MODE);
+    constexpr int N = NV * VEC / 2, kTensors = backward_tensors(MODE);
     // the tensors' places in a ring slot
     constexpr int kX = 0, kDn = 1, kDr = 2, kY = 3, kGate = 4;
     extern __shared__ __align__(16) unsigned char dynamic[];
@@ -341,98 +378,121 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) fetch(first + k, k);
     const Weights<T, VEC, NV> weight_of(p, team, MODE != kNoBlock);
-    float dw2[N] = {}, db2[N] = {}, tah[N] = {}, ta[N] = {};
+    float2 dw2[N], db2[N], tah[N], ta[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) dw2[i] = db2[i] = tah[i] = ta[i] = both(0.f);
+    bool on[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) on[j] = (j * tpr + team.me) * VEC < channels;
     int turn = 0, ring = 0;
     for (long long tile = first; tile < last; ++tile) {
         const At at = at_of(tile);
         const size_t row = static_cast<size_t>(at.q) * channels;
         const size_t gate_row = p.gate_mode == kGateSample ? static_cast<size_t>(at.sample) * channels : row;
-        float mean = 0.f, rho = 0.f, mean2 = 0.f, rho2 = 0.f;
+        float2 rho = both(0.f), shift = both(0.f), rho2 = both(0.f), shift2 = both(0.f);
         if (at.here) {
-            mean = p.post ? p.stats[at.q] : 0.f;
-            rho = p.post ? p.stats[p.positions + at.q] : 1.f;
+            rho = both(1.f);
+            if (p.post) {
+                rho = both(p.stats[p.positions + at.q]);
+                shift = both(-p.stats[at.q] * rho.x);
+            }
             if (p.dn) {
-                mean2 = p.stats[2 * p.positions + at.q];
-                rho2 = p.stats[3 * p.positions + at.q];
+                rho2 = both(p.stats[3 * p.positions + at.q]);
+                shift2 = both(-p.stats[2 * p.positions + at.q] * rho2.x);
             }
         }
         fetch(tile + kAhead, ring == 0 ? kAhead : ring - 1);
         copy_wait<kAhead>();
-        float h[N], a[N], k[N], g[N];
+        // s: the sigmoid of the gate, or its plain value; the gate itself is read again where silu needs
+        // it, since registers are what this kernel is short of
+        float2 h[N], s[N], k[N], g[N];
+        auto gate_of = [&](float2 (&a)[N]) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) a[i] = s[i];
+            if (p.act == kActSilu) {
+                F::read(slot(ring, kGate), p.gate, gate_row, team, channels, at.here, a);
+#pragma unroll
+                for (int i = 0; i < N; ++i) a[i] = mul2(a[i], s[i]);
+            }
+        };
         if constexpr (MODE != kNoBlock) {
             F::read(slot(ring, kY), p.y, row, team, channels, at.here, h);
 #pragma unroll
-            for (int i = 0; i < N; ++i) h[i] = (h[i] - mean) * rho;
+            for (int i = 0; i < N; ++i) h[i] = fma2(h[i], rho, shift);
             if constexpr (MODE == kFull) {
-                F::read(slot(ring, kGate), p.gate, gate_row, team, channels, at.here, a);
-                activate_all(a, p.act);
+                F::read(slot(ring, kGate), p.gate, gate_row, team, channels, at.here, s);
+                if (p.act != kActNone) activate_all(s, kActSigmoid);
             }
         }
         if (p.dn) {
             F::read(slot(ring, kX), p.x, row, team, channels, at.here, k);
             F::read(slot(ring, kDn), p.dn, row, team, channels, at.here, g);  // zeros where there is no channel
-            float s0 = 0.f, s1 = 0.f;
+            float2 a[N];
+            if constexpr (MODE == kFull) gate_of(a);
+            float2 s0 = both(0.f), s1 = both(0.f);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 if constexpr (MODE != kNoBlock) {
-                    const float z = fmaf(h[i], weight_of.w[i], weight_of.b[i]);
-                    k[i] = MODE == kPlain ? k[i] + z : fmaf(a[i], z, k[i]);
+                    const float2 z = fma2(h[i], weight_of.w[i], weight_of.b[i]);
+                    k[i] = MODE == kPlain ? add2(k[i], z) : fma2(a[i], z, k[i]);
                 }
-                k[i] = (k[i] - mean2) * rho2;
-                dw2[i] = fmaf(g[i], k[i], dw2[i]);
-                db2[i] += g[i];
-                g[i] *= weight_of.w2[i];
-                s0 += g[i];
-                s1 = fmaf(g[i], k[i], s1);
+                k[i] = fma2(k[i], rho2, shift2);
+                dw2[i] = fma2(g[i], k[i], dw2[i]);
+                db2[i] = add2(db2[i], g[i]);
+                g[i] = mul2(g[i], weight_of.w2[i]);
+                s0 = add2(s0, g[i]);
+                s1 = fma2(g[i], k[i], s1);
             }
-            const float2 m = team.sum(s0, s1, turn);
-            const float m1 = p.kind == kLayer ? m.x * p.inv_c : 0.f, m2 = m.y * p.inv_c;
+            float m[2] = {s0.x + s0.y, s1.x + s1.y};
+            team.sum(m, turn);
+            const float2 m1 = both(p.kind == kLayer ? -m[0] * p.inv_c : 0.f), m2 = both(-m[1] * p.inv_c);
 #pragma unroll
-            for (int i = 0; i < N; ++i) g[i] = rho2 * (g[i] - m1 - k[i] * m2);
+            for (int i = 0; i < N; ++i) g[i] = mul2(rho2, add2(fma2(k[i], m2, g[i]), m1));
         } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) g[i] = 0.f;
+            for (int i = 0; i < N; ++i) g[i] = both(0.f);
         }
         if (p.dr) {
             F::read(slot(ring, kDr), p.dr, row, team, channels, at.here, k);
 #pragma unroll
-            for (int i = 0; i < N; ++i) g[i] += k[i];
+            for (int i = 0; i < N; ++i) g[i] = add2(g[i], k[i]);
         }
-        // g: the gradient of r; back to zero where there is no channel
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-            if ((j * tpr + team.me) * VEC >= channels) {
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) g[j * VEC + i] = 0.f;
-            }
+        clear_dead<VEC, NV>(g, on);
+        // g: the gradient of r
         if (p.dx) F::store(p.dx, row, team, channels, at.here, g);
         if constexpr (MODE != kNoBlock) {
-            float s0 = 0.f, s1 = 0.f;
+            float2 s0 = both(0.f), s1 = both(0.f), a[N];
+            if constexpr (MODE == kFull) {
+                gate_of(a);
+                if (p.dgate && p.gate_mode == kGateFull) {
+                    float2 o[N];
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const float2 rest = make_float2(1.f - s[i].x, 1.f - s[i].y);
+                        o[i] = p.act == kActSilu ? fma2(a[i], rest, s[i])
+                                                 : p.act == kActSigmoid ? mul2(s[i], rest) : both(1.f);
+                        o[i] = mul2(mul2(g[i], fma2(h[i], weight_of.w[i], weight_of.b[i])), o[i]);
+                    }
+                    F::store(p.dgate, row, team, channels, at.here, o);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float v = MODE == kPlain ? g[i] : g[i] * a[i];
-                const float kept = p.slots ? g[i] : v;
-                tah[i] = fmaf(kept, h[i], tah[i]);
-                ta[i] += kept;
-                k[i] = v * weight_of.w[i];
-                s0 += k[i];
-                s1 = fmaf(k[i], h[i], s1);
-            }
-            if (MODE == kFull && p.dgate && p.gate_mode == kGateFull) {
-                // the gate again, for its slope: registers are what this kernel is short of
-                float slope[N];
-                F::read(slot(ring, kGate), p.gate, gate_row, team, channels, at.here, a);
-                activate_all(a, slope, p.act);
-#pragma unroll
-                for (int i = 0; i < N; ++i) a[i] = g[i] * fmaf(h[i], weight_of.w[i], weight_of.b[i]) * slope[i];
-                F::store(p.dgate, row, team, channels, at.here, a);
+                const float2 v = MODE == kPlain ? g[i] : mul2(g[i], a[i]);
+                const float2 kept = p.slots ? g[i] : v;
+                tah[i] = fma2(kept, h[i], tah[i]);
+                ta[i] = add2(ta[i], kept);
+                k[i] = mul2(v, weight_of.w[i]);
+                s0 = add2(s0, k[i]);
+                s1 = fma2(k[i], h[i], s1);
             }
             if (p.dy) {
                 if (p.post) {
-                    const float2 m = team.sum(s0, s1, turn);
-                    const float m3 = p.kind == kLayer ? m.x * p.inv_c : 0.f, m4 = m.y * p.inv_c;
+                    float m[2] = {s0.x + s0.y, s1.x + s1.y};
+                    team.sum(m, turn);
+                    const float2 m3 = both(p.kind == kLayer ? -m[0] * p.inv_c : 0.f), m4 = both(-m[1] * p.inv_c);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) k[i] = rho * (k[i] - m3 - h[i] * m4);
+                    for (int i = 0; i < N; ++i) k[i] = mul2(rho, add2(fma2(h[i], m4, k[i]), m3));
                 }
                 F::store(p.dy, row, team, channels, at.here, k);
             }
@@ -444,7 +504,7 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
                 store_sums<VEC, NV>(p, team, meet, tah, to);
                 store_sums<VEC, NV>(p, team, meet, ta, to + channels);
 #pragma unroll
-                for (int i = 0; i < N; ++i) tah[i] = ta[i] = 0.f;
+                for (int i = 0; i < N; ++i) tah[i] = ta[i] = both(0.f);
             }
         }
         ring = ring == kAhead ? 0 : ring + 1;
@@ -494,6 +554,7 @@ cudaError_t backward_as(Problem& p, cudaStream_t s) {
     p.tiles_per_sample = (p.length + rows - 1) / rows;
     p.tiles = p.batch * p.tiles_per_sample;
     p.parts = static_cast<int>(std::min<long long>(std::min(max_parts(p.channels), per_sm * scx::num_sms()), p.tiles));
+    p.partials = p.parts;
     token_backward_kernel<T, VEC, NV, MODE><<<p.parts, threads, smem, s>>>(p, tpr);
     return cudaGetLastError();
 }
