@@ -14,81 +14,17 @@ repeatable.  A failed check raises RuntimeError.
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
 
-import _scx
+import _scx  # noqa: F401  (loads libscx.so, with its message where that is missing)
+import _scx_torch
 from spectral_conv_ext import _check
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _KINDS = {"rms": 0, "layer": 1}
 _ACTIVATIONS = {"none": 0, "sigmoid": 1, "silu": 2}
-
-
-def _ptr(t: torch.Tensor | None) -> int | None:
-    return t.data_ptr() if t is not None else None
-
-
-def _tensors(x, y, gate, post_weight, post_bias, pre_weight, pre_bias, scale, r=None, n=None, stats=None):
-    return _scx.ResidualNormTensors(x.data_ptr(), _ptr(y), _ptr(gate), _ptr(post_weight), _ptr(post_bias),
-                                    _ptr(pre_weight), _ptr(pre_bias), _ptr(scale), _ptr(r), _ptr(n), _ptr(stats))
-
-
-def _forward(config, x, y, gate, vectors, keep_stats: bool):
-    """(r or None, n or None, stats or None) of contiguous inputs."""
-    r = torch.empty_like(x) if y is not None else None
-    n = torch.empty_like(x) if config.pre_norm else None
-    stats = None
-    if keep_stats:
-        stats = torch.empty(4, config.batch * config.length, dtype=torch.float32, device=x.device)
-    with _scx.device_guard(x.device):
-        t = _tensors(x, y, gate, *vectors, r, n, stats)
-        _scx.check(_scx.lib.scx_residual_norm_fwd(ctypes.addressof(config), ctypes.addressof(t),
-                                                  _scx.stream_of(x.device)), "scx_residual_norm_fwd")
-    return r, n, stats
-
-
-class ResidualNormFunction(torch.autograd.Function):
-    """Autograd form of ``residual_norm``.  Keeps the inputs and four statistics per position; r is
-    recomputed in the backward."""
-
-    @staticmethod
-    def forward(ctx, config, x, y, gate, post_weight, post_bias, pre_weight, pre_bias, scale):
-        r, n, stats = _forward(config, x, y, gate, (post_weight, post_bias, pre_weight, pre_bias, scale), True)
-        ctx.config = config
-        ctx.save_for_backward(x, y, gate, post_weight, post_bias, pre_weight, pre_bias, scale, stats)
-        ctx.set_materialize_grads(False)
-        # without y, r is x: returned from here so that its gradient joins n's before the rounding
-        return (x if y is None else r), n
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dr, dn):
-        x, y, gate, *vectors, stats = ctx.saved_tensors
-        none = (None,) * 9
-        if dr is None and dn is None:
-            return none
-        if x.numel() == 0:
-            return (None, *[torch.zeros_like(t) if t is not None and need else None
-                            for t, need in zip((x, y, gate, *vectors), ctx.needs_input_grad[1:])])
-        dr = dr.contiguous() if dr is not None else None
-        dn = dn.contiguous() if dn is not None else None
-        grads = [torch.empty_like(t) if t is not None and need else None
-                 for t, need in zip((x, y, gate, *vectors), ctx.needs_input_grad[1:])]
-        config = ctx.config
-        dx, dy, dgate, d_post_w, d_post_b, d_pre_w, d_pre_b, d_scale = grads
-        with _scx.device_guard(x.device):
-            nbytes = _scx.lib.scx_residual_norm_bwd_workspace_size(ctypes.addressof(config))
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-            t = _tensors(x, y, gate, *vectors, stats=stats)
-            g = _scx.ResidualNormGrads(_ptr(dr), _ptr(dn), _ptr(dx), _ptr(dy), _ptr(dgate), _ptr(d_post_w),
-                                       _ptr(d_post_b), _ptr(d_pre_w), _ptr(d_pre_b), _ptr(d_scale))
-            _scx.check(_scx.lib.scx_residual_norm_bwd(ctypes.addressof(config), ctypes.addressof(t),
-                                                      ctypes.addressof(g), ws.data_ptr(), nbytes,
-                                                      _scx.stream_of(x.device)), "scx_residual_norm_bwd")
-        return (None, *grads)
 
 
 def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *, pre_weight: torch.Tensor | None = None,
@@ -164,12 +100,6 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *, pre_weight:
                 _check(wide is None and (v.dtype is torch.float32 or v.dtype is dtype),
                        "weights, biases and scale must all be float32 or all of x's type")
                 wide = v.dtype
-    config = _scx.ResidualNormConfig(batch, length, channels, last, _TYPES[dtype],
-                                     _TYPES[wide or torch.float32], _KINDS[kind], mode,
-                                     _ACTIVATIONS[gate_activation], bool(post_norm), bool(pre_norm), eps, number)
-    wanted = torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in (x, y, gate, *vectors)])
-    args = [t if t is None or t.is_contiguous() else t.contiguous() for t in (x, y, gate, *vectors)]
-    if wanted:
-        return ResidualNormFunction.apply(config, *args)
-    r, n, _ = _forward(config, args[0], args[1], args[2], args[3:], False)
-    return (x if y is None else r), n
+    options = [batch, length, channels, last, _TYPES[dtype], _TYPES[wide or torch.float32], _KINDS[kind], mode,
+               _ACTIVATIONS[gate_activation], bool(post_norm), bool(pre_norm)]
+    return _scx_torch.residual_norm(options, eps, number, x, y, gate, *vectors)

@@ -80,6 +80,14 @@ def test_python_refusals():
             op(*args, **kwargs)
 
 
+def test_the_binding_formats_its_messages():
+    """Numbers in a message go through the C++ runtime's streams, which have to be torch's."""
+    import _scx_torch
+
+    with pytest.raises(RuntimeError, match="11 options, got 2"):
+        _scx_torch.residual_norm([1, 2], 0.0, 1.0, torch.zeros(2, 2), None, None, None, None, None, None, None)
+
+
 class _Cuda(torch.Tensor):
     """A host tensor that claims to be on the device, for the checks behind that one."""
 

@@ -6,7 +6,6 @@ from __future__ import annotations
 import pytest
 import torch
 
-import residual_norm_ops
 from residual_norm_ops import residual_norm
 from residual_norm_reference import like, reference, rows_of, within
 
@@ -191,6 +190,15 @@ def test_layouts_strides_and_offsets(cuda_device):
         torch.testing.assert_close(leaf.grad, g, rtol=1e-5, atol=1e-5)
 
 
+def test_a_second_derivative_is_refused(cuda_device):
+    x = torch.randn(3, 8, device=cuda_device, requires_grad=True)
+    y = torch.randn(3, 8, device=cuda_device, requires_grad=True)
+    r, n = residual_norm(x, y)
+    gx, gy = torch.autograd.grad((r * r).sum() + (n * n).sum(), (x, y), create_graph=True)
+    with pytest.raises(RuntimeError, match="once only"):
+        (gx.sum() + gy.sum()).backward()
+
+
 def test_empty(cuda_device):
     for shape, dim in (((0, 5, 8), -1), ((3, 0, 8), -1), ((0, 8, 4), 1), ((2, 8, 0), 1)):
         x = torch.zeros(shape, device=cuda_device, requires_grad=True)
@@ -304,4 +312,3 @@ def test_other_types_on_the_device_are_refused(cuda_device):
         residual_norm(x, pre_weight=torch.ones(4))
     with pytest.raises(RuntimeError, match="float32"):
         residual_norm(x.double())
-    assert residual_norm_ops.ResidualNormFunction is not None
