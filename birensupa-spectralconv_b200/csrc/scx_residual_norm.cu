@@ -300,63 +300,95 @@ __global__ void __launch_bounds__(kAnyThreads) any_sums_kernel(const __grid_cons
 
 // ---------------------------------------------------------------------------- the last sums
 
-constexpr int kFinishRows = 32;
+constexpr int kFinishChannels = 8, kFinishRows = 64;
+constexpr int kFinishThreads = kFinishChannels * kFinishRows;
 
-// Adds the blocks' partials per channel (in 64 bits and a fixed order), and the slots of each sample
-// into the gradient of its gate.  Grid (channels / 32, 2): the norm before the next block, then
-// the norm after the block, the scale and the gate.  Block 32 channels x kFinishRows.
+// Sums over a block's rows, in 64 bits and a fixed order; valid in row 0.
+__device__ double2 sum_rows(double2 v) {
+    __shared__ double2 red[kFinishThreads / 32][kFinishChannels];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    for (int o = 16; o >= kFinishChannels; o /= 2) {
+        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+    __syncthreads();
+    if (lane < kFinishChannels) red[warp][lane] = v;
+    __syncthreads();
+    if (threadIdx.x < kFinishChannels) {
+        for (int k = 1; k < kFinishThreads / 32; ++k) {
+            v.x += red[k][lane].x;
+            v.y += red[k][lane].y;
+        }
+    }
+    return v;
+}
+
+// Adds the parts' sums per channel, and the slots of each sample into the gradient of its gate.  Grid
+// (channels / 8, 2 + samples): y = 0 the norm before the next block, 1 the norm after the block and
+// the scale, from 2 on the gates.  Latency is all there is to it (a few hundred rows per channel):
+// narrow blocks and 64 rows of threads keep the chains of loads short (8 us at 32 rows of 32
+// channels, under 4 us so).
 template <typename T>
-__global__ void __launch_bounds__(32 * kFinishRows) finish_kernel(const __grid_constant__ Problem p) {
-    __shared__ double red[2][kFinishRows][33];
-    grid_dep_wait();
-    const int lane = threadIdx.x % 32, row = threadIdx.x / 32;
-    const int c = blockIdx.x * 32 + lane;
+__global__ void __launch_bounds__(kFinishThreads) finish_kernel(const __grid_constant__ Problem p) {
+    const int row = threadIdx.x / kFinishChannels;
+    const int c = blockIdx.x * kFinishChannels + threadIdx.x % kFinishChannels;
     const bool live = c < p.channels;
-    const bool second = blockIdx.y == 1;
     const float w = live ? weight<T>(p.post_w, c, p.wide, 1.f) : 0.f, b = live ? weight<T>(p.post_b, c, p.wide, 0.f) : 0.f;
     const float scale = p.scale * (live ? weight<T>(p.scale_w, c, p.wide, 1.f) : 0.f);
-    double s0 = 0.0, s1 = 0.0;
-    if (live && second && p.slots) {
-        for (long long s = row; s < p.batch; s += kFinishRows) {
-            double th = 0.0, t = 0.0;
-            const long long to = part_of_tile(p, (s + 1) * p.tiles_per_sample - 1);
-            for (long long k = part_of_tile(p, s * p.tiles_per_sample); k <= to; ++k) {
-                const float* slot = slot_of(p, k, s);
-                th += slot[c];
-                t += slot[static_cast<size_t>(p.channels) + c];
-            }
-            const size_t g = static_cast<size_t>(s) * p.channels + c;
+    auto add_slot = [&](double2& s, long long part, long long sample, double a) {
+        const float* slot = slot_of(p, part, sample) + c;
+        s.x += a * slot[0];
+        s.y += a * slot[p.channels];
+    };
+    grid_dep_wait();
+    if (blockIdx.y >= 2) {
+        for (long long sample = blockIdx.y - 2; sample < p.batch; sample += gridDim.y - 2) {
+            double2 s = make_double2(0.0, 0.0);
+            const long long last = part_of_tile(p, (sample + 1) * p.tiles_per_sample - 1);
+#pragma unroll 4
+            for (long long k = part_of_tile(p, sample * p.tiles_per_sample) + row; k <= last; k += kFinishRows)
+                if (live) add_slot(s, k, sample, 1.0);
+            s = sum_rows(s);
+            if (row != 0 || !live) continue;
+            const size_t g = static_cast<size_t>(sample) * p.channels + c;
             float slope;
-            const float a = activate(to_f32(static_cast<const T*>(p.gate)[g]), p.act, slope);
-            if (p.dgate)
-                from_f32(static_cast<T*>(p.dgate)[g], static_cast<float>(w * th + b * t) * scale * slope);
-            s0 += a * th;
-            s1 += a * t;
+            activate(to_f32(static_cast<const T*>(p.gate)[g]), p.act, slope);
+            from_f32(static_cast<T*>(p.dgate)[g], static_cast<float>(w * s.x + b * s.y) * scale * slope);
+        }
+        return;
+    }
+    const bool second = blockIdx.y == 1;
+    double2 s = make_double2(0.0, 0.0);
+    if (second && p.slots) {
+        // the rows share out the samples, as many rows to a sample as there are
+        int groups = 1;
+        while (groups < kFinishRows && groups < p.batch) groups *= 2;
+        const int per_sample = kFinishRows / groups;
+        for (long long sample = row / per_sample; live && sample < p.batch; sample += groups) {
+            const float a = activate(to_f32(static_cast<const T*>(p.gate)[static_cast<size_t>(sample) * p.channels + c]), p.act);
+            const long long last = part_of_tile(p, (sample + 1) * p.tiles_per_sample - 1);
+#pragma unroll 4
+            for (long long k = part_of_tile(p, sample * p.tiles_per_sample) + row % per_sample; k <= last; k += per_sample)
+                add_slot(s, k, sample, a);
         }
     } else if (live) {
         const float* from = p.partial + static_cast<size_t>(second ? kTah : kDPreW) * p.channels + c;
-#pragma unroll 4
+#pragma unroll 8
         for (int k = row; k < p.partials; k += kFinishRows) {
             const float* at = from + static_cast<size_t>(k) * kSums * p.channels;
-            s0 += at[0];
-            s1 += at[p.channels];
+            s.x += at[0];
+            s.y += at[p.channels];
         }
     }
-    red[0][row][lane] = s0;
-    red[1][row][lane] = s1;
-    __syncthreads();
+    s = sum_rows(s);
     if (row != 0 || !live) return;
-    for (int k = 1; k < kFinishRows; ++k) {
-        s0 += red[0][k][lane];
-        s1 += red[1][k][lane];
-    }
     if (!second) {
-        if (p.d_pre_w) store_weight<T>(p.d_pre_w, c, p.wide, static_cast<float>(s0));
-        if (p.d_pre_b) store_weight<T>(p.d_pre_b, c, p.wide, static_cast<float>(s1));
+        if (p.d_pre_w) store_weight<T>(p.d_pre_w, c, p.wide, static_cast<float>(s.x));
+        if (p.d_pre_b) store_weight<T>(p.d_pre_b, c, p.wide, static_cast<float>(s.y));
     } else {
-        if (p.d_post_w) store_weight<T>(p.d_post_w, c, p.wide, static_cast<float>(scale * s0));
-        if (p.d_post_b) store_weight<T>(p.d_post_b, c, p.wide, static_cast<float>(scale * s1));
-        if (p.d_scale) store_weight<T>(p.d_scale, c, p.wide, static_cast<float>(p.scale * (w * s0 + b * s1)));
+        if (p.d_post_w) store_weight<T>(p.d_post_w, c, p.wide, static_cast<float>(scale * s.x));
+        if (p.d_post_b) store_weight<T>(p.d_post_b, c, p.wide, static_cast<float>(scale * s.y));
+        if (p.d_scale) store_weight<T>(p.d_scale, c, p.wide, static_cast<float>(p.scale * (w * s.x + b * s.y)));
     }
 }
 
@@ -491,7 +523,9 @@ cudaError_t backward(Problem& p, cudaStream_t s) {
     cudaError_t e = p.channels_last ? token_backward<T>(p, s) : field_backward<T>(p, s);
     if (e == cudaErrorNotSupported) e = any_backward<T>(p, s);
     if (e != cudaSuccess || !p.sums) return e;
-    return scx::launch_chained(finish_kernel<T>, dim3((p.channels + 31) / 32, 2), dim3(32 * kFinishRows), 0, s, p);
+    const int gates = p.slots && p.dgate ? static_cast<int>(std::min<long long>(p.batch, 1024)) : 0;
+    return scx::launch_chained(finish_kernel<T>, dim3((p.channels + kFinishChannels - 1) / kFinishChannels, 2 + gates),
+                               dim3(kFinishThreads), 0, s, p);
 }
 
 }  // namespace

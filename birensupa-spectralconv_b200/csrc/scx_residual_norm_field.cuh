@@ -2,7 +2,7 @@
 // `length` elements apart, so a warp takes neighbouring positions of a few channels, and a block's
 // warps together all channels of a tile of positions.
 //
-// A thread has V neighbouring positions (one access) of EPT channels, 8 values for V = 4, and every
+// A thread has V neighbouring positions (one access) of EPT channels, 8 values, and every
 // tensor is read once: the next tile's values are copied into the thread's own slots in shared
 // memory while this tile's are in registers.  A warp's 32 lanes are 32/LC positions x LC channel
 // groups: LC = 2 keeps accesses of 16 bytes and warps of 4 channels, larger LC serves channel counts
@@ -244,20 +244,33 @@ __device__ __forceinline__ void two_means(Shared<V, EPT, LC>& sh, const Problem&
     });
 }
 
-// Where a tile lies, for one thread.
+// Where a tile lies, for one thread; moved on by a fixed number of tiles without a division.
 template <int V, int EPT, int LC>
 struct Tile {
-    int sample, l0;
-    bool live;    // whether the thread's positions exist
-    size_t base;  // the thread's first element
+    int sample, index;  // the tile's index in its sample
+    int step_samples, step_index, per_sample;
 
-    __device__ __forceinline__ Tile(const Problem& p, const Where& at, int tile) {
-        const int ts = static_cast<int>(p.tiles_per_sample);
-        sample = tile / ts;
-        l0 = (tile - sample * ts) * Shape<V, EPT, LC>::kPos;
-        const int l = l0 + at.pos * V;
-        live = l < static_cast<int>(p.length);
-        base = (static_cast<size_t>(sample) * p.channels + at.c0) * p.length + l;
+    __device__ __forceinline__ Tile(const Problem& p, int tile, int step) : per_sample(static_cast<int>(p.tiles_per_sample)) {
+        sample = tile / per_sample;
+        index = tile - sample * per_sample;
+        step_samples = step / per_sample;
+        step_index = step - step_samples * per_sample;
+    }
+    __device__ __forceinline__ void next() {
+        sample += step_samples;
+        index += step_index;
+        if (index >= per_sample) {
+            index -= per_sample;
+            ++sample;
+        }
+    }
+    __device__ __forceinline__ int l0() const { return index * Shape<V, EPT, LC>::kPos; }
+    // whether the thread's positions exist, and its first element
+    __device__ __forceinline__ bool live(const Problem& p, const Where& at) const {
+        return l0() + at.pos * V < static_cast<int>(p.length);
+    }
+    __device__ __forceinline__ size_t base(const Problem& p, const Where& at) const {
+        return (static_cast<size_t>(sample) * p.channels + at.c0) * p.length + (l0() + at.pos * V);
     }
 };
 
@@ -333,45 +346,48 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) field_forward_kernel(const 
     constexpr int kTensors = forward_tensors(MODE);
     auto* slots = reinterpret_cast<typename F::E*>(dynamic + sizeof(sh)) + threadIdx.x;
     auto slot = [&](int turn, int tensor) { return slots + (turn * kTensors + tensor) * EPT * blockDim.x; };
-    auto fetch = [&](int tile, int turn) {
-        if (tile < tiles) {
-            const Tile<V, EPT, LC> t(p, at, tile);
-            const int end = t.live ? at.mine : 0;
-            F::fetch(slot(turn, 0), p.x, t.base, stride, end);
-            if constexpr (MODE != kNoBlock) F::fetch(slot(turn, 1), p.y, t.base, stride, end);
-            if constexpr (MODE == kFull) F::fetch(slot(turn, 2), p.gate, t.base, stride, end);
+    using TILE = Tile<V, EPT, LC>;
+    auto fetch = [&](const TILE& t, bool exists, int turn) {
+        if (exists) {
+            const size_t base = t.base(p, at);
+            const int end = t.live(p, at) ? at.mine : 0;
+            F::fetch(slot(turn, 0), p.x, base, stride, end);
+            if constexpr (MODE != kNoBlock) F::fetch(slot(turn, 1), p.y, base, stride, end);
+            if constexpr (MODE == kFull) F::fetch(slot(turn, 2), p.gate, base, stride, end);
         }
         copy_commit();
     };
-    fetch(blockIdx.x, 0);
+    TILE t(p, blockIdx.x, gridDim.x);
+    fetch(t, static_cast<int>(blockIdx.x) < tiles, 0);
     load_vectors<T>(sh, p, at.warps * EPT * LC);
     int turn = 0;
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
-        const Tile<V, EPT, LC> t(p, at, tile);
-        const int end = t.live ? at.mine : 0;
-        const size_t q0 = static_cast<size_t>(t.sample) * p.length + t.l0;
-        const int live_pos = static_cast<int>(p.length) - t.l0;
-        fetch(tile + gridDim.x, turn ^ 1);
+        const size_t base = t.base(p, at);
+        const int end = t.live(p, at) ? at.mine : 0, sample = t.sample;
+        const size_t q0 = static_cast<size_t>(sample) * p.length + t.l0();
+        const int live_pos = static_cast<int>(p.length) - t.l0();
+        t.next();
+        fetch(t, tile + static_cast<int>(gridDim.x) < tiles, turn ^ 1);
         copy_wait<1>();
         float2 r[P::kCount], rho[P::kSpots], shift[P::kSpots];
-        F::read(slot(turn, 0), p.x, t.base, stride, end, r);
+        F::read(slot(turn, 0), p.x, base, stride, end, r);
         if constexpr (MODE != kNoBlock) {
             float2 h[P::kCount], a[P::kCount];
-            F::read(slot(turn, 1), p.y, t.base, stride, end, h);
-            if constexpr (MODE == kFull) F::read(slot(turn, 2), p.gate, t.base, stride, end, a);
+            F::read(slot(turn, 1), p.y, base, stride, end, h);
+            if constexpr (MODE == kFull) F::read(slot(turn, 2), p.gate, base, stride, end, a);
             if (p.post) {
                 statistics<V, EPT, LC>(sh, p, h, at, rho, shift, p.stats ? p.stats + q0 : nullptr, live_pos);
 #pragma unroll
                 for (int i = 0; i < P::kCount; ++i) h[i] = fma2(h[i], rho[P::spot(i)], shift[P::spot(i)]);
             }
             if constexpr (MODE == kFull) activate_all(a, p.act);
-            if constexpr (MODE == kSample) sample_gate<T, V, EPT>(p, at, t.sample, a);
+            if constexpr (MODE == kSample) sample_gate<T, V, EPT>(p, at, sample, a);
 #pragma unroll
             for (int i = 0; i < P::kCount; ++i) {
                 const float2 z = fma2(h[i], P::channels(&sh.vec[kPostW][at.c0], i), P::channels(&sh.vec[kPostB][at.c0], i));
                 r[i] = MODE == kPlain ? add2(r[i], z) : fma2(a[i], z, r[i]);
             }
-            F::store(p.r, t.base, stride, end, r);
+            F::store(p.r, base, stride, end, r);
         }
         if (!p.pre) continue;
         statistics<V, EPT, LC>(sh, p, r, at, rho, shift, p.stats ? p.stats + 2 * p.positions + q0 : nullptr, live_pos);
@@ -379,7 +395,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) field_forward_kernel(const 
         for (int i = 0; i < P::kCount; ++i)
             r[i] = fma2(fma2(r[i], rho[P::spot(i)], shift[P::spot(i)]), P::channels(&sh.vec[kPreW][at.c0], i),
                         P::channels(&sh.vec[kPreB][at.c0], i));
-        F::store(p.n, t.base, stride, end, r);
+        F::store(p.n, base, stride, end, r);
     }
     copy_wait<0>();
 }
@@ -392,11 +408,11 @@ struct Saved {
     float2 mean[kSpots], rho[kSpots], mean2[kSpots], rho2[kSpots];
 
     template <typename TILE>
-    __device__ __forceinline__ void load(const Problem& p, const TILE& t, int pos) {
+    __device__ __forceinline__ void load(const Problem& p, const TILE& t, const Where& at) {
 #pragma unroll
         for (int s = 0; s < kSpots; ++s) mean[s] = rho[s] = mean2[s] = rho2[s] = both(0.f);
-        if (!t.live) return;
-        const float* st = p.stats + static_cast<size_t>(t.sample) * p.length + t.l0 + pos * V;
+        if (!t.live(p, at)) return;
+        const float* st = p.stats + static_cast<size_t>(t.sample) * p.length + t.l0() + at.pos * V;
         const size_t row = static_cast<size_t>(p.positions);
 #pragma unroll
         for (int s = 0; s < kSpots; ++s) {
@@ -425,8 +441,10 @@ __device__ __forceinline__ float sum_positions(float v) {
 // Tensors a backward reads: x, y, dn, dr, and a gate per element.
 __host__ __device__ constexpr int backward_tensors(int mode) { return mode == kFull ? 5 : 4; }
 
-template <typename T, int V, int EPT, int LC, int MODE>
-__global__ void __launch_bounds__(kMaxWarps * 32) field_backward_kernel(const __grid_constant__ Problem p) {
+// MAXW: the most warps it is launched with.  Up to 10 the registers are held to what lets two blocks
+// share an SM (36 channels of 7 x 96 x 160 with a gate per sample: 30 us against 40 us).
+template <typename T, int V, int EPT, int LC, int MODE, int MAXW>
+__global__ void __launch_bounds__(MAXW * 32, MAXW <= 10 ? 2 : 1) field_backward_kernel(const __grid_constant__ Problem p) {
     using F = Slots<T, V, EPT>;
     using P = Pairs<V, EPT>;
     using TILE = Tile<V, EPT, LC>;
@@ -440,23 +458,24 @@ __global__ void __launch_bounds__(kMaxWarps * 32) field_backward_kernel(const __
     auto* slots = reinterpret_cast<typename F::E*>(dynamic + sizeof(sh)) + threadIdx.x;
     auto slot = [&](int turn, int tensor) { return slots + (turn * kTensors + tensor) * EPT * blockDim.x; };
     const int first = static_cast<int>(tile_begin(p, blockIdx.x)), last = static_cast<int>(tile_begin(p, blockIdx.x + 1));
-    auto fetch = [&](int tile, int turn) {
-        if (tile < last) {
-            const TILE t(p, at, tile);
-            const int end = t.live ? at.mine : 0;
-            if constexpr (MODE != kNoBlock) F::fetch(slot(turn, 1), p.y, t.base, stride, end);
+    Saved<V> ahead;
+    auto fetch = [&](const TILE& t, bool exists, int turn) {
+        if (exists) {
+            const size_t base = t.base(p, at);
+            const int end = t.live(p, at) ? at.mine : 0;
+            if constexpr (MODE != kNoBlock) F::fetch(slot(turn, 1), p.y, base, stride, end);
             if (p.dn) {
-                F::fetch(slot(turn, 0), p.x, t.base, stride, end);
-                F::fetch(slot(turn, 2), p.dn, t.base, stride, end);
+                F::fetch(slot(turn, 0), p.x, base, stride, end);
+                F::fetch(slot(turn, 2), p.dn, base, stride, end);
             }
-            if (p.dr) F::fetch(slot(turn, 3), p.dr, t.base, stride, end);
-            if constexpr (MODE == kFull) F::fetch(slot(turn, 4), p.gate, t.base, stride, end);
+            if (p.dr) F::fetch(slot(turn, 3), p.dr, base, stride, end);
+            if constexpr (MODE == kFull) F::fetch(slot(turn, 4), p.gate, base, stride, end);
+            ahead.load(p, t, at);
         }
         copy_commit();
     };
-    fetch(first, 0);
-    Saved<V> ahead;
-    if (first < last) ahead.load(p, TILE(p, at, first), at.pos);
+    TILE t(p, first, 1);
+    fetch(t, first < last, 0);
     load_vectors<T>(sh, p, at.warps * EPT * LC);
     int turn = 0;
     // sums over positions: per channel (V = 4: to be added over the pair), or per pair of channels
@@ -470,8 +489,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32) field_backward_kernel(const __
         return V == 1 ? (j % 2 ? sum[kind][j / 2].y : sum[kind][j / 2].x) : sum[kind][j % kAcc].x + sum[kind][j % kAcc].y;
     };
     for (int tile = first; tile < last; ++tile, turn ^= 1) {
-        const TILE t(p, at, tile);
-        const int end = t.live ? at.mine : 0;
+        const size_t base = t.base(p, at);
+        const int end = t.live(p, at) ? at.mine : 0, sample = t.sample;
+        const bool sample_ends = t.index + 1 == t.per_sample;
         float2 rho[kSpots], shift[kSpots], rho2[kSpots], shift2[kSpots];
 #pragma unroll
         for (int s = 0; s < kSpots; ++s) {
@@ -480,23 +500,23 @@ __global__ void __launch_bounds__(kMaxWarps * 32) field_backward_kernel(const __
             shift[s] = make_float2(-ahead.mean[s].x * rho[s].x, -ahead.mean[s].y * rho[s].y);
             shift2[s] = make_float2(-ahead.mean2[s].x * rho2[s].x, -ahead.mean2[s].y * rho2[s].y);
         }
-        fetch(tile + 1, turn ^ 1);
-        if (tile + 1 < last) ahead.load(p, TILE(p, at, tile + 1), at.pos);
+        t.next();
+        fetch(t, tile + 1 < last, turn ^ 1);
         copy_wait<1>();
         float2 h[N], a[N], slope[N], k[N], g[N];
         if constexpr (MODE != kNoBlock) {
-            F::read(slot(turn, 1), p.y, t.base, stride, end, h);
+            F::read(slot(turn, 1), p.y, base, stride, end, h);
 #pragma unroll
             for (int i = 0; i < N; ++i) h[i] = fma2(h[i], rho[P::spot(i)], shift[P::spot(i)]);
             if constexpr (MODE == kFull) {
-                F::read(slot(turn, 4), p.gate, t.base, stride, end, a);
+                F::read(slot(turn, 4), p.gate, base, stride, end, a);
                 activate_all(a, slope, p.act);
             }
-            if constexpr (MODE == kSample) sample_gate<T, V, EPT>(p, at, t.sample, a);
+            if constexpr (MODE == kSample) sample_gate<T, V, EPT>(p, at, sample, a);
         }
         if (p.dn) {
-            F::read(slot(turn, 0), p.x, t.base, stride, end, k);
-            F::read(slot(turn, 2), p.dn, t.base, stride, end, g);
+            F::read(slot(turn, 0), p.x, base, stride, end, k);
+            F::read(slot(turn, 2), p.dn, base, stride, end, g);
             float2 gk[N], m1[kSpots], m2[kSpots];
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -522,12 +542,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32) field_backward_kernel(const __
             for (int i = 0; i < N; ++i) g[i] = both(0.f);
         }
         if (p.dr) {
-            F::read(slot(turn, 3), p.dr, t.base, stride, end, k);
+            F::read(slot(turn, 3), p.dr, base, stride, end, k);
 #pragma unroll
             for (int i = 0; i < N; ++i) g[i] = add2(g[i], k[i]);
         }
         // g: the gradient of r
-        if (p.dx) F::store(p.dx, t.base, stride, end, g);
+        if (p.dx) F::store(p.dx, base, stride, end, g);
         if constexpr (MODE != kNoBlock) {
             float2 kh[N];
 #pragma unroll
@@ -544,7 +564,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32) field_backward_kernel(const __
                 for (int i = 0; i < N; ++i)
                     a[i] = mul2(mul2(g[i], slope[i]),
                                 fma2(h[i], P::channels(&sh.vec[kPostW][at.c0], i), P::channels(&sh.vec[kPostB][at.c0], i)));
-                F::store(p.dgate, t.base, stride, end, a);
+                F::store(p.dgate, base, stride, end, a);
             }
             if (p.dy) {
                 if (p.post) {
@@ -556,11 +576,10 @@ __global__ void __launch_bounds__(kMaxWarps * 32) field_backward_kernel(const __
                     for (int i = 0; i < N; ++i)
                         k[i] = mul2(rho[P::spot(i)], add2(fma2(h[i], m2[P::spot(i)], k[i]), m1[P::spot(i)]));
                 }
-                F::store(p.dy, t.base, stride, end, k);
+                F::store(p.dy, base, stride, end, k);
             }
-            if (MODE == kSample && p.slots &&
-                (tile + 1 == last || t.l0 + Shape<V, EPT, LC>::kPos >= static_cast<int>(p.length))) {
-                float* to = slot_of(p, blockIdx.x, t.sample);
+            if (MODE == kSample && p.slots && (tile + 1 == last || sample_ends)) {
+                float* to = slot_of(p, blockIdx.x, sample);
 #pragma unroll
                 for (int j = 0; j < EPT; ++j) {
 #pragma unroll
@@ -616,7 +635,7 @@ cudaError_t forward_as(Problem p, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-template <typename T, int V, int EPT, int LC, int MODE>
+template <typename T, int V, int EPT, int LC, int MODE, int MAXW = kMaxWarps>
 cudaError_t backward_as(Problem& p, cudaStream_t s) {
     using S = Shape<V, EPT, LC>;
     Problem q = p;
@@ -625,13 +644,13 @@ cudaError_t backward_as(Problem& p, cudaStream_t s) {
     const size_t smem = sizeof(Shared<V, EPT, LC>) +
                         (kCopied<Vec<T, V>> ? 2 * backward_tensors(MODE) * EPT * sizeof(Vec<T, V>) * threads : 0);
     int per_sm = 0;
-    const cudaError_t e = scx::prepare_kernel(reinterpret_cast<const void*>(field_backward_kernel<T, V, EPT, LC, MODE>),
+    const cudaError_t e = scx::prepare_kernel(reinterpret_cast<const void*>(field_backward_kernel<T, V, EPT, LC, MODE, MAXW>),
                                               smem, threads, &per_sm);
     if (e != cudaSuccess) return e;
     q.parts = static_cast<int>(std::min<long long>(std::min(max_parts(p.channels), per_sm * scx::num_sms()), q.tiles));
     q.partials = q.parts;
     p = q;
-    field_backward_kernel<T, V, EPT, LC, MODE><<<p.parts, threads, smem, s>>>(p);
+    field_backward_kernel<T, V, EPT, LC, MODE, MAXW><<<p.parts, threads, smem, s>>>(p);
     return cudaGetLastError();
 }
 
@@ -653,21 +672,23 @@ cudaError_t forward_in(const Problem& p, cudaStream_t s) {
         if (p.channels <= 512) return forward_as<T, 4, 2, 16, MODE>(p, s);
         return cudaErrorNotSupported;
     }
-    if (p.channels <= 64) return forward_as<T, 1, 4, 1, MODE>(p, s);
-    if (p.channels <= 256) return forward_as<T, 1, 4, 4, MODE>(p, s);
+    if (p.channels <= 128) return forward_as<T, 1, 8, 1, MODE>(p, s);
+    if (p.channels <= 512) return forward_as<T, 1, 8, 4, MODE>(p, s);
     return cudaErrorNotSupported;
 }
 
 template <typename T, int MODE>
 cudaError_t backward_in(Problem& p, cudaStream_t s) {
     if (vectors_fit<T, 4>(p)) {
+        if (p.channels <= 40) return backward_as<T, 4, 2, 2, MODE, 10>(p, s);
         if (p.channels <= 64) return backward_as<T, 4, 2, 2, MODE>(p, s);
         if (p.channels <= 128) return backward_as<T, 4, 2, 4, MODE>(p, s);
         if (p.channels <= 512) return backward_as<T, 4, 2, 16, MODE>(p, s);
         return cudaErrorNotSupported;
     }
-    if (p.channels <= 64) return backward_as<T, 1, 4, 1, MODE>(p, s);
-    if (p.channels <= 256) return backward_as<T, 1, 4, 4, MODE>(p, s);
+    if (p.channels <= 80) return backward_as<T, 1, 8, 1, MODE, 10>(p, s);
+    if (p.channels <= 128) return backward_as<T, 1, 8, 1, MODE>(p, s);
+    if (p.channels <= 512) return backward_as<T, 1, 8, 4, MODE>(p, s);
     return cudaErrorNotSupported;
 }
 

@@ -4,6 +4,10 @@
 // while this one's are in registers.  A thread keeps its channels from position to position, with
 // their weights, and in the backward their sums, in registers.  Statistics are sums over a
 // position's threads, by shuffles within a warp and through shared memory across warps.
+//
+// What a thread keeps bounds a block to 512 threads and 16 bytes of each tensor per thread.  Longer
+// positions (over 4096 channels of 2 bytes) are cut over a cluster of CL = 2 or 4 blocks, which
+// exchange their parts of each sum through distributed shared memory.
 #pragma once
 
 #include <algorithm>
@@ -16,22 +20,46 @@ namespace {
 
 constexpr int kMaxThreads = 512;
 constexpr int kAhead = 2;  // positions whose copies are under way while one is computed
-constexpr int kPartBytes = 2 * kMaxThreads / 32 * sizeof(float2);
+constexpr int kParts = kMaxThreads / 32 * 4;  // of the warps of a cluster
+constexpr int kPartBytes = 2 * kParts * sizeof(float2);
 
-// A block of blockDim threads takes blockDim / tpr positions, tpr threads (a power of two) each.
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Writes v to the same place of block `rank`'s shared memory as `at` has in this one's.
+__device__ __forceinline__ void store_in_block(float2* at, int rank, float2 v) {
+    unsigned to;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                 : "=r"(to)
+                 : "r"(static_cast<unsigned>(__cvta_generic_to_shared(at))), "r"(rank));
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(v.x), "f"(v.y) : "memory");
+}
+
+// A cluster of CL blocks takes blockDim / tpr positions (one, where CL > 1), tpr threads (a power of
+// two) of each block to a position.
+template <int VEC, int CL>
 struct Team {
-    int tpr, me, row, rows;
-    float2* part;  // [2][warps]
+    int tpr, me, row, rows, rank;
+    int first, end;  // this thread's first channel, and where the block's channels end
+    float2* part;    // [2][kParts]
 
-    __device__ __forceinline__ Team(int threads, float2* shared)
-        : tpr(threads), me(threadIdx.x % threads), row(threadIdx.x / threads), rows(blockDim.x / threads), part(shared) {}
+    __device__ __forceinline__ Team(int threads, int columns, int channels, float2* shared)
+        : tpr(threads), me(threadIdx.x % threads), row(threadIdx.x / threads), rows(blockDim.x / threads),
+          rank(blockIdx.x % CL), first(rank * columns + me * VEC), end(min(channels, (rank + 1) * columns)), part(shared) {
+        if (CL > 1) cluster_barrier();  // the others' shared memory is there
+    }
+
+    // The first channel of the thread's vector j, and whether it exists.
+    __device__ __forceinline__ int channel(int j) const { return first + j * tpr * VEC; }
+    __device__ __forceinline__ bool has(int j) const { return channel(j) < end; }
 
     // Sums over the position's threads, the same bits in all of them.  Across warps every warp adds
     // the warps' parts itself; `turn` alternates between calls, so that one barrier per call is
     // enough.
     template <int K>
     __device__ __forceinline__ void sum(float (&v)[K], int& turn) {
-        if (tpr < 32) {
+        if (CL == 1 && tpr < 32) {
             for (int o = tpr / 2; o > 0; o >>= 1) {
 #pragma unroll
                 for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
@@ -43,18 +71,30 @@ struct Team {
 #pragma unroll
             for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
         }
-        if (tpr == 32) return;
-        float2* now = part + turn * (kMaxThreads / 32);
+        if (CL == 1 && tpr == 32) return;
+        float2* now = part + turn * kParts;
         turn ^= 1;
-        if (threadIdx.x % 32 == 0) now[threadIdx.x / 32] = make_float2(v[0], v[K - 1]);
-        __syncthreads();
-        const int warps = tpr / 32;  // 2, 4, 8 or 16; the 16 lanes that hold more parts than there are hold zeros
-        const int lane = threadIdx.x % 16;
-        const float2 s = lane < warps ? now[row * warps + lane] : make_float2(0.f, 0.f);
+        const int warp = threadIdx.x / 32;
+        float2 s = make_float2(0.f, 0.f);
+        if (CL > 1) {
+            const int lane = threadIdx.x % 32;
+            // one lane per block of the cluster
+            if (lane < CL) store_in_block(now + rank * (kMaxThreads / 32) + warp, lane, make_float2(v[0], v[K - 1]));
+            __syncwarp();
+            cluster_barrier();
+#pragma unroll
+            for (int e = 0; e < CL * (kMaxThreads / 32); e += 32) s = add2(s, now[e + lane]);
+        } else {
+            if (threadIdx.x % 32 == 0) now[warp] = make_float2(v[0], v[K - 1]);
+            __syncthreads();
+            const int warps = tpr / 32;  // 2, 4, 8 or 16; the lanes past them hold zeros
+            const int lane = threadIdx.x % 16;
+            if (lane < warps) s = now[row * warps + lane];
+        }
         v[0] = s.x;
         v[K - 1] = s.y;
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) {
+        for (int o = CL > 1 ? 16 : 8; o > 0; o >>= 1) {
 #pragma unroll
             for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
         }
@@ -91,8 +131,8 @@ __device__ __forceinline__ float sum_of(const float2 (&v)[P]) {
 }
 
 // Mean and 1 / sqrt(variance + eps) of a position's values; vectors that do not exist hold zeros.
-template <int VEC, int NV>
-__device__ __forceinline__ float2 statistics(const Problem& p, Team& team, const float2 (&v)[NV * VEC / 2],
+template <int VEC, int NV, typename TEAM>
+__device__ __forceinline__ float2 statistics(const Problem& p, TEAM& team, const float2 (&v)[NV * VEC / 2],
                                              const bool (&on)[NV], int& turn) {
     constexpr int P = NV * VEC / 2;
     float mean = 0.f, s[1];
@@ -117,15 +157,12 @@ __device__ __forceinline__ float2 statistics(const Problem& p, Team& team, const
     return make_float2(mean, rsqrtf(fmaf(s[0], p.inv_c, p.eps)));
 }
 
-template <typename T, int VEC, int NV>
-__device__ __forceinline__ void weight_pairs(const void* w, const Problem& p, const Team& team, float other,
+template <typename T, int VEC, int NV, typename TEAM>
+__device__ __forceinline__ void weight_pairs(const void* w, const Problem& p, const TEAM& team, float other,
                                              float2 (&out)[NV * VEC / 2]) {
     float v[NV][VEC];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int c = (j * team.tpr + team.me) * VEC;
-        weights<T, VEC>(w, c, c < p.channels, p.wide, other, v[j]);
-    }
+    for (int j = 0; j < NV; ++j) weights<T, VEC>(w, team.channel(j), team.has(j), p.wide, other, v[j]);
 #pragma unroll
     for (int i = 0; i < NV * VEC / 2; ++i) out[i] = make_float2(v[2 * i / VEC][2 * i % VEC], v[(2 * i + 1) / VEC][(2 * i + 1) % VEC]);
 }
@@ -135,7 +172,8 @@ template <typename T, int VEC, int NV>
 struct Weights {
     float2 w[NV * VEC / 2], b[NV * VEC / 2], w2[NV * VEC / 2];
 
-    __device__ __forceinline__ Weights(const Problem& p, const Team& team, bool block) {
+    template <typename TEAM>
+    __device__ __forceinline__ Weights(const Problem& p, const TEAM& team, bool block) {
         if (block) {
             float2 scale[NV * VEC / 2];
             weight_pairs<T, VEC, NV>(p.scale_w, p, team, 1.f, scale);
@@ -157,47 +195,42 @@ template <typename T, int VEC, int NV>
 struct Slots {
     using E = Vec<T, VEC>;
 
-    static __device__ __forceinline__ void fetch(E* slot, const void* from, size_t row, const Team& team, int channels,
-                                                 bool here) {
+    template <typename TEAM>
+    static __device__ __forceinline__ void fetch(E* slot, const void* from, size_t row, const TEAM& team, bool here) {
         if constexpr (kCopied<E>) {
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-                const int c = (j * team.tpr + team.me) * VEC;
-                const bool live = here && c < channels;
-                copy_async(slot + j * blockDim.x, static_cast<const T*>(from) + (live ? row + c : 0), live);
+                const bool live = here && team.has(j);
+                copy_async(slot + j * blockDim.x, static_cast<const T*>(from) + (live ? row + team.channel(j) : 0), live);
             }
         }
     }
 
-    static __device__ __forceinline__ void read(const E* slot, const void* from, size_t row, const Team& team,
-                                                int channels, bool here, float2 (&out)[NV * VEC / 2]) {
+    template <typename TEAM>
+    static __device__ __forceinline__ void read(const E* slot, const void* from, size_t row, const TEAM& team, bool here,
+                                                float2 (&out)[NV * VEC / 2]) {
         E v[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             v[j] = E{};
-            if constexpr (kCopied<E>) {
-                v[j] = slot[j * blockDim.x];
-            } else {
-                const int c = (j * team.tpr + team.me) * VEC;
-                if (here && c < channels) v[j] = load_vec<T, VEC>(from, row + c);
-            }
+            if constexpr (kCopied<E>) v[j] = slot[j * blockDim.x];
+            else if (here && team.has(j)) v[j] = load_vec<T, VEC>(from, row + team.channel(j));
         }
 #pragma unroll
         for (int i = 0; i < NV * VEC / 2; ++i)
             out[i] = unpack(v[2 * i / VEC].v[2 * i % VEC], v[(2 * i + 1) / VEC].v[(2 * i + 1) % VEC]);
     }
 
-    static __device__ __forceinline__ void store(void* to, size_t row, const Team& team, int channels, bool here,
+    template <typename TEAM>
+    static __device__ __forceinline__ void store(void* to, size_t row, const TEAM& team, bool here,
                                                  const float2 (&v)[NV * VEC / 2]) {
         E o[NV];
 #pragma unroll
         for (int i = 0; i < NV * VEC / 2; ++i)
             pack(o[2 * i / VEC].v[2 * i % VEC], o[(2 * i + 1) / VEC].v[(2 * i + 1) % VEC], v[i]);
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int c = (j * team.tpr + team.me) * VEC;
-            if (here && c < channels) store_vec<T, VEC>(to, row + c, o[j]);
-        }
+        for (int j = 0; j < NV; ++j)
+            if (here && team.has(j)) store_vec<T, VEC>(to, row + team.channel(j), o[j]);
     }
 };
 
@@ -216,14 +249,16 @@ __host__ __device__ constexpr int backward_tensors(int mode) { return mode == kN
 
 // A gate per sample is read like one per element, from the sample's row: kSample and kFull are one
 // mode here.
-template <typename T, int VEC, int NV, int MODE>
-__global__ void __launch_bounds__(kMaxThreads) token_forward_kernel(const __grid_constant__ Problem p, int tpr) {
+template <typename T, int VEC, int NV, int CL, int MODE>
+__global__ void __launch_bounds__(kMaxThreads) token_forward_kernel(const __grid_constant__ Problem p, int tpr,
+                                                                    int columns) {
     using F = Slots<T, VEC, NV>;
     constexpr int N = NV * VEC / 2, kTensors = forward_tensors(MODE);
     extern __shared__ __align__(16) unsigned char dynamic[];
     auto* part = reinterpret_cast<float2*>(dynamic);
-    Team team(tpr, part);
+    Team<VEC, CL> team(tpr, columns, p.channels, part);
     const int channels = p.channels;
+    const long long block = blockIdx.x / CL, blocks = gridDim.x / CL;  // clusters
     const long long groups = (p.positions + team.rows - 1) / team.rows;
     auto* slots = reinterpret_cast<typename F::E*>(dynamic + kPartBytes) + threadIdx.x;
     auto slot = [&](int ring, int tensor) { return slots + (ring * kTensors + tensor) * NV * blockDim.x; };
@@ -235,33 +270,32 @@ __global__ void __launch_bounds__(kMaxThreads) token_forward_kernel(const __grid
             const long long q = group * team.rows + team.row;
             const bool here = q < p.positions;
             const size_t row = static_cast<size_t>(q) * channels;
-            F::fetch(slot(ring, 0), p.x, row, team, channels, here);
-            if constexpr (MODE != kNoBlock) F::fetch(slot(ring, 1), p.y, row, team, channels, here);
-            if constexpr (MODE == kFull) F::fetch(slot(ring, 2), p.gate, here ? gate_row(q) : 0, team, channels, here);
+            F::fetch(slot(ring, 0), p.x, row, team, here);
+            if constexpr (MODE != kNoBlock) F::fetch(slot(ring, 1), p.y, row, team, here);
+            if constexpr (MODE == kFull) F::fetch(slot(ring, 2), p.gate, here ? gate_row(q) : 0, team, here);
         }
         copy_commit();
     };
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) fetch(blockIdx.x + static_cast<long long>(k) * gridDim.x, k);
+    for (int k = 0; k < kAhead; ++k) fetch(block + k * blocks, k);
     const Weights<T, VEC, NV> weight_of(p, team, MODE != kNoBlock);
     bool on[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) on[j] = (j * tpr + team.me) * VEC < channels;
+    for (int j = 0; j < NV; ++j) on[j] = team.has(j);
     int turn = 0, ring = 0;
-    for (long long group = blockIdx.x; group < groups; group += gridDim.x) {
+    for (long long group = block; group < groups; group += blocks) {
         const long long q = group * team.rows + team.row;
         const bool here = q < p.positions;
         const size_t row = static_cast<size_t>(q) * channels;
-        const int next = ring + kAhead >= kAhead + 1 ? ring - 1 : ring + kAhead;
-        fetch(group + static_cast<long long>(kAhead) * gridDim.x, next);
+        fetch(group + kAhead * blocks, ring == 0 ? kAhead : ring - 1);
         copy_wait<kAhead>();
         float2 r[N], st = make_float2(0.f, 1.f), st2 = st;
-        F::read(slot(ring, 0), p.x, row, team, channels, here, r);
+        F::read(slot(ring, 0), p.x, row, team, here, r);
         if constexpr (MODE != kNoBlock) {
             float2 h[N], a[N];
-            F::read(slot(ring, 1), p.y, row, team, channels, here, h);
+            F::read(slot(ring, 1), p.y, row, team, here, h);
             if constexpr (MODE == kFull) {
-                F::read(slot(ring, 2), p.gate, here ? gate_row(q) : 0, team, channels, here, a);
+                F::read(slot(ring, 2), p.gate, here ? gate_row(q) : 0, team, here, a);
                 activate_all(a, p.act);
             }
             if (p.post) st = statistics<VEC, NV>(p, team, h, on, turn);
@@ -271,7 +305,7 @@ __global__ void __launch_bounds__(kMaxThreads) token_forward_kernel(const __grid
                 const float2 z = fma2(fma2(h[i], rho, shift), weight_of.w[i], weight_of.b[i]);
                 r[i] = MODE == kPlain ? add2(r[i], z) : fma2(a[i], z, r[i]);
             }
-            F::store(p.r, row, team, channels, here, r);
+            F::store(p.r, row, team, here, r);
             clear_dead<VEC, NV>(r, on);
         }
         if (p.pre) {
@@ -281,9 +315,9 @@ __global__ void __launch_bounds__(kMaxThreads) token_forward_kernel(const __grid
             weight_pairs<T, VEC, NV>(p.pre_b, p, team, 0.f, b);
 #pragma unroll
             for (int i = 0; i < N; ++i) r[i] = fma2(fma2(r[i], rho, shift), weight_of.w2[i], b[i]);
-            F::store(p.n, row, team, channels, here, r);
+            F::store(p.n, row, team, here, r);
         }
-        if (p.stats && team.me == 0 && here) {
+        if (p.stats && team.rank == 0 && team.me == 0 && here) {
             p.stats[q] = st.x;
             p.stats[p.positions + q] = st.y;
             p.stats[2 * p.positions + q] = st2.x;
@@ -296,8 +330,8 @@ __global__ void __launch_bounds__(kMaxThreads) token_forward_kernel(const __grid
 
 // Sums over a block's positions: the rows' threads of one channel are added through shared memory in
 // row order.  Every thread of the block calls it.
-template <int VEC, int NV>
-__device__ void store_sums(const Problem& p, const Team& team, float* shared, const float2 (&sum)[NV * VEC / 2], float* out) {
+template <int VEC, int NV, typename TEAM>
+__device__ void store_sums(const Problem& p, const TEAM& team, float* shared, const float2 (&sum)[NV * VEC / 2], float* out) {
     float v[NV * VEC];
 #pragma unroll
     for (int i = 0; i < NV * VEC / 2; ++i) {
@@ -322,8 +356,8 @@ __device__ void store_sums(const Problem& p, const Team& team, float* shared, co
     constexpr int kPer = VEC < 4 ? VEC : 4;  // VEC >= 4 divides the channels, so `out` starts on 16 bytes
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int c = (j * team.tpr + team.me) * VEC;
-        if (c >= p.channels) continue;
+        const int c = team.channel(j);
+        if (!team.has(j)) continue;
 #pragma unroll
         for (int i = 0; i < VEC; i += kPer) {
             Vec<float, kPer> o;
@@ -334,8 +368,9 @@ __device__ void store_sums(const Problem& p, const Team& team, float* shared, co
     }
 }
 
-template <typename T, int VEC, int NV, int MODE>
-__global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __grid_constant__ Problem p, int tpr) {
+template <typename T, int VEC, int NV, int CL, int MODE>
+__global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __grid_constant__ Problem p, int tpr,
+                                                                     int columns) {
     using F = Slots<T, VEC, NV>;
     constexpr int N = NV * VEC / 2, kTensors = backward_tensors(MODE);
     // the tensors' places in a ring slot
@@ -343,11 +378,12 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
     extern __shared__ __align__(16) unsigned char dynamic[];
     auto* part = reinterpret_cast<float2*>(dynamic);
     grid_dep_launch();
-    Team team(tpr, part);
+    Team<VEC, CL> team(tpr, columns, p.channels, part);
     const int channels = p.channels;
+    const long long block = blockIdx.x / CL;  // the cluster
     auto* slots = reinterpret_cast<typename F::E*>(dynamic + kPartBytes) + threadIdx.x;
     auto slot = [&](int ring, int tensor) { return slots + (ring * kTensors + tensor) * NV * blockDim.x; };
-    const long long first = tile_begin(p, blockIdx.x), last = tile_begin(p, blockIdx.x + 1);
+    const long long first = tile_begin(p, block), last = tile_begin(p, block + 1);
     const bool samples = p.tiles_per_sample != p.tiles;  // otherwise no division
     struct At {
         long long sample, q;
@@ -363,15 +399,14 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
             const At at = at_of(tile);
             const size_t row = static_cast<size_t>(at.q) * channels;
             if (p.dn) {
-                F::fetch(slot(ring, kX), p.x, row, team, channels, at.here);
-                F::fetch(slot(ring, kDn), p.dn, row, team, channels, at.here);
+                F::fetch(slot(ring, kX), p.x, row, team, at.here);
+                F::fetch(slot(ring, kDn), p.dn, row, team, at.here);
             }
-            if (p.dr) F::fetch(slot(ring, kDr), p.dr, row, team, channels, at.here);
-            if constexpr (MODE != kNoBlock) F::fetch(slot(ring, kY), p.y, row, team, channels, at.here);
+            if (p.dr) F::fetch(slot(ring, kDr), p.dr, row, team, at.here);
+            if constexpr (MODE != kNoBlock) F::fetch(slot(ring, kY), p.y, row, team, at.here);
             if constexpr (MODE == kFull)
                 F::fetch(slot(ring, kGate), p.gate,
-                         p.gate_mode == kGateSample ? static_cast<size_t>(at.sample) * channels : row, team, channels,
-                         at.here);
+                         p.gate_mode == kGateSample ? static_cast<size_t>(at.sample) * channels : row, team, at.here);
         }
         copy_commit();
     };
@@ -383,7 +418,7 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
     for (int i = 0; i < N; ++i) dw2[i] = db2[i] = tah[i] = ta[i] = both(0.f);
     bool on[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) on[j] = (j * tpr + team.me) * VEC < channels;
+    for (int j = 0; j < NV; ++j) on[j] = team.has(j);
     int turn = 0, ring = 0;
     for (long long tile = first; tile < last; ++tile) {
         const At at = at_of(tile);
@@ -410,23 +445,23 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
 #pragma unroll
             for (int i = 0; i < N; ++i) a[i] = s[i];
             if (p.act == kActSilu) {
-                F::read(slot(ring, kGate), p.gate, gate_row, team, channels, at.here, a);
+                F::read(slot(ring, kGate), p.gate, gate_row, team, at.here, a);
 #pragma unroll
                 for (int i = 0; i < N; ++i) a[i] = mul2(a[i], s[i]);
             }
         };
         if constexpr (MODE != kNoBlock) {
-            F::read(slot(ring, kY), p.y, row, team, channels, at.here, h);
+            F::read(slot(ring, kY), p.y, row, team, at.here, h);
 #pragma unroll
             for (int i = 0; i < N; ++i) h[i] = fma2(h[i], rho, shift);
             if constexpr (MODE == kFull) {
-                F::read(slot(ring, kGate), p.gate, gate_row, team, channels, at.here, s);
+                F::read(slot(ring, kGate), p.gate, gate_row, team, at.here, s);
                 if (p.act != kActNone) activate_all(s, kActSigmoid);
             }
         }
         if (p.dn) {
-            F::read(slot(ring, kX), p.x, row, team, channels, at.here, k);
-            F::read(slot(ring, kDn), p.dn, row, team, channels, at.here, g);  // zeros where there is no channel
+            F::read(slot(ring, kX), p.x, row, team, at.here, k);
+            F::read(slot(ring, kDn), p.dn, row, team, at.here, g);  // zeros where there is no channel
             float2 a[N];
             if constexpr (MODE == kFull) gate_of(a);
             float2 s0 = both(0.f), s1 = both(0.f);
@@ -453,13 +488,13 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
             for (int i = 0; i < N; ++i) g[i] = both(0.f);
         }
         if (p.dr) {
-            F::read(slot(ring, kDr), p.dr, row, team, channels, at.here, k);
+            F::read(slot(ring, kDr), p.dr, row, team, at.here, k);
 #pragma unroll
             for (int i = 0; i < N; ++i) g[i] = add2(g[i], k[i]);
         }
         clear_dead<VEC, NV>(g, on);
         // g: the gradient of r
-        if (p.dx) F::store(p.dx, row, team, channels, at.here, g);
+        if (p.dx) F::store(p.dx, row, team, at.here, g);
         if constexpr (MODE != kNoBlock) {
             float2 s0 = both(0.f), s1 = both(0.f), a[N];
             if constexpr (MODE == kFull) {
@@ -473,7 +508,7 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
                                                  : p.act == kActSigmoid ? mul2(s[i], rest) : both(1.f);
                         o[i] = mul2(mul2(g[i], fma2(h[i], weight_of.w[i], weight_of.b[i])), o[i]);
                     }
-                    F::store(p.dgate, row, team, channels, at.here, o);
+                    F::store(p.dgate, row, team, at.here, o);
                 }
             }
 #pragma unroll
@@ -494,13 +529,13 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
 #pragma unroll
                     for (int i = 0; i < N; ++i) k[i] = mul2(rho, add2(fma2(h[i], m4, k[i]), m3));
                 }
-                F::store(p.dy, row, team, channels, at.here, k);
+                F::store(p.dy, row, team, at.here, k);
             }
             if (p.slots && (tile + 1 == last || (tile + 1) % p.tiles_per_sample == 0)) {
                 // this ring slot has been read, and its next copies are kAhead positions away: the sums
                 // of several rows meet in the space behind the ring
                 float* meet = reinterpret_cast<float*>(slots - threadIdx.x + (kAhead + 1) * kTensors * NV * blockDim.x);
-                float* to = slot_of(p, blockIdx.x, at.sample);
+                float* to = slot_of(p, block, at.sample);
                 store_sums<VEC, NV>(p, team, meet, tah, to);
                 store_sums<VEC, NV>(p, team, meet, ta, to + channels);
 #pragma unroll
@@ -512,51 +547,72 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
     copy_wait<0>();
     if (!p.sums) return;
     float* meet = reinterpret_cast<float*>(slots - threadIdx.x + (kAhead + 1) * kTensors * NV * blockDim.x);
-    float* out = p.partial + static_cast<size_t>(blockIdx.x) * kSums * channels;
+    float* out = p.partial + static_cast<size_t>(block) * kSums * channels;
     store_sums<VEC, NV>(p, team, meet, dw2, out + static_cast<size_t>(kDPreW) * channels);
     store_sums<VEC, NV>(p, team, meet, db2, out + static_cast<size_t>(kDPreB) * channels);
     store_sums<VEC, NV>(p, team, meet, tah, out + static_cast<size_t>(kTah) * channels);
     store_sums<VEC, NV>(p, team, meet, ta, out + static_cast<size_t>(kTa) * channels);
 }
 
-// Threads per position: a power of two that covers the channels.
-int team_for(int channels, int per_thread) {
-    int tpr = 4;
-    while (tpr * per_thread < channels) tpr *= 2;
-    return tpr;
+// How a call's positions are laid over threads: tpr threads of each block of a cluster, `columns`
+// channels of a block.
+struct Lay {
+    int tpr, columns, threads, rows;
+    Lay(int channels, int vec, int nv, int cluster) {
+        columns = ((channels + vec - 1) / vec + cluster - 1) / cluster * vec;
+        tpr = 4;
+        while (tpr * vec * nv < columns) tpr *= 2;
+        threads = std::max(cluster > 1 ? kMaxThreads : 128, tpr);
+        if (cluster > 1) tpr = kMaxThreads;
+        rows = threads / tpr;
+    }
+};
+
+template <int CL>
+cudaError_t launch(const void* kernel, int clusters, int threads, size_t smem, cudaStream_t s, const Problem& p, Lay lay) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(clusters * CL);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {CL, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = CL > 1 ? 1 : 0;
+    Problem q = p;
+    void* args[] = {&q, &lay.tpr, &lay.columns};
+    return cudaLaunchKernelExC(&cfg, kernel, args);
 }
 
-template <typename T, int VEC, int NV, int MODE>
+template <typename T, int VEC, int NV, int CL, int MODE>
 cudaError_t forward_as(const Problem& p, cudaStream_t s) {
-    const int tpr = team_for(p.channels, VEC * NV);
-    const int threads = std::max(128, tpr), rows = threads / tpr;
-    const long long groups = (p.positions + rows - 1) / rows;
-    const size_t smem = kPartBytes + (kAhead + 1) * forward_tensors(MODE) * NV * sizeof(Vec<T, VEC>) * threads;
+    const Lay lay(p.channels, VEC, NV, CL);
+    const long long groups = (p.positions + lay.rows - 1) / lay.rows;
+    const size_t smem = kPartBytes + (kAhead + 1) * forward_tensors(MODE) * NV * sizeof(Vec<T, VEC>) * lay.threads;
+    const void* kernel = reinterpret_cast<const void*>(token_forward_kernel<T, VEC, NV, CL, MODE>);
     int per_sm = 0;
-    const cudaError_t e =
-        scx::prepare_kernel(reinterpret_cast<const void*>(token_forward_kernel<T, VEC, NV, MODE>), smem, threads, &per_sm);
+    const cudaError_t e = scx::prepare_kernel(kernel, smem, lay.threads, &per_sm);
     if (e != cudaSuccess) return e;
-    const int grid = static_cast<int>(std::min<long long>(groups, static_cast<long long>(per_sm) * scx::num_sms()));
-    token_forward_kernel<T, VEC, NV, MODE><<<grid, threads, smem, s>>>(p, tpr);
-    return cudaGetLastError();
+    const int clusters = static_cast<int>(std::min<long long>(groups, std::max(1, per_sm * scx::num_sms() / CL)));
+    return launch<CL>(kernel, clusters, lay.threads, smem, s, p, lay);
 }
 
-template <typename T, int VEC, int NV, int MODE>
+template <typename T, int VEC, int NV, int CL, int MODE>
 cudaError_t backward_as(Problem& p, cudaStream_t s) {
-    const int tpr = team_for(p.channels, VEC * NV);
-    const int threads = std::max(128, tpr), rows = threads / tpr;
-    const size_t smem = kPartBytes + (kAhead + 1) * backward_tensors(MODE) * NV * sizeof(Vec<T, VEC>) * threads +
-                        (rows > 1 ? sizeof(float) * threads * VEC * NV : 0);
+    const Lay lay(p.channels, VEC, NV, CL);
+    const size_t smem = kPartBytes + (kAhead + 1) * backward_tensors(MODE) * NV * sizeof(Vec<T, VEC>) * lay.threads +
+                        (lay.rows > 1 ? sizeof(float) * lay.threads * VEC * NV : 0);
+    const void* kernel = reinterpret_cast<const void*>(token_backward_kernel<T, VEC, NV, CL, MODE>);
     int per_sm = 0;
-    const cudaError_t e =
-        scx::prepare_kernel(reinterpret_cast<const void*>(token_backward_kernel<T, VEC, NV, MODE>), smem, threads, &per_sm);
+    const cudaError_t e = scx::prepare_kernel(kernel, smem, lay.threads, &per_sm);
     if (e != cudaSuccess) return e;
-    p.tiles_per_sample = (p.length + rows - 1) / rows;
+    p.tiles_per_sample = (p.length + lay.rows - 1) / lay.rows;
     p.tiles = p.batch * p.tiles_per_sample;
-    p.parts = static_cast<int>(std::min<long long>(std::min(max_parts(p.channels), per_sm * scx::num_sms()), p.tiles));
+    p.parts = static_cast<int>(std::min<long long>(
+        std::min(max_parts(p.channels), std::max(1, per_sm * scx::num_sms() / CL)), p.tiles));
     p.partials = p.parts;
-    token_backward_kernel<T, VEC, NV, MODE><<<p.parts, threads, smem, s>>>(p, tpr);
-    return cudaGetLastError();
+    return launch<CL>(kernel, p.parts, lay.threads, smem, s, p, lay);
 }
 
 // Whether rows can be moved by 16-byte accesses: whole vectors per row, every base aligned.
@@ -573,11 +629,13 @@ template <typename T, int MODE>
 cudaError_t forward_in(const Problem& p, cudaStream_t s) {
     constexpr int VEC = 16 / static_cast<int>(sizeof(T));
     if (vectors_fit<T>(p)) {
-        if (p.channels <= VEC * kMaxThreads) return forward_as<T, VEC, 1, MODE>(p, s);
-        if (p.channels <= 2 * VEC * kMaxThreads) return forward_as<T, VEC, 2, MODE>(p, s);
+        if (p.channels <= VEC * kMaxThreads) return forward_as<T, VEC, 1, 1, MODE>(p, s);
+        if (p.channels <= 2 * VEC * kMaxThreads) return forward_as<T, VEC, 1, 2, MODE>(p, s);
+        if (p.channels <= 4 * VEC * kMaxThreads) return forward_as<T, VEC, 1, 4, MODE>(p, s);
         return cudaErrorNotSupported;
     }
-    if (p.channels <= 4 * kMaxThreads) return forward_as<T, 1, 4, MODE>(p, s);
+    if (p.channels <= 4 * kMaxThreads) return forward_as<T, 1, 4, 1, MODE>(p, s);
+    if (p.channels <= 16 * kMaxThreads) return forward_as<T, 1, 4, 4, MODE>(p, s);
     return cudaErrorNotSupported;
 }
 
@@ -585,10 +643,13 @@ template <typename T, int MODE>
 cudaError_t backward_in(Problem& p, cudaStream_t s) {
     constexpr int VEC = 16 / static_cast<int>(sizeof(T));
     if (vectors_fit<T>(p)) {
-        if (p.channels <= VEC * kMaxThreads) return backward_as<T, VEC, 1, MODE>(p, s);
+        if (p.channels <= VEC * kMaxThreads) return backward_as<T, VEC, 1, 1, MODE>(p, s);
+        if (p.channels <= 2 * VEC * kMaxThreads) return backward_as<T, VEC, 1, 2, MODE>(p, s);
+        if (p.channels <= 4 * VEC * kMaxThreads) return backward_as<T, VEC, 1, 4, MODE>(p, s);
         return cudaErrorNotSupported;
     }
-    if (p.channels <= 4 * kMaxThreads) return backward_as<T, 1, 4, MODE>(p, s);
+    if (p.channels <= 4 * kMaxThreads) return backward_as<T, 1, 4, 1, MODE>(p, s);
+    if (p.channels <= 16 * kMaxThreads) return backward_as<T, 1, 4, 4, MODE>(p, s);
     return cudaErrorNotSupported;
 }
 
