@@ -244,23 +244,21 @@ __device__ __forceinline__ void two_means(Shared<V, EPT, LC>& sh, const Problem&
     });
 }
 
-// Where a tile lies, for one thread; moved on by a fixed number of tiles without a division.
+// Where a tile lies, for one thread; moved on by `step` tiles without a division.
 template <int V, int EPT, int LC>
 struct Tile {
     int sample, index;  // the tile's index in its sample
-    int step_samples, step_index, per_sample;
 
-    __device__ __forceinline__ Tile(const Problem& p, int tile, int step) : per_sample(static_cast<int>(p.tiles_per_sample)) {
+    __device__ __forceinline__ Tile(const Problem& p, int tile) {
+        const int per_sample = static_cast<int>(p.tiles_per_sample);
         sample = tile / per_sample;
         index = tile - sample * per_sample;
-        step_samples = step / per_sample;
-        step_index = step - step_samples * per_sample;
     }
-    __device__ __forceinline__ void next() {
+    __device__ __forceinline__ void next(const Problem& p, int step_samples, int step_index) {
         sample += step_samples;
         index += step_index;
-        if (index >= per_sample) {
-            index -= per_sample;
+        if (index >= static_cast<int>(p.tiles_per_sample)) {
+            index -= static_cast<int>(p.tiles_per_sample);
             ++sample;
         }
     }
@@ -357,7 +355,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) field_forward_kernel(const 
         }
         copy_commit();
     };
-    TILE t(p, blockIdx.x, gridDim.x);
+    TILE t(p, blockIdx.x);
+    const TILE step(p, gridDim.x);  // as a number of samples and of tiles
     fetch(t, static_cast<int>(blockIdx.x) < tiles, 0);
     load_vectors<T>(sh, p, at.warps * EPT * LC);
     int turn = 0;
@@ -366,7 +365,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) field_forward_kernel(const 
         const int end = t.live(p, at) ? at.mine : 0, sample = t.sample;
         const size_t q0 = static_cast<size_t>(sample) * p.length + t.l0();
         const int live_pos = static_cast<int>(p.length) - t.l0();
-        t.next();
+        t.next(p, step.sample, step.index);
         fetch(t, tile + static_cast<int>(gridDim.x) < tiles, turn ^ 1);
         copy_wait<1>();
         float2 r[P::kCount], rho[P::kSpots], shift[P::kSpots];
@@ -474,7 +473,7 @@ __global__ void __launch_bounds__(MAXW * 32, MAXW <= 10 ? 2 : 1) field_backward_
         }
         copy_commit();
     };
-    TILE t(p, first, 1);
+    TILE t(p, first);
     fetch(t, first < last, 0);
     load_vectors<T>(sh, p, at.warps * EPT * LC);
     int turn = 0;
@@ -491,7 +490,7 @@ __global__ void __launch_bounds__(MAXW * 32, MAXW <= 10 ? 2 : 1) field_backward_
     for (int tile = first; tile < last; ++tile, turn ^= 1) {
         const size_t base = t.base(p, at);
         const int end = t.live(p, at) ? at.mine : 0, sample = t.sample;
-        const bool sample_ends = t.index + 1 == t.per_sample;
+        const bool sample_ends = t.index + 1 == static_cast<int>(p.tiles_per_sample);
         float2 rho[kSpots], shift[kSpots], rho2[kSpots], shift2[kSpots];
 #pragma unroll
         for (int s = 0; s < kSpots; ++s) {
@@ -500,7 +499,7 @@ __global__ void __launch_bounds__(MAXW * 32, MAXW <= 10 ? 2 : 1) field_backward_
             shift[s] = make_float2(-ahead.mean[s].x * rho[s].x, -ahead.mean[s].y * rho[s].y);
             shift2[s] = make_float2(-ahead.mean2[s].x * rho2[s].x, -ahead.mean2[s].y * rho2[s].y);
         }
-        t.next();
+        t.next(p, 0, 1);
         fetch(t, tile + 1 < last, turn ^ 1);
         copy_wait<1>();
         float2 h[N], a[N], slope[N], k[N], g[N];
@@ -673,6 +672,7 @@ cudaError_t forward_in(const Problem& p, cudaStream_t s) {
         return cudaErrorNotSupported;
     }
     if (p.channels <= 128) return forward_as<T, 1, 8, 1, MODE>(p, s);
+    if (p.channels <= 256) return forward_as<T, 1, 8, 2, MODE>(p, s);
     if (p.channels <= 512) return forward_as<T, 1, 8, 4, MODE>(p, s);
     return cudaErrorNotSupported;
 }
@@ -680,14 +680,16 @@ cudaError_t forward_in(const Problem& p, cudaStream_t s) {
 template <typename T, int MODE>
 cudaError_t backward_in(Problem& p, cudaStream_t s) {
     if (vectors_fit<T, 4>(p)) {
+        if (p.channels <= 32) return backward_as<T, 4, 2, 2, MODE, 8>(p, s);
         if (p.channels <= 40) return backward_as<T, 4, 2, 2, MODE, 10>(p, s);
         if (p.channels <= 64) return backward_as<T, 4, 2, 2, MODE>(p, s);
         if (p.channels <= 128) return backward_as<T, 4, 2, 4, MODE>(p, s);
         if (p.channels <= 512) return backward_as<T, 4, 2, 16, MODE>(p, s);
         return cudaErrorNotSupported;
     }
-    if (p.channels <= 80) return backward_as<T, 1, 8, 1, MODE, 10>(p, s);
+    if (p.channels <= 64) return backward_as<T, 1, 8, 1, MODE, 8>(p, s);
     if (p.channels <= 128) return backward_as<T, 1, 8, 1, MODE>(p, s);
+    if (p.channels <= 256) return backward_as<T, 1, 8, 2, MODE>(p, s);
     if (p.channels <= 512) return backward_as<T, 1, 8, 4, MODE>(p, s);
     return cudaErrorNotSupported;
 }
