@@ -14,6 +14,8 @@ the reference and reference state dicts load unchanged.  Differences:
 * ``FNO2d.forward_autograd`` is the differentiable device forward that training uses
   (fno_train.py): spectral convolutions through the library's forward and backward kernels.
 * ``instance_norm=False`` builds the norm-free layer (SpectralConv + 1x1 skip + GELU).
+* ``ResidualFNO2d`` (no counterpart there) is the same stack with a residual stream: gated blocks
+  between norms, for stacks deeper than the reference's four layers.
 """
 
 from __future__ import annotations
@@ -26,6 +28,7 @@ import torch.nn.functional as F
 
 import _scx
 import spectral_conv_ext
+from residual_norm_ops import residual_norm
 from spectral_conv_ops import spectral_conv2d_autograd, spectral_conv2d_supa
 
 
@@ -260,6 +263,114 @@ class FNO2d(nn.Module):
         device = x.device if x.is_cuda else torch.device("cuda", torch.cuda.current_device())
         x = x.to(device=device, dtype=torch.float32)
         return self.forward_device(x).cpu()
+
+
+def _residual_norm_host(h, y=None, *, pre_weight, post_weight=None, gate=None, scale=None, kind="rms",
+                        eps=1e-5):
+    """``residual_norm`` of fields in torch operations, for the host path."""
+    def norm(v, weight):
+        if kind == "layer":
+            v = v - v.mean(1, keepdim=True)
+        return v * torch.rsqrt(v.square().mean(1, keepdim=True) + eps) * weight[:, None, None]
+
+    if y is not None:
+        z = norm(y, post_weight) * scale[:, None, None]
+        if gate is not None:
+            z = z * torch.sigmoid(gate if gate.dim() == 4 else gate[:, :, None, None])
+        h = h + z
+    return h, norm(h, pre_weight)
+
+
+class ResidualFourierLayer(nn.Module):
+    """One block of ResidualFNO2d: y = GELU(SpectralConv(n) + 1x1 n) of the normed input n, and the
+    weights of what joins y to the residual stream: the norm after the block, the residual scale,
+    the gate and the norm before the next block."""
+
+    def __init__(self, width: int, modes1: int, modes2: int, gate: str, scale: float):
+        super().__init__()
+        self.spectral_conv = SpectralConv2d(width, width, modes1, modes2)
+        self.conv = nn.Conv2d(width, width, 1)
+        self.post_weight = nn.Parameter(torch.ones(width))
+        self.scale = nn.Parameter(torch.full((width,), scale))
+        self.next_weight = nn.Parameter(torch.ones(width))
+        self.gate = {"none": lambda: None, "element": lambda: nn.Conv2d(width, width, 1),
+                     "sample": lambda: nn.Linear(width, width)}[gate]()
+
+    def gate_of(self, n: torch.Tensor) -> torch.Tensor | None:
+        """Before its sigmoid: None, [B, C, H, W], or [B, C] from the mean over the positions."""
+        if isinstance(self.gate, nn.Conv2d):
+            return _conv1x1(self.gate, n)
+        return self.gate(n.mean((2, 3))) if self.gate is not None else None
+
+
+class ResidualFNO2d(nn.Module):
+    """FNO2d with a residual stream h and norms before and after each block:
+
+        h, n = residual_norm(lift(x));  per layer  y = GELU(SpectralConv(n) + 1x1 n),
+        r = h + scale * sigmoid(gate(n)) * norm(y),  n = norm(r),  h = r;  output project(n)
+
+    ``gate``: "none", "element" (a 1x1 convolution of n) or "sample" (a linear map of n's mean over
+    the positions).  ``norm``: "rms" or "layer".  The layer kernels are ``residual_norm``'s, forward
+    and backward, and the spectral convolutions the library's; 1x1 convolutions and GELU run as torch
+    operations in full float32.  Interfaces as FNO2d's: ``forward_device``, ``forward_autograd``,
+    ``forward(x, use_supa)``."""
+
+    def __init__(self, modes1: int = 12, modes2: int = 12, width: int = 32, n_layers: int = 4, in_channels: int = 10,
+                 out_channels: int = 1, gate: str = "element", norm: str = "rms", scale: float = 0.5):
+        super().__init__()
+        if n_layers < 1:
+            raise ValueError("at least one layer")
+        if gate not in ("none", "element", "sample"):
+            raise ValueError(f"gate must be 'none', 'element' or 'sample', got {gate!r}")
+        if norm not in ("rms", "layer"):
+            raise ValueError(f"norm must be 'rms' or 'layer', got {norm!r}")
+        self.in_channels, self.out_channels, self.width, self.norm = in_channels, out_channels, width, norm
+        self.lift = nn.Conv2d(in_channels + 2, width, 1)
+        self.first_weight = nn.Parameter(torch.ones(width))
+        self.layers = nn.ModuleList(
+            [ResidualFourierLayer(width, modes1, modes2, gate, scale) for _ in range(n_layers)])
+        self.project = nn.Sequential(nn.Conv2d(width, 128, 1), nn.GELU(), nn.Conv2d(128, out_channels, 1))
+
+    def _run(self, x: torch.Tensor, spectral, join) -> torch.Tensor:
+        if x.dim() != 4 or x.shape[1] != self.in_channels:
+            raise ValueError(f"x must be [B,{self.in_channels},H,W], got {tuple(x.shape)}")
+        x = x.to(torch.float32)
+        h = _conv1x1(self.lift, torch.cat([x, FNO2d.get_grid(x.shape, x.device)], dim=1)).contiguous()
+        h, n = join(h, pre_weight=self.first_weight, kind=self.norm)
+        for layer in self.layers:
+            y = F.gelu(spectral(layer.spectral_conv, n) + _conv1x1(layer.conv, n))
+            gate = layer.gate_of(n)
+            h, n = join(h, y, post_weight=layer.post_weight, gate=gate, scale=layer.scale,
+                        pre_weight=layer.next_weight, kind=self.norm)
+        return _conv1x1(self.project[2], F.gelu(_conv1x1(self.project[0], n)))
+
+    def _run_device(self, x: torch.Tensor, spectral) -> torch.Tensor:
+        def join(h, y=None, gate=None, **more):
+            return residual_norm(h, y, gate=gate, gate_activation="none" if gate is None else "sigmoid", **more)
+
+        return self._run(x, spectral, join)
+
+    def forward_autograd(self, x: torch.Tensor) -> torch.Tensor:
+        """Differentiable forward on x's CUDA device."""
+        if not x.is_cuda:
+            raise RuntimeError("forward_autograd needs a CUDA tensor")
+        return self._run_device(x, lambda sc, n: spectral_conv2d_autograd(n, sc.weights1, sc.weights2, sc.modes1,
+                                                                          sc.modes2))
+
+    @torch.no_grad()
+    def forward_device(self, x: torch.Tensor) -> torch.Tensor:
+        """Forward on x's CUDA device, [B, T, H, W] to [B, out_channels, H, W]."""
+        if not x.is_cuda:
+            raise RuntimeError("forward_device needs a CUDA tensor")
+        return self._run_device(x, lambda sc, n: sc(n))
+
+    def forward(self, x: torch.Tensor, use_supa: bool = True) -> torch.Tensor:
+        """As FNO2d's: on the CUDA device with a host result, or (``use_supa=False``) in torch
+        operations on the host."""
+        if use_supa:
+            device = x.device if x.is_cuda else torch.device("cuda", torch.cuda.current_device())
+            return self.forward_device(x.to(device=device, dtype=torch.float32)).cpu()
+        return self._run(x.cpu(), lambda sc, n: sc(n, use_supa=False), _residual_norm_host)
 
 
 def count_parameters(model: nn.Module) -> int:

@@ -13,7 +13,12 @@ Reference recipe kept: FNO2d(width 32, 4 layers, 10 input frames), Adam(lr 2e-4,
   (``FNO2d.forward_device``), instead of the reference's CPU torch path (``use_supa=False``);
 * batches are drawn from a seeded permutation on the device, not a host DataLoader.
 
+Beyond the recipe, off unless asked for: clipping by the global gradient norm (``max_grad_norm``), the
+Adam step that applies the clipping factor itself (``fused_adam``, ``optim_ops.FusedAdam``), and the
+stack with a residual stream (``--residual``, ``fno_model.ResidualFNO2d``).
+
     python birensupa-spectralconv_b200/fno_train.py --epochs 5 --n-train 256 --n-test 64
+    python birensupa-spectralconv_b200/fno_train.py --residual element --layers 8 --fused-adam --max-grad-norm 1.0
 """
 
 from __future__ import annotations
@@ -31,6 +36,7 @@ if str(PKG_DIR) not in sys.path:
     sys.path.insert(0, str(PKG_DIR))
 
 import fno_model  # noqa: E402
+import optim_ops  # noqa: E402
 import scx_data  # noqa: E402
 
 
@@ -42,7 +48,7 @@ def relative_l2(pred: torch.Tensor, target: torch.Tensor) -> float:
     return float((diff / ref).mean().item())
 
 
-def evaluate(model: fno_model.FNO2d, x: torch.Tensor, y: torch.Tensor, batch_size: int) -> float:
+def evaluate(model: fno_model.FNO2d | fno_model.ResidualFNO2d, x: torch.Tensor, y: torch.Tensor, batch_size: int) -> float:
     """Test score with the fused device forward, batch by batch (train_official.py:47-53)."""
     model.eval()
     scores = []
@@ -52,16 +58,22 @@ def evaluate(model: fno_model.FNO2d, x: torch.Tensor, y: torch.Tensor, batch_siz
     return sum(scores) / max(len(scores), 1)
 
 
-def train(model: fno_model.FNO2d, x_train, y_train, x_test, y_test, *, epochs: int, batch_size: int = 16,
-          lr: float = 2.0e-4, weight_decay: float = 1.0e-4, seed: int = 0, scheduler: bool = True,
-          checkpoint: str | None = None, log=print) -> dict:
-    """Trains ``model`` (on the data's device) and returns a summary with the per-epoch losses."""
+def train(model: fno_model.FNO2d | fno_model.ResidualFNO2d, x_train, y_train, x_test, y_test, *, epochs: int,
+          batch_size: int = 16, lr: float = 2.0e-4, weight_decay: float = 1.0e-4, seed: int = 0,
+          scheduler: bool = True, checkpoint: str | None = None, max_grad_norm: float | None = None,
+          fused_adam: bool = False, log=print) -> dict:
+    """Trains ``model`` (on the data's device) and returns a summary with the per-epoch losses, and
+    with ``max_grad_norm`` the gradient norm of each epoch's last step."""
     device = x_train.device
     g = torch.Generator(device=device)
     g.manual_seed(seed)
-    optim = torch.optim.Adam(model.parameters(), lr=lr, weight_decay=weight_decay)
+    if fused_adam:
+        optim = optim_ops.FusedAdam(model.parameters(), lr=lr, weight_decay=weight_decay, max_norm=max_grad_norm)
+    else:
+        optim = torch.optim.Adam(model.parameters(), lr=lr, weight_decay=weight_decay)
     sched = torch.optim.lr_scheduler.CosineAnnealingLR(optim, T_max=max(epochs, 3)) if scheduler else None
     n = x_train.shape[0]
+    grad_norm = None
     history, best_l2, step = [], float("inf"), 0
     t0 = time.time()
     for epoch in range(epochs):
@@ -75,7 +87,11 @@ def train(model: fno_model.FNO2d, x_train, y_train, x_test, y_test, *, epochs: i
             pred = model.forward_autograd(x)
             loss = torch.norm(pred - y) / torch.norm(y).clamp_min(1e-12)
             loss.backward()
+            if max_grad_norm is not None and not fused_adam:
+                grad_norm = optim_ops.clip_grad_norm_(model.parameters(), max_grad_norm)
             optim.step()
+            if fused_adam:
+                grad_norm = optim.last_norm
             loss_sum += float(loss.item())
             count += 1
             step += 1
@@ -91,6 +107,8 @@ def train(model: fno_model.FNO2d, x_train, y_train, x_test, y_test, *, epochs: i
                            checkpoint)
         history.append({"epoch": epoch + 1, "step": step, "train_l2": train_l2, "test_l2": test_l2,
                         "lr": optim.param_groups[0]["lr"]})
+        if grad_norm is not None:
+            history[-1]["grad_norm"] = float(grad_norm)
         log(f"step {step:5d} | epoch {epoch + 1:3d} | train_l2={train_l2:.6f} | test_l2={test_l2:.6f} | "
             f"best_l2={best_l2:.6f}{'  *best*' if improved else ''}")
     torch.cuda.synchronize(device)
@@ -108,15 +126,25 @@ def main(argv=None) -> None:
     ap.add_argument("--modes", type=int, default=16)
     ap.add_argument("--seed", type=int, default=20260722)
     ap.add_argument("--checkpoint", default=None)
+    ap.add_argument("--residual", choices=("none", "element", "sample"), default=None,
+                    help="train ResidualFNO2d with this gate instead of FNO2d")
+    ap.add_argument("--norm", choices=("rms", "layer"), default="rms", help="the norm of ResidualFNO2d")
+    ap.add_argument("--layers", type=int, default=4)
+    ap.add_argument("--max-grad-norm", type=float, default=None)
+    ap.add_argument("--fused-adam", action="store_true")
     args = ap.parse_args(argv)
     device = torch.device("cuda", torch.cuda.current_device())
     torch.manual_seed(args.seed)
     x_tr, y_tr = scx_data.fno_pairs_device(args.n_train, args.seed, device)
     x_te, y_te = scx_data.fno_pairs_device(args.n_test, args.seed + 1, device)
-    model = fno_model.FNO2d(modes1=args.modes, modes2=args.modes, width=32, n_layers=4, in_channels=10,
-                            out_channels=1).to(device)
+    sizes = dict(modes1=args.modes, modes2=args.modes, width=32, n_layers=args.layers, in_channels=10, out_channels=1)
+    if args.residual is None:
+        model = fno_model.FNO2d(**sizes).to(device)
+    else:
+        model = fno_model.ResidualFNO2d(**sizes, gate=args.residual, norm=args.norm).to(device)
     summary = train(model, x_tr, y_tr, x_te, y_te, epochs=args.epochs, batch_size=args.batch_size, lr=args.lr,
-                    seed=args.seed, checkpoint=args.checkpoint)
+                    seed=args.seed, checkpoint=args.checkpoint, max_grad_norm=args.max_grad_norm,
+                    fused_adam=args.fused_adam)
     print(json.dumps({k: v for k, v in summary.items() if k != "history"}, indent=1))
 
 
