@@ -19,9 +19,6 @@
 // norm adds the partials in the same order), so it is bitwise repeatable, with no atomics.  Sums
 // are held in 64 bits: the squares of fp32 and bf16 gradients leave the fp32 range well before the
 // gradients do.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -29,8 +26,13 @@
 
 #include "scx.h"
 #include "scx_internal.h"
+#include "scx_vec.cuh"
 
 namespace {
+
+using scx::from_f32;
+using scx::to_f32;
+using scx::Vec;
 
 constexpr int kThreads = 256;
 constexpr int kUnit = 1024;        // elements per unit
@@ -78,18 +80,6 @@ struct AdamScalars {
 
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ void from_f32(float& o, float v) { o = v; }
-__device__ __forceinline__ void from_f32(__nv_bfloat16& o, float v) { o = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void from_f32(__half& o, float v) { o = __float2half_rn(v); }
-
-template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
-    T v[V];
-};
 
 // Sum over the block, the same bits in every thread.
 __device__ double block_sum(double v) {
@@ -166,9 +156,11 @@ __device__ double square_sum(const T* __restrict__ p, long long n) {
     for (long long i = threadIdx.x; i < body; i += kThreads) {
         const Vec<T, V> x = q[i];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const double d = to_f32(x.v[j]);
-            s = fma(d, d, s);
+        for (int j = 0; j < V / 2; ++j) {
+            const float2 two = x.pair(j);
+            const double a = two.x, b = two.y;
+            s = fma(a, a, s);
+            s = fma(b, b, s);
         }
     }
     for (long long i = threadIdx.x; i < n - body * V; i += kThreads) {
@@ -198,7 +190,10 @@ __device__ void scale_piece(T* __restrict__ p, long long n, float c) {
         for (int d = 0; d < kDeep; ++d) {
             if (i < d * kThreads) break;
 #pragma unroll
-            for (int j = 0; j < V; ++j) from_f32(x[d].v[j], to_f32(x[d].v[j]) * c);
+            for (int j = 0; j < V / 2; ++j) {
+                const float2 two = x[d].pair(j);
+                x[d].set_pair(j, make_float2(two.x * c, two.y * c));
+            }
             q[i - d * kThreads] = x[d];
         }
     }
@@ -311,10 +306,12 @@ __device__ void adam_piece(T* __restrict__ p, const T* __restrict__ g, float* __
         for (int d = 0; d < DEEP; ++d) {
             if (i < d * kThreads) break;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float x = to_f32(pi[d].v[j]);
-                adam_one(x, to_f32(gi[d].v[j]), mi[d].v[j], vi[d].v[j], c, k, s);
-                from_f32(pi[d].v[j], x);
+            for (int j = 0; j < V / 2; ++j) {
+                float2 two = pi[d].pair(j);
+                const float2 g2 = gi[d].pair(j);
+                adam_one(two.x, g2.x, mi[d].w[2 * j], vi[d].w[2 * j], c, k, s);
+                adam_one(two.y, g2.y, mi[d].w[2 * j + 1], vi[d].w[2 * j + 1], c, k, s);
+                pi[d].set_pair(j, two);
             }
             pv[i - d * kThreads] = pi[d];
             mv[i - d * kThreads] = mi[d];

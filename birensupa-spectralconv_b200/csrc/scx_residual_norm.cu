@@ -300,21 +300,21 @@ __global__ void __launch_bounds__(kAnyThreads) any_sums_kernel(const __grid_cons
 
 // ---------------------------------------------------------------------------- the last sums
 
-constexpr int kFinishChannels = 8, kFinishRows = 64;
-constexpr int kFinishThreads = kFinishChannels * kFinishRows;
+constexpr int kFinishThreads = 512;
 
 // Sums over a block's rows, in 64 bits and a fixed order; valid in row 0.
+template <int CH>
 __device__ double2 sum_rows(double2 v) {
-    __shared__ double2 red[kFinishThreads / 32][kFinishChannels];
+    __shared__ double2 red[kFinishThreads / 32][CH];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    for (int o = 16; o >= kFinishChannels; o /= 2) {
+    for (int o = 16; o >= CH; o /= 2) {
         v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
         v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
     }
     __syncthreads();
-    if (lane < kFinishChannels) red[warp][lane] = v;
+    if (lane < CH) red[warp][lane] = v;
     __syncthreads();
-    if (threadIdx.x < kFinishChannels) {
+    if (threadIdx.x < CH) {
         for (int k = 1; k < kFinishThreads / 32; ++k) {
             v.x += red[k][lane].x;
             v.y += red[k][lane].y;
@@ -324,14 +324,16 @@ __device__ double2 sum_rows(double2 v) {
 }
 
 // Adds the parts' sums per channel, and the slots of each sample into the gradient of its gate.  Grid
-// (channels / 8, 2 + samples): y = 0 the norm before the next block, 1 the norm after the block and
-// the scale, from 2 on the gates.  Latency is all there is to it (a few hundred rows per channel):
-// narrow blocks and 64 rows of threads keep the chains of loads short (8 us at 32 rows of 32
-// channels, under 4 us so).
-template <typename T>
+// (channels / CH, 2 + samples): y = 0 the norm before the next block, 1 the norm after the block and
+// the scale, from 2 on the gates.  Latency is all there is to it, a few hundred rows per channel:
+// with few channels, 64 rows of 8 threads keep the chains of loads short (36 channels of 7 samples:
+// 7.7 us cold, 12.3 us with 32 rows of 32); with many, whole lines count (2048 channels: 13 us with 8
+// threads to a row, 9 us with 32).
+template <typename T, int CH>
 __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const __grid_constant__ Problem p) {
-    const int row = threadIdx.x / kFinishChannels;
-    const int c = blockIdx.x * kFinishChannels + threadIdx.x % kFinishChannels;
+    constexpr int kFinishRows = kFinishThreads / CH;
+    const int row = threadIdx.x / CH;
+    const int c = blockIdx.x * CH + threadIdx.x % CH;
     const bool live = c < p.channels;
     const float w = live ? weight<T>(p.post_w, c, p.wide, 1.f) : 0.f, b = live ? weight<T>(p.post_b, c, p.wide, 0.f) : 0.f;
     const float scale = p.scale * (live ? weight<T>(p.scale_w, c, p.wide, 1.f) : 0.f);
@@ -348,7 +350,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const __grid_con
 #pragma unroll 4
             for (long long k = part_of_tile(p, sample * p.tiles_per_sample) + row; k <= last; k += kFinishRows)
                 if (live) add_slot(s, k, sample, 1.0);
-            s = sum_rows(s);
+            s = sum_rows<CH>(s);
             if (row != 0 || !live) continue;
             const size_t g = static_cast<size_t>(sample) * p.channels + c;
             float slope;
@@ -380,7 +382,7 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const __grid_con
             s.y += at[p.channels];
         }
     }
-    s = sum_rows(s);
+    s = sum_rows<CH>(s);
     if (row != 0 || !live) return;
     if (!second) {
         if (p.d_pre_w) store_weight<T>(p.d_pre_w, c, p.wide, static_cast<float>(s.x));
@@ -524,8 +526,10 @@ cudaError_t backward(Problem& p, cudaStream_t s) {
     if (e == cudaErrorNotSupported) e = any_backward<T>(p, s);
     if (e != cudaSuccess || !p.sums) return e;
     const int gates = p.slots && p.dgate ? static_cast<int>(std::min<long long>(p.batch, 1024)) : 0;
-    return scx::launch_chained(finish_kernel<T>, dim3((p.channels + kFinishChannels - 1) / kFinishChannels, 2 + gates),
-                               dim3(kFinishThreads), 0, s, p);
+    const bool many = p.channels >= 1024;
+    const int ch = many ? 32 : 8;
+    return scx::launch_chained(many ? finish_kernel<T, 32> : finish_kernel<T, 8>,
+                               dim3((p.channels + ch - 1) / ch, 2 + gates), dim3(kFinishThreads), 0, s, p);
 }
 
 }  // namespace

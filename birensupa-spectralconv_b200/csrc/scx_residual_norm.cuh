@@ -2,14 +2,19 @@
 // activation, and how a backward's blocks split the positions.
 #pragma once
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <cstdint>
 
 #include <cuda_runtime.h>
 
+#include "scx_vec.cuh"
+
 namespace scx_rn {
+
+using scx::from_f32;
+using scx::load_vec;
+using scx::store_vec;
+using scx::to_f32;
+using scx::Vec;
 
 enum : int { kF32 = 0, kBf16 = 1, kF16 = 2 };
 enum : int { kRms = 0, kLayer = 1 };
@@ -65,55 +70,12 @@ __device__ __forceinline__ float* slot_of(const Problem& p, long long b, long lo
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ void from_f32(float& o, float v) { o = v; }
-__device__ __forceinline__ void from_f32(__nv_bfloat16& o, float v) { o = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void from_f32(__half& o, float v) { o = __float2half_rn(v); }
-
-template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
-    T v[V];
-};
-
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> load_vec(const void* p, size_t e) {
-    return *reinterpret_cast<const Vec<T, V>*>(static_cast<const T*>(p) + e);
-}
-
-template <typename T, int V>
-__device__ __forceinline__ void store_vec(void* p, size_t e, const Vec<T, V>& v) {
-    *reinterpret_cast<Vec<T, V>*>(static_cast<T*>(p) + e) = v;
-}
-
 // Two fp32 values at once: sm_100a has packed fp32 arithmetic, which halves the instructions of
 // these kernels' inner loops (the token kernels in bf16 are bound by them).
 __device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
-
-__device__ __forceinline__ float2 unpack(float a, float b) { return make_float2(a, b); }
-__device__ __forceinline__ float2 unpack(__nv_bfloat16 a, __nv_bfloat16 b) {
-    return make_float2(__bfloat162float(a), __bfloat162float(b));
-}
-__device__ __forceinline__ float2 unpack(__half a, __half b) { return make_float2(__half2float(a), __half2float(b)); }
-
-__device__ __forceinline__ void pack(float& a, float& b, float2 v) {
-    a = v.x;
-    b = v.y;
-}
-__device__ __forceinline__ void pack(__nv_bfloat16& a, __nv_bfloat16& b, float2 v) {
-    const __nv_bfloat162 o = __floats2bfloat162_rn(v.x, v.y);
-    a = o.x;
-    b = o.y;
-}
-__device__ __forceinline__ void pack(__half& a, __half& b, float2 v) {
-    const __half2 o = __floats2half2_rn(v.x, v.y);
-    a = __low2half(o);
-    b = __high2half(o);
-}
 
 template <typename T>
 __device__ __forceinline__ float weight(const void* w, int c, bool wide, float other) {
@@ -127,8 +89,39 @@ __device__ __forceinline__ void store_weight(void* w, int c, bool wide, float v)
     else from_f32(static_cast<T*>(w)[c], v);
 }
 
-// 1 / (1 + exp(-g)) to about 4 units in the last place.
-__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.f, 1.f + expf(-g)); }
+// Reciprocal and power of two from the hardware's approximations (PTX rcp and ex2, both within a few
+// units in the last place), and bounds that keep NaN.
+__device__ __forceinline__ float rcp_approx(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float exp2_approx(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float within(float v, float bound) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(bound));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(r), "f"(-bound));
+    return r;
+}
+
+// 1 / (1 + exp(-g)) of a pair.  exp(-g) = 2^t (1 + ln2 (t* - t)) with t* = -g log2(e) and t its rounding:
+// the difference comes exactly from a fused product, with log2(e) in two parts, so that the error
+// does not grow with g.  Relative error below 8 roundings down to g = -87, where the result leaves
+// the normal numbers and is zero.
+__device__ __forceinline__ float2 sigmoid2(float2 g) {
+    constexpr float kLog2e = 1.44269504f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.69314718f;
+    g = make_float2(within(g.x, 88.f), within(g.y, 88.f));  // 2^t stays finite
+    const float2 t = mul2(g, both(-kLog2e));
+    const float2 over = fma2(g, both(kLog2eRest), fma2(g, both(kLog2e), t));  // t - t*
+    float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
+    e = add2(fma2(mul2(e, both(-kLn2)), over, e), both(1.f));
+    return make_float2(rcp_approx(e.x), rcp_approx(e.y));
+}
+__device__ __forceinline__ float sigmoid(float g) { return sigmoid2(both(g)).x; }
 
 // act(g) and its derivative.
 __device__ __forceinline__ float activate(float g, int act, float& slope) {
@@ -155,10 +148,10 @@ template <int P>
 __device__ __forceinline__ void activate_all(float2 (&g)[P], int act) {
     if (act == kActSilu) {
 #pragma unroll
-        for (int i = 0; i < P; ++i) g[i] = mul2(g[i], make_float2(sigmoid(g[i].x), sigmoid(g[i].y)));
+        for (int i = 0; i < P; ++i) g[i] = mul2(g[i], sigmoid2(g[i]));
     } else if (act == kActSigmoid) {
 #pragma unroll
-        for (int i = 0; i < P; ++i) g[i] = make_float2(sigmoid(g[i].x), sigmoid(g[i].y));
+        for (int i = 0; i < P; ++i) g[i] = sigmoid2(g[i]);
     }
 }
 
@@ -173,14 +166,14 @@ __device__ __forceinline__ void activate_all(float2 (&g)[P], float2 (&slope)[P],
     if (act == kActSilu) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const float2 s = make_float2(sigmoid(g[i].x), sigmoid(g[i].y));
+            const float2 s = sigmoid2(g[i]);
             g[i] = mul2(g[i], s);
             slope[i] = fma2(g[i], make_float2(1.f - s.x, 1.f - s.y), s);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            g[i] = make_float2(sigmoid(g[i].x), sigmoid(g[i].y));
+            g[i] = sigmoid2(g[i]);
             slope[i] = mul2(g[i], make_float2(1.f - g[i].x, 1.f - g[i].y));
         }
     }

@@ -297,8 +297,8 @@ struct Slots {
         }
 #pragma unroll
         for (int i = 0; i < P::kCount; ++i) {
-            if constexpr (V == 1) out[i] = unpack(v[2 * i].v[0], v[2 * i + 1].v[0]);
-            else out[i] = unpack(v[i / P::kSpots].v[i % P::kSpots * 2], v[i / P::kSpots].v[i % P::kSpots * 2 + 1]);
+            if constexpr (V == 1) out[i] = make_float2(v[2 * i].one(), v[2 * i + 1].one());
+            else out[i] = v[i / P::kSpots].pair(i % P::kSpots);
         }
     }
 
@@ -307,8 +307,12 @@ struct Slots {
         E o[EPT];
 #pragma unroll
         for (int i = 0; i < P::kCount; ++i) {
-            if constexpr (V == 1) pack(o[2 * i].v[0], o[2 * i + 1].v[0], v[i]);
-            else pack(o[i / P::kSpots].v[i % P::kSpots * 2], o[i / P::kSpots].v[i % P::kSpots * 2 + 1], v[i]);
+            if constexpr (V == 1) {
+                o[2 * i].set_one(v[i].x);
+                o[2 * i + 1].set_one(v[i].y);
+            } else {
+                o[i / P::kSpots].set_pair(i % P::kSpots, v[i]);
+            }
         }
 #pragma unroll
         for (int j = 0; j < EPT; ++j)

@@ -112,12 +112,20 @@ __device__ __forceinline__ void weights(const void* w, int c, bool live, bool wi
         for (int i = 0; i < VEC; i += kPer) {
             const Vec<float, kPer> v = load_vec<float, kPer>(w, c + i);
 #pragma unroll
-            for (int k = 0; k < kPer; ++k) out[i + k] = v.v[k];
+            for (int k = 0; k < kPer; ++k) out[i + k] = v.w[k];
         }
     } else {
         const Vec<T, VEC> v = load_vec<T, VEC>(w, c);
+        if constexpr (VEC == 1) {
+            out[0] = v.one();
+        } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) out[i] = to_f32(v.v[i]);
+            for (int i = 0; i < VEC / 2; ++i) {
+                const float2 two = v.pair(i);
+                out[2 * i] = two.x;
+                out[2 * i + 1] = two.y;
+            }
+        }
     }
 }
 
@@ -217,8 +225,10 @@ struct Slots {
             else if (here && team.has(j)) v[j] = load_vec<T, VEC>(from, row + team.channel(j));
         }
 #pragma unroll
-        for (int i = 0; i < NV * VEC / 2; ++i)
-            out[i] = unpack(v[2 * i / VEC].v[2 * i % VEC], v[(2 * i + 1) / VEC].v[(2 * i + 1) % VEC]);
+        for (int i = 0; i < NV * VEC / 2; ++i) {
+            if constexpr (VEC == 1) out[i] = make_float2(v[2 * i].one(), v[2 * i + 1].one());
+            else out[i] = v[2 * i / VEC].pair(i % (VEC / 2));
+        }
     }
 
     template <typename TEAM>
@@ -226,8 +236,14 @@ struct Slots {
                                                  const float2 (&v)[NV * VEC / 2]) {
         E o[NV];
 #pragma unroll
-        for (int i = 0; i < NV * VEC / 2; ++i)
-            pack(o[2 * i / VEC].v[2 * i % VEC], o[(2 * i + 1) / VEC].v[(2 * i + 1) % VEC], v[i]);
+        for (int i = 0; i < NV * VEC / 2; ++i) {
+            if constexpr (VEC == 1) {
+                o[2 * i].set_one(v[i].x);
+                o[2 * i + 1].set_one(v[i].y);
+            } else {
+                o[2 * i / VEC].set_pair(i % (VEC / 2), v[i]);
+            }
+        }
 #pragma unroll
         for (int j = 0; j < NV; ++j)
             if (here && team.has(j)) store_vec<T, VEC>(to, row + team.channel(j), o[j]);
@@ -362,7 +378,7 @@ __device__ void store_sums(const Problem& p, const TEAM& team, float* shared, co
         for (int i = 0; i < VEC; i += kPer) {
             Vec<float, kPer> o;
 #pragma unroll
-            for (int k = 0; k < kPer; ++k) o.v[k] = v[j * VEC + i + k];
+            for (int k = 0; k < kPer; ++k) o.w[k] = v[j * VEC + i + k];
             store_vec<float, kPer>(out, c + i, o);
         }
     }

@@ -113,6 +113,25 @@ def test_gates(gate, act, shape, dim, cuda_device):
     _run(t, dim, dr, dn, kind="layer", act=act)
 
 
+def test_the_sigmoid_over_its_range(cuda_device):
+    """x = 0 and y = 1 without norms: r is the activation itself.  Within 10 roundings of the value where
+    that is a normal number, below the smallest of them otherwise; the ends and NaN as they are."""
+    g = torch.cat([torch.linspace(-95.0, 95.0, 200_003), torch.linspace(-1.0, 1.0, 100_001),
+                   torch.tensor([float("inf"), float("-inf"), float("nan"), 0.0, -0.0, 3e38, -3e38, 1e-40])]).to(cuda_device)
+    g = g[:g.numel() // 4 * 4].view(-1, 4) if g.numel() % 4 else g.view(-1, 4)
+    for act in ("sigmoid", "silu"):
+        r, _ = residual_norm(torch.zeros_like(g), torch.ones_like(g), gate=g, gate_activation=act, post_norm=False,
+                             pre_norm=False, dim=-1)
+        s = torch.special.expit(g.double())
+        want = s if act == "sigmoid" else g.double() * s
+        finite = torch.isfinite(want)
+        off = (r.double() - want).abs()[finite]
+        # where the sigmoid is below the normal numbers it may be zero
+        small = torch.where(s < 1.2e-38, want.abs(), 0 * s)[finite]
+        assert bool((off <= 10 * 2.0**-24 * want.abs()[finite] + small + 1.2e-38).all())
+        assert torch.equal(torch.isnan(r)[~finite], torch.isnan(want)[~finite])
+
+
 @pytest.mark.parametrize("shape, dim", [((3, 19, 40), -1), ((2, 32, 8, 12), 1), ((1, 2, 3000), -1)], ids=str)
 @pytest.mark.parametrize("option", ["no_vectors", "narrow", "number", "no_post", "no_pre", "no_y", "only_dr", "only_dn",
                                     "frozen_vectors", "frozen_y", "frozen_x", "sample_frozen", "weights_only"])
