@@ -570,6 +570,11 @@ extern "C" int scx_residual_norm_bwd(const scx_residual_norm_config* cfg, const 
         !valid_pointer(g->d_scale, cfg->weight_dtype, false) || workspace == nullptr ||
         reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < layout_of(*cfg).total)
         return cudaErrorInvalidValue;
+    // a gradient of what the forward did not have would be left unwritten
+    if ((!t->y && (g->dy || g->dgate || g->d_post_weight || g->d_post_bias || g->d_scale)) ||
+        (cfg->gate_mode == kGateNone && g->dgate) || (!cfg->post_norm && (g->d_post_weight || g->d_post_bias)) ||
+        (!cfg->pre_norm && (g->dn || g->d_pre_weight || g->d_pre_bias)))
+        return cudaErrorInvalidValue;
     Problem p = problem_of(*cfg, *t);
     p.dr = g->dr;
     p.dn = p.pre ? g->dn : nullptr;

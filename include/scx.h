@@ -368,7 +368,8 @@ int scx_adam_step(int n_tensors, void* const* params, const void* const* grads,
  * weights and scale vector then are ones, biases zeros (at most 262144 channels); y NULL: r = x (t.r is not written), n =
  * pre(x).  post_norm 0: z = y; pre_norm 0: no n.  The scale vector multiplies config.scale.
  * Statistics and sums are fp32, and n is computed from the unrounded r.  stats (may be NULL in
- * the forward): [4][batch*length] floats for the backward. */
+ * the forward): [4][batch*length] floats for the backward.  Outputs must not overlap the inputs or
+ * one another. */
 #define SCX_NORM_RMS 0
 #define SCX_NORM_LAYER 1
 #define SCX_GATE_NONE 0
@@ -393,7 +394,8 @@ typedef struct {
 } scx_residual_norm_grads;
 int scx_residual_norm_fwd(const scx_residual_norm_config* config, const scx_residual_norm_tensors* t,
                           scx_stream_t stream);
-/* Backward, from the forward's inputs and stats (t.r and t.n are not read).  workspace: device
+/* Backward, from the forward's inputs and stats (t.r and t.n are not read); gradients of what the
+ * forward did not have (y, a gate, a norm) are refused.  workspace: device
  * memory of scx_residual_norm_bwd_workspace_size() bytes, 16-byte aligned, in use until the
  * call's kernels end; 0 on an invalid or empty configuration, for which the call is refused. */
 size_t scx_residual_norm_bwd_workspace_size(const scx_residual_norm_config* config);

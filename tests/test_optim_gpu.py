@@ -446,3 +446,31 @@ def test_versions_move_with_the_step(cuda_device):
     version = p._version
     opt.step()
     assert p._version > version and float(p.detach()[0]) < 1.0
+
+
+def test_more_than_2_31_values(cuda_device):
+    """One tensor past 32-bit offsets, zero but for its ends, beside a small one."""
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of device memory")
+    n = (1 << 31) + 12_345
+    big = torch.zeros(n, dtype=torch.bfloat16, device=cuda_device)
+    big[:100], big[-100:] = 3.0, 4.0
+    small = torch.full((5,), 2.0, device=cuda_device)
+    want = math.sqrt(100 * 9 + 100 * 16 + 5 * 4)
+    assert abs(float(optim_ops.grad_norm([big, small])) - want) <= 1.01 * U32 * want
+    p = torch.full((n,), 1.0, dtype=torch.bfloat16, device=cuda_device)
+    m, v = torch.zeros(n, device=cuda_device), torch.zeros(n, device=cuda_device)
+    step = torch.zeros((), device=cuda_device)
+    optim_ops.adam_step_([p], [big], [m], [v], [step], lr=0.25, max_norm=want / 2)
+    assert float(m[-1]) > 0.0 and float(m[100]) == 0.0 and float(p[n // 2]) == 1.0
+    assert float(p[0]) == float(p[-1]) == 0.75 and float(p[-101]) == 1.0  # a first step moves by lr
+    optim_ops.clip_grads_([big, small], want / 2)
+    assert float(big[0]) == 1.5 and float(big[-1]) == 2.0 and float(big[-101]) == 0.0 and float(small[0]) == 1.0
+
+
+def test_only_empty_tensors(cuda_device):
+    empty = [torch.zeros(0, device=cuda_device), torch.zeros(3, 0, dtype=torch.complex64, device=cuda_device)]
+    assert float(optim_ops.grad_norm(empty)) == 0.0 and float(optim_ops.clip_grads_(empty, 1.0)) == 0.0
+    steps = [torch.zeros((), device=cuda_device) for _ in empty]
+    got = optim_ops.adam_step_(empty, empty, empty, empty, steps, lr=1.0, max_norm=1.0)
+    assert float(got) == 0.0 and [float(s) for s in steps] == [1.0, 1.0]

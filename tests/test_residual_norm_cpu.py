@@ -70,6 +70,19 @@ def test_backward_refused(bad):
     assert _scx.lib.scx_residual_norm_bwd(ctypes.byref(config), ctypes.byref(t), ctypes.byref(g), ws, size, None) == INVALID
 
 
+@pytest.mark.parametrize("config, y, grads", [
+    (dict(), None, dict(dy=512)), (dict(), None, dict(d_scale=512)), (dict(), None, dict(d_post_weight=512)),
+    (dict(), 512, dict(dgate=512)), (dict(post_norm=0), 512, dict(d_post_bias=512)),
+    (dict(pre_norm=0), 512, dict(dn=512)), (dict(pre_norm=0), 512, dict(d_pre_weight=512)),
+])
+def test_gradients_of_what_is_not_there_are_refused(config, y, grads):
+    c = _config(**config)
+    need = _scx.lib.scx_residual_norm_bwd_workspace_size(ctypes.byref(c))
+    g = _scx.ResidualNormGrads(dr=8192, dx=16384, **grads)
+    assert _scx.lib.scx_residual_norm_bwd(ctypes.byref(c), ctypes.byref(_tensors(y=y)), ctypes.byref(g),
+                                          ctypes.c_void_p(4096), need, None) == INVALID
+
+
 def test_python_refusals():
     op = residual_norm_ops.residual_norm
     x = torch.zeros(2, 4, 3)

@@ -331,3 +331,34 @@ def test_other_types_on_the_device_are_refused(cuda_device):
         residual_norm(x, pre_weight=torch.ones(4))
     with pytest.raises(RuntimeError, match="float32"):
         residual_norm(x.double())
+
+
+@pytest.mark.parametrize("dim, shape", [(-1, (2, 551_000, 2048)), (1, (2, 36, 31_000_004)), (1, (1, 33, 66_000_003))], ids=str)
+def test_offsets_past_32_bits(dim, shape, cuda_device):
+    """Over 2^31 elements, all zeros but the first and the last positions: those give what a tensor of
+    their own gives (bitwise, being the same sums in the same order), gradients included."""
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of device memory")
+    dev, half = cuda_device, torch.float16
+    C = shape[-1] if dim == -1 else shape[1]
+    few = 8
+
+    def ends(t):  # the first positions of the first sample and the last of the last one
+        return (t[0, :few], t[-1, -few:]) if dim == -1 else (t[0, :, :few], t[-1, :, -few:])
+
+    g = torch.Generator(device=dev).manual_seed(0)
+    full, small = {}, {}
+    for k in ("x", "y", "dr", "dn"):
+        full[k] = torch.zeros(shape, dtype=half, device=dev)
+        for part in ends(full[k]):
+            part.copy_(torch.randn(part.shape, device=dev, generator=g))
+        small[k] = torch.stack(ends(full[k]))
+    w = (1.0 + 0.1 * torch.randn(C, device=dev, generator=g))
+    got = []
+    for t in (full, small):
+        x, y, v = t["x"].requires_grad_(True), t["y"].requires_grad_(True), w.clone().requires_grad_(True)
+        r, n = residual_norm(x, y, pre_weight=v, post_weight=w, dim=dim)
+        got.append((r, n, *torch.autograd.grad((r, n), (x, y, v), (t["dr"], t["dn"]))))
+    for a, b in zip(got[0][:4], got[1][:4]):
+        assert torch.equal(torch.stack(ends(a.detach())), b.detach())
+    torch.testing.assert_close(got[0][4], got[1][4], rtol=1e-5, atol=1e-5)
