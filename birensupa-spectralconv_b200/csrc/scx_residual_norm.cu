@@ -148,19 +148,29 @@ __global__ void __launch_bounds__(kAnyThreads) any_forward_kernel(const __grid_c
                                                        weight<T>(p.pre_b, c, p.wide, 0.f)));
         }
         if (live && at.c == 0 && p.stats) {
-            p.stats[q] = mean;
-            p.stats[p.positions + q] = rho;
-            p.stats[2 * p.positions + q] = mean2;
-            p.stats[3 * p.positions + q] = rho2;
+            if (p.channels_last) {
+                reinterpret_cast<float4*>(p.stats)[q] = make_float4(mean, rho, mean2, rho2);
+            } else {
+                p.stats[q] = mean;
+                p.stats[p.positions + q] = rho;
+                p.stats[2 * p.positions + q] = mean2;
+                p.stats[3 * p.positions + q] = rho2;
+            }
         }
     }
 }
 
 struct RowStats {
     float mean, rho, mean2, rho2;
-    __device__ __forceinline__ RowStats(const Problem& p, long long q)
-        : mean(p.stats[q]), rho(p.stats[p.positions + q]), mean2(p.stats[2 * p.positions + q]),
-          rho2(p.stats[3 * p.positions + q]) {}
+    __device__ __forceinline__ RowStats(const Problem& p, long long q) {
+        const float4 s = p.channels_last ? reinterpret_cast<const float4*>(p.stats)[q]
+                                         : make_float4(p.stats[q], p.stats[p.positions + q], p.stats[2 * p.positions + q],
+                                                       p.stats[3 * p.positions + q]);
+        mean = s.x;
+        rho = s.y;
+        mean2 = s.z;
+        rho2 = s.w;
+    }
 };
 
 template <typename T>
@@ -539,7 +549,7 @@ extern "C" int scx_residual_norm_fwd(const scx_residual_norm_config* cfg, const 
     if (!valid_config(cfg) || !t) return cudaErrorInvalidValue;
     if (cfg->batch == 0 || cfg->length == 0) return cudaSuccess;
     if (!valid_inputs(*cfg, *t) || !valid_pointer(t->r, cfg->dtype, t->y != nullptr) ||
-        !valid_pointer(t->n, cfg->dtype, cfg->pre_norm != 0) || !valid_pointer(t->stats, kF32, false))
+        !valid_pointer(t->n, cfg->dtype, cfg->pre_norm != 0) || !aligned(t->stats, 16))
         return cudaErrorInvalidValue;
     Problem p = problem_of(*cfg, *t);
     if (!p.y) p.r = nullptr;  // r is x
@@ -560,7 +570,7 @@ extern "C" int scx_residual_norm_bwd(const scx_residual_norm_config* cfg, const 
                                      const scx_residual_norm_grads* g, void* workspace, size_t workspace_bytes,
                                      scx_stream_t stream) {
     if (!valid_config(cfg) || !t || !g || cfg->batch == 0 || cfg->length == 0) return cudaErrorInvalidValue;
-    if (!valid_inputs(*cfg, *t) || !valid_pointer(t->stats, kF32, true) || !valid_pointer(g->dr, cfg->dtype, false) ||
+    if (!valid_inputs(*cfg, *t) || t->stats == nullptr || !aligned(t->stats, 16) || !valid_pointer(g->dr, cfg->dtype, false) ||
         !valid_pointer(g->dn, cfg->dtype, false) || !valid_pointer(g->dx, cfg->dtype, false) ||
         !valid_pointer(g->dy, cfg->dtype, false) || !valid_pointer(g->dgate, cfg->dtype, false) ||
         !valid_pointer(g->d_post_weight, cfg->weight_dtype, false) ||

@@ -32,7 +32,7 @@ struct Problem {
     float eps, inv_c, scale;
     const void *x, *y, *gate, *post_w, *post_b, *pre_w, *pre_b, *scale_w;
     void *r, *n;
-    float* stats;  // [4][positions]: post mean, post rho, pre mean, pre rho
+    float* stats;  // post mean, post rho, pre mean, pre rho: [positions][4] of tokens, [4][positions] of fields
     const void *dr, *dn;
     void *dx, *dy, *dgate, *d_post_w, *d_post_b, *d_pre_w, *d_pre_b, *d_scale;
     int sums;        // whether any gradient summed over positions is wanted
@@ -193,9 +193,12 @@ inline int mode_of(const Problem& p) {
 template <typename V>
 constexpr bool kCopied = sizeof(V) >= 4;
 
+__device__ __forceinline__ unsigned shared_address(const void* p) {
+    return static_cast<unsigned>(__cvta_generic_to_shared(p));
+}
+
 template <typename V>
-__device__ __forceinline__ void copy_async(V* to, const void* from, bool live) {
-    const unsigned dst = static_cast<unsigned>(__cvta_generic_to_shared(to));
+__device__ __forceinline__ void copy_async(unsigned dst, const void* from, bool live) {
     const int bytes = live ? static_cast<int>(sizeof(V)) : 0;
     if constexpr (sizeof(V) == 16)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");

@@ -272,28 +272,56 @@ struct Tile {
     }
 };
 
-// A thread's slots for one tensor of one tile, and how it fills and reads them.
+// Where a thread's channels of one tile lie in a tensor, in bytes; the tensor's start where there is
+// nothing.
+template <int EPT>
+struct Spots {
+    size_t at[EPT];
+    bool live[EPT];
+};
+
+// A thread's slots in shared memory, and how it fills and reads them: slot k is a tensor of a tile, EPT
+// vectors, `pitch` bytes apart.
 template <typename T, int V, int EPT>
 struct Slots {
     using E = Vec<T, V>;
     using P = Pairs<V, EPT>;
+    unsigned char* base;
+    unsigned address, pitch;
+    size_t stride;  // from channel to channel, in bytes
+    int mine;
 
-    static __device__ __forceinline__ void fetch(E* slot, const void* from, size_t base, size_t stride, int end) {
+    __device__ __forceinline__ Slots(unsigned char* shared, const Problem& p, const Where& at)
+        : base(shared + threadIdx.x * sizeof(E)), address(shared_address(base)), pitch(blockDim.x * sizeof(E)),
+          stride(static_cast<size_t>(p.length) * sizeof(T)), mine(at.mine) {}
+
+    // `first`: the thread's first element
+    __device__ __forceinline__ Spots<EPT> spots(size_t first, bool live) const {
+        Spots<EPT> s;
+        const size_t bytes = live && mine > 0 ? first * sizeof(T) : 0;
+#pragma unroll
+        for (int j = 0; j < EPT; ++j) {
+            s.live[j] = live && j < mine;
+            s.at[j] = bytes + (j < mine && live ? j * stride : 0);
+        }
+        return s;
+    }
+
+    __device__ __forceinline__ void fetch(unsigned k, const void* from, const Spots<EPT>& s) const {
         if constexpr (kCopied<E>) {
 #pragma unroll
             for (int j = 0; j < EPT; ++j)
-                copy_async(slot + j * blockDim.x, static_cast<const T*>(from) + (j < end ? base + j * stride : 0), j < end);
+                copy_async<E>(address + (k * EPT + j) * pitch, static_cast<const char*>(from) + s.at[j], s.live[j]);
         }
     }
 
-    static __device__ __forceinline__ void read(const E* slot, const void* from, size_t base, size_t stride, int end,
-                                                float2 (&out)[P::kCount]) {
+    __device__ __forceinline__ void read(unsigned k, const void* from, const Spots<EPT>& s, float2 (&out)[P::kCount]) const {
         E v[EPT];
 #pragma unroll
         for (int j = 0; j < EPT; ++j) {
             v[j] = E{};
-            if constexpr (kCopied<E>) v[j] = slot[j * blockDim.x];
-            else if (j < end) v[j] = load_vec<T, V>(from, base + j * stride);
+            if constexpr (kCopied<E>) v[j] = *reinterpret_cast<const E*>(base + (k * EPT + j) * pitch);
+            else if (s.live[j]) v[j] = *reinterpret_cast<const E*>(static_cast<const char*>(from) + s.at[j]);
         }
 #pragma unroll
         for (int i = 0; i < P::kCount; ++i) {
@@ -302,8 +330,7 @@ struct Slots {
         }
     }
 
-    static __device__ __forceinline__ void store(void* to, size_t base, size_t stride, int end,
-                                                 const float2 (&v)[P::kCount]) {
+    __device__ __forceinline__ void store(void* to, const Spots<EPT>& s, const float2 (&v)[P::kCount]) const {
         E o[EPT];
 #pragma unroll
         for (int i = 0; i < P::kCount; ++i) {
@@ -316,7 +343,7 @@ struct Slots {
         }
 #pragma unroll
         for (int j = 0; j < EPT; ++j)
-            if (j < end) store_vec<T, V>(to, base + j * stride, o[j]);
+            if (s.live[j]) *reinterpret_cast<E*>(static_cast<char*>(to) + s.at[j]) = o[j];
     }
 };
 
@@ -343,19 +370,17 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) field_forward_kernel(const 
     extern __shared__ __align__(16) unsigned char dynamic[];
     auto& sh = *reinterpret_cast<Shared<V, EPT, LC>*>(dynamic);
     const Where at = where<V, EPT, LC>(p);
-    const size_t stride = static_cast<size_t>(p.length);
     const int tiles = static_cast<int>(p.tiles);
     constexpr int kTensors = forward_tensors(MODE);
-    auto* slots = reinterpret_cast<typename F::E*>(dynamic + sizeof(sh)) + threadIdx.x;
-    auto slot = [&](int turn, int tensor) { return slots + (turn * kTensors + tensor) * EPT * blockDim.x; };
+    const F slots(dynamic + sizeof(sh), p, at);
     using TILE = Tile<V, EPT, LC>;
     auto fetch = [&](const TILE& t, bool exists, int turn) {
         if (exists) {
-            const size_t base = t.base(p, at);
-            const int end = t.live(p, at) ? at.mine : 0;
-            F::fetch(slot(turn, 0), p.x, base, stride, end);
-            if constexpr (MODE != kNoBlock) F::fetch(slot(turn, 1), p.y, base, stride, end);
-            if constexpr (MODE == kFull) F::fetch(slot(turn, 2), p.gate, base, stride, end);
+            const Spots<EPT> spots = slots.spots(t.base(p, at), t.live(p, at));
+            const unsigned k = turn * kTensors;
+            slots.fetch(k, p.x, spots);
+            if constexpr (MODE != kNoBlock) slots.fetch(k + 1, p.y, spots);
+            if constexpr (MODE == kFull) slots.fetch(k + 2, p.gate, spots);
         }
         copy_commit();
     };
@@ -365,19 +390,20 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) field_forward_kernel(const 
     load_vectors<T>(sh, p, at.warps * EPT * LC);
     int turn = 0;
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
-        const size_t base = t.base(p, at);
-        const int end = t.live(p, at) ? at.mine : 0, sample = t.sample;
+        const Spots<EPT> spots = slots.spots(t.base(p, at), t.live(p, at));
+        const int sample = t.sample;
+        const unsigned slot = turn * kTensors;
         const size_t q0 = static_cast<size_t>(sample) * p.length + t.l0();
         const int live_pos = static_cast<int>(p.length) - t.l0();
         t.next(p, step.sample, step.index);
         fetch(t, tile + static_cast<int>(gridDim.x) < tiles, turn ^ 1);
         copy_wait<1>();
         float2 r[P::kCount], rho[P::kSpots], shift[P::kSpots];
-        F::read(slot(turn, 0), p.x, base, stride, end, r);
+        slots.read(slot, p.x, spots, r);
         if constexpr (MODE != kNoBlock) {
             float2 h[P::kCount], a[P::kCount];
-            F::read(slot(turn, 1), p.y, base, stride, end, h);
-            if constexpr (MODE == kFull) F::read(slot(turn, 2), p.gate, base, stride, end, a);
+            slots.read(slot + 1, p.y, spots, h);
+            if constexpr (MODE == kFull) slots.read(slot + 2, p.gate, spots, a);
             if (p.post) {
                 statistics<V, EPT, LC>(sh, p, h, at, rho, shift, p.stats ? p.stats + q0 : nullptr, live_pos);
 #pragma unroll
@@ -390,7 +416,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) field_forward_kernel(const 
                 const float2 z = fma2(h[i], P::channels(&sh.vec[kPostW][at.c0], i), P::channels(&sh.vec[kPostB][at.c0], i));
                 r[i] = MODE == kPlain ? add2(r[i], z) : fma2(a[i], z, r[i]);
             }
-            F::store(p.r, base, stride, end, r);
+            slots.store(p.r, spots, r);
         }
         if (!p.pre) continue;
         statistics<V, EPT, LC>(sh, p, r, at, rho, shift, p.stats ? p.stats + 2 * p.positions + q0 : nullptr, live_pos);
@@ -398,7 +424,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) field_forward_kernel(const 
         for (int i = 0; i < P::kCount; ++i)
             r[i] = fma2(fma2(r[i], rho[P::spot(i)], shift[P::spot(i)]), P::channels(&sh.vec[kPreW][at.c0], i),
                         P::channels(&sh.vec[kPreB][at.c0], i));
-        F::store(p.n, base, stride, end, r);
+        slots.store(p.n, spots, r);
     }
     copy_wait<0>();
 }
@@ -415,20 +441,22 @@ struct Saved {
 #pragma unroll
         for (int s = 0; s < kSpots; ++s) mean[s] = rho[s] = mean2[s] = rho2[s] = both(0.f);
         if (!t.live(p, at)) return;
-        const float* st = p.stats + static_cast<size_t>(t.sample) * p.length + t.l0() + at.pos * V;
-        const size_t row = static_cast<size_t>(p.positions);
+        // V divides the length, so V positions' numbers of one kind are one aligned access
+        const size_t q = static_cast<size_t>(t.sample) * p.length + t.l0() + at.pos * V, row = static_cast<size_t>(p.positions);
+        auto read = [&](size_t from, float2 (&to)[kSpots]) {
+            const Vec<float, V> v = load_vec<float, V>(p.stats, from);
 #pragma unroll
-        for (int s = 0; s < kSpots; ++s) {
-            const int b = V == 1 ? 0 : 1;
-            rho[s] = both(1.f);
-            if (p.post) {
-                mean[s] = make_float2(st[2 * s], st[2 * s + b]);
-                rho[s] = make_float2(st[row + 2 * s], st[row + 2 * s + b]);
-            }
-            if (p.dn) {
-                mean2[s] = make_float2(st[2 * row + 2 * s], st[2 * row + 2 * s + b]);
-                rho2[s] = make_float2(st[3 * row + 2 * s], st[3 * row + 2 * s + b]);
-            }
+            for (int s = 0; s < kSpots; ++s) to[s] = V == 1 ? both(v.w[0]) : make_float2(v.w[2 * s % V], v.w[(2 * s + 1) % V]);
+        };
+#pragma unroll
+        for (int s = 0; s < kSpots; ++s) rho[s] = both(1.f);
+        if (p.post) {
+            read(q, mean);
+            read(row + q, rho);
+        }
+        if (p.dn) {
+            read(2 * row + q, mean2);
+            read(3 * row + q, rho2);
         }
     }
 };
@@ -456,23 +484,21 @@ __global__ void __launch_bounds__(MAXW * 32, MAXW <= 10 ? 2 : 1) field_backward_
     auto& sh = *reinterpret_cast<Shared<V, EPT, LC>*>(dynamic);
     grid_dep_launch();
     const Where at = where<V, EPT, LC>(p);
-    const size_t stride = static_cast<size_t>(p.length);
     constexpr int kTensors = backward_tensors(MODE);
-    auto* slots = reinterpret_cast<typename F::E*>(dynamic + sizeof(sh)) + threadIdx.x;
-    auto slot = [&](int turn, int tensor) { return slots + (turn * kTensors + tensor) * EPT * blockDim.x; };
+    const F slots(dynamic + sizeof(sh), p, at);
     const int first = static_cast<int>(tile_begin(p, blockIdx.x)), last = static_cast<int>(tile_begin(p, blockIdx.x + 1));
     Saved<V> ahead;
     auto fetch = [&](const TILE& t, bool exists, int turn) {
         if (exists) {
-            const size_t base = t.base(p, at);
-            const int end = t.live(p, at) ? at.mine : 0;
-            if constexpr (MODE != kNoBlock) F::fetch(slot(turn, 1), p.y, base, stride, end);
+            const Spots<EPT> spots = slots.spots(t.base(p, at), t.live(p, at));
+            const unsigned k = turn * kTensors;
+            if constexpr (MODE != kNoBlock) slots.fetch(k + 1, p.y, spots);
             if (p.dn) {
-                F::fetch(slot(turn, 0), p.x, base, stride, end);
-                F::fetch(slot(turn, 2), p.dn, base, stride, end);
+                slots.fetch(k, p.x, spots);
+                slots.fetch(k + 2, p.dn, spots);
             }
-            if (p.dr) F::fetch(slot(turn, 3), p.dr, base, stride, end);
-            if constexpr (MODE == kFull) F::fetch(slot(turn, 4), p.gate, base, stride, end);
+            if (p.dr) slots.fetch(k + 3, p.dr, spots);
+            if constexpr (MODE == kFull) slots.fetch(k + 4, p.gate, spots);
             ahead.load(p, t, at);
         }
         copy_commit();
@@ -492,8 +518,9 @@ __global__ void __launch_bounds__(MAXW * 32, MAXW <= 10 ? 2 : 1) field_backward_
         return V == 1 ? (j % 2 ? sum[kind][j / 2].y : sum[kind][j / 2].x) : sum[kind][j % kAcc].x + sum[kind][j % kAcc].y;
     };
     for (int tile = first; tile < last; ++tile, turn ^= 1) {
-        const size_t base = t.base(p, at);
-        const int end = t.live(p, at) ? at.mine : 0, sample = t.sample;
+        const Spots<EPT> spots = slots.spots(t.base(p, at), t.live(p, at));
+        const int sample = t.sample;
+        const unsigned slot = turn * kTensors;
         const bool sample_ends = t.index + 1 == static_cast<int>(p.tiles_per_sample);
         float2 rho[kSpots], shift[kSpots], rho2[kSpots], shift2[kSpots];
 #pragma unroll
@@ -508,18 +535,18 @@ __global__ void __launch_bounds__(MAXW * 32, MAXW <= 10 ? 2 : 1) field_backward_
         copy_wait<1>();
         float2 h[N], a[N], slope[N], k[N], g[N];
         if constexpr (MODE != kNoBlock) {
-            F::read(slot(turn, 1), p.y, base, stride, end, h);
+            slots.read(slot + 1, p.y, spots, h);
 #pragma unroll
             for (int i = 0; i < N; ++i) h[i] = fma2(h[i], rho[P::spot(i)], shift[P::spot(i)]);
             if constexpr (MODE == kFull) {
-                F::read(slot(turn, 4), p.gate, base, stride, end, a);
+                slots.read(slot + 4, p.gate, spots, a);
                 activate_all(a, slope, p.act);
             }
             if constexpr (MODE == kSample) sample_gate<T, V, EPT>(p, at, sample, a);
         }
         if (p.dn) {
-            F::read(slot(turn, 0), p.x, base, stride, end, k);
-            F::read(slot(turn, 2), p.dn, base, stride, end, g);
+            slots.read(slot + 0, p.x, spots, k);
+            slots.read(slot + 2, p.dn, spots, g);
             float2 gk[N], m1[kSpots], m2[kSpots];
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -545,12 +572,12 @@ __global__ void __launch_bounds__(MAXW * 32, MAXW <= 10 ? 2 : 1) field_backward_
             for (int i = 0; i < N; ++i) g[i] = both(0.f);
         }
         if (p.dr) {
-            F::read(slot(turn, 3), p.dr, base, stride, end, k);
+            slots.read(slot + 3, p.dr, spots, k);
 #pragma unroll
             for (int i = 0; i < N; ++i) g[i] = add2(g[i], k[i]);
         }
         // g: the gradient of r
-        if (p.dx) F::store(p.dx, base, stride, end, g);
+        if (p.dx) slots.store(p.dx, spots, g);
         if constexpr (MODE != kNoBlock) {
             float2 kh[N];
 #pragma unroll
@@ -567,7 +594,7 @@ __global__ void __launch_bounds__(MAXW * 32, MAXW <= 10 ? 2 : 1) field_backward_
                 for (int i = 0; i < N; ++i)
                     a[i] = mul2(mul2(g[i], slope[i]),
                                 fma2(h[i], P::channels(&sh.vec[kPostW][at.c0], i), P::channels(&sh.vec[kPostB][at.c0], i)));
-                F::store(p.dgate, base, stride, end, a);
+                slots.store(p.dgate, spots, a);
             }
             if (p.dy) {
                 if (p.post) {
@@ -579,7 +606,7 @@ __global__ void __launch_bounds__(MAXW * 32, MAXW <= 10 ? 2 : 1) field_backward_
                     for (int i = 0; i < N; ++i)
                         k[i] = mul2(rho[P::spot(i)], add2(fma2(h[i], m2[P::spot(i)], k[i]), m1[P::spot(i)]));
                 }
-                F::store(p.dy, base, stride, end, k);
+                slots.store(p.dy, spots, k);
             }
             if (MODE == kSample && p.slots && (tile + 1 == last || sample_ends)) {
                 float* to = slot_of(p, blockIdx.x, sample);

@@ -20,20 +20,20 @@ namespace {
 
 constexpr int kMaxThreads = 512;
 constexpr int kAhead = 2;  // positions whose copies are under way while one is computed
-constexpr int kParts = kMaxThreads / 32 * 4;  // of the warps of a cluster
-constexpr int kPartBytes = 2 * kParts * sizeof(float2);
+constexpr int kParts = kMaxThreads / 32 * 4 * 2;  // two numbers per warp of a cluster
+constexpr int kPartBytes = 2 * kParts * sizeof(float);
 
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // Writes v to the same place of block `rank`'s shared memory as `at` has in this one's.
-__device__ __forceinline__ void store_in_block(float2* at, int rank, float2 v) {
+__device__ __forceinline__ void store_in_block(float* at, int rank, float v) {
     unsigned to;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
                  : "=r"(to)
                  : "r"(static_cast<unsigned>(__cvta_generic_to_shared(at))), "r"(rank));
-    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(v.x), "f"(v.y) : "memory");
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
 }
 
 // A cluster of CL blocks takes blockDim / tpr positions (one, where CL > 1), tpr threads (a power of
@@ -42,9 +42,9 @@ template <int VEC, int CL>
 struct Team {
     int tpr, me, row, rows, rank;
     int first, end;  // this thread's first channel, and where the block's channels end
-    float2* part;    // [2][kParts]
+    float* part;     // [2][kParts]
 
-    __device__ __forceinline__ Team(int threads, int columns, int channels, float2* shared)
+    __device__ __forceinline__ Team(int threads, int columns, int channels, float* shared)
         : tpr(threads), me(threadIdx.x % threads), row(threadIdx.x / threads), rows(blockDim.x / threads),
           rank(blockIdx.x % CL), first(rank * columns + me * VEC), end(min(channels, (rank + 1) * columns)), part(shared) {
         if (CL > 1) cluster_barrier();  // the others' shared memory is there
@@ -54,11 +54,13 @@ struct Team {
     __device__ __forceinline__ int channel(int j) const { return first + j * tpr * VEC; }
     __device__ __forceinline__ bool has(int j) const { return channel(j) < end; }
 
-    // Sums over the position's threads, the same bits in all of them.  Across warps every warp adds
-    // the warps' parts itself; `turn` alternates between calls, so that one barrier per call is
-    // enough.
+    // Sums K (one or two) numbers over the position's threads, the same bits in all of them.  Two share
+    // the steps: after the first, one half of the warp adds the first number and the other the second.
+    // Across warps every warp adds the warps' parts itself; `turn` alternates between calls, so that
+    // one barrier per call is enough.
     template <int K>
     __device__ __forceinline__ void sum(float (&v)[K], int& turn) {
+        const int lane = threadIdx.x % 32;
         if (CL == 1 && tpr < 32) {
             for (int o = tpr / 2; o > 0; o >>= 1) {
 #pragma unroll
@@ -66,37 +68,49 @@ struct Team {
             }
             return;
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-#pragma unroll
-            for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+        float s = v[0];
+        if (K == 2) {
+            const float give = lane < 16 ? v[K - 1] : v[0];
+            s = (lane < 16 ? v[0] : v[K - 1]) + __shfl_xor_sync(0xffffffffu, give, 16);
+        } else {
+            s += __shfl_xor_sync(0xffffffffu, s, 16);
         }
-        if (CL == 1 && tpr == 32) return;
-        float2* now = part + turn * kParts;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (CL == 1 && tpr == 32) {
+            const float other = K == 2 ? __shfl_xor_sync(0xffffffffu, s, 16) : s;
+            v[0] = lane < 16 ? s : other;
+            v[K - 1] = lane < 16 ? other : s;
+            return;
+        }
+        // the warps' numbers, K to a warp, in a row; a lane takes every 32nd, so always number lane % K
+        constexpr int kMost = kMaxThreads / 32;  // warps of a block
+        float* now = part + turn * kParts;
         turn ^= 1;
         const int warp = threadIdx.x / 32;
-        float2 s = make_float2(0.f, 0.f);
         if (CL > 1) {
-            const int lane = threadIdx.x % 32;
-            // one lane per block of the cluster
-            if (lane < CL) store_in_block(now + rank * (kMaxThreads / 32) + warp, lane, make_float2(v[0], v[K - 1]));
+            // to every block of the cluster: one lane per block and number
+            const float mine = __shfl_sync(0xffffffffu, s, lane < CL ? 0 : 16);
+            if (lane < CL * K) store_in_block(now + (rank * kMost + warp) * K + lane / CL, lane % CL, mine);
             __syncwarp();
             cluster_barrier();
+            s = 0.f;
 #pragma unroll
-            for (int e = 0; e < CL * (kMaxThreads / 32); e += 32) s = add2(s, now[e + lane]);
+            for (int e = 0; e < CL * kMost * K; e += 32) s += now[e + lane];
         } else {
-            if (threadIdx.x % 32 == 0) now[warp] = make_float2(v[0], v[K - 1]);
+            if (lane % 16 == 0 && lane < 16 * K) now[warp * K + lane / 16] = s;
             __syncthreads();
-            const int warps = tpr / 32;  // 2, 4, 8 or 16; the lanes past them hold zeros
-            const int lane = threadIdx.x % 16;
-            if (lane < warps) s = now[row * warps + lane];
+            const int warps = tpr / 32;  // 2, 4, 8 or 16
+            s = lane < warps * K ? now[row * warps * K + lane] : 0.f;
         }
-        v[0] = s.x;
-        v[K - 1] = s.y;
 #pragma unroll
-        for (int o = CL > 1 ? 16 : 8; o > 0; o >>= 1) {
-#pragma unroll
-            for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+        for (int o = 16; o >= K; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (K == 2) {
+            const float other = __shfl_xor_sync(0xffffffffu, s, 1);
+            v[0] = lane % 2 ? other : s;
+            v[K - 1] = lane % 2 ? s : other;
+        } else {
+            v[0] = s;
         }
     }
 };
@@ -198,31 +212,61 @@ struct Weights {
     }
 };
 
-// A thread's slots for one tensor of one position, and how it fills and reads them.
+// Where a thread's vectors of one position lie in a tensor, in bytes; zero where there is none.
+template <int NV>
+struct Row {
+    size_t at[NV];
+    bool live[NV];
+};
+
+// A thread's slots in shared memory, and how it fills and reads them: slot k is a tensor of a position
+// under way, NV vectors, `pitch` bytes apart.
 template <typename T, int VEC, int NV>
 struct Slots {
     using E = Vec<T, VEC>;
+    unsigned char* base;
+    unsigned address, pitch;
+    int channel[NV];  // in bytes
+    bool on[NV];
 
     template <typename TEAM>
-    static __device__ __forceinline__ void fetch(E* slot, const void* from, size_t row, const TEAM& team, bool here) {
-        if constexpr (kCopied<E>) {
+    __device__ __forceinline__ Slots(unsigned char* shared, const TEAM& team)
+        : base(shared + threadIdx.x * sizeof(E)), address(shared_address(base)), pitch(blockDim.x * sizeof(E)) {
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const bool live = here && team.has(j);
-                copy_async(slot + j * blockDim.x, static_cast<const T*>(from) + (live ? row + team.channel(j) : 0), live);
-            }
+        for (int j = 0; j < NV; ++j) {
+            on[j] = team.has(j);
+            channel[j] = on[j] ? team.channel(j) * static_cast<int>(sizeof(T)) : 0;
         }
     }
 
-    template <typename TEAM>
-    static __device__ __forceinline__ void read(const E* slot, const void* from, size_t row, const TEAM& team, bool here,
-                                                float2 (&out)[NV * VEC / 2]) {
+    // `first`: the position's first element
+    __device__ __forceinline__ Row<NV> row(size_t first, bool here) const {
+        Row<NV> r;
+        const size_t bytes = here ? first * sizeof(T) : 0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            r.at[j] = bytes + channel[j];
+            r.live[j] = here && on[j];
+        }
+        return r;
+    }
+
+    __device__ __forceinline__ void fetch(unsigned k, const void* from, const Row<NV>& r) const {
+        if constexpr (kCopied<E>) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                copy_async<E>(address + (k * NV + j) * pitch, static_cast<const char*>(from) + r.at[j], r.live[j]);
+        }
+    }
+
+    __device__ __forceinline__ void read(unsigned k, const void* from, const Row<NV>& r,
+                                         float2 (&out)[NV * VEC / 2]) const {
         E v[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             v[j] = E{};
-            if constexpr (kCopied<E>) v[j] = slot[j * blockDim.x];
-            else if (here && team.has(j)) v[j] = load_vec<T, VEC>(from, row + team.channel(j));
+            if constexpr (kCopied<E>) v[j] = *reinterpret_cast<const E*>(base + (k * NV + j) * pitch);
+            else if (r.live[j]) v[j] = *reinterpret_cast<const E*>(static_cast<const char*>(from) + r.at[j]);
         }
 #pragma unroll
         for (int i = 0; i < NV * VEC / 2; ++i) {
@@ -231,9 +275,7 @@ struct Slots {
         }
     }
 
-    template <typename TEAM>
-    static __device__ __forceinline__ void store(void* to, size_t row, const TEAM& team, bool here,
-                                                 const float2 (&v)[NV * VEC / 2]) {
+    __device__ __forceinline__ void store(void* to, const Row<NV>& r, const float2 (&v)[NV * VEC / 2]) const {
         E o[NV];
 #pragma unroll
         for (int i = 0; i < NV * VEC / 2; ++i) {
@@ -246,7 +288,7 @@ struct Slots {
         }
 #pragma unroll
         for (int j = 0; j < NV; ++j)
-            if (here && team.has(j)) store_vec<T, VEC>(to, row + team.channel(j), o[j]);
+            if (r.live[j]) *reinterpret_cast<E*>(static_cast<char*>(to) + r.at[j]) = o[j];
     }
 };
 
@@ -271,47 +313,46 @@ __global__ void __launch_bounds__(kMaxThreads) token_forward_kernel(const __grid
     using F = Slots<T, VEC, NV>;
     constexpr int N = NV * VEC / 2, kTensors = forward_tensors(MODE);
     extern __shared__ __align__(16) unsigned char dynamic[];
-    auto* part = reinterpret_cast<float2*>(dynamic);
+    auto* part = reinterpret_cast<float*>(dynamic);
     Team<VEC, CL> team(tpr, columns, p.channels, part);
     const int channels = p.channels;
     const long long block = blockIdx.x / CL, blocks = gridDim.x / CL;  // clusters
     const long long groups = (p.positions + team.rows - 1) / team.rows;
-    auto* slots = reinterpret_cast<typename F::E*>(dynamic + kPartBytes) + threadIdx.x;
-    auto slot = [&](int ring, int tensor) { return slots + (ring * kTensors + tensor) * NV * blockDim.x; };
-    auto gate_row = [&](long long q) {
-        return static_cast<size_t>(p.gate_mode == kGateSample ? q / p.length : q) * channels;
+    const F slots(dynamic + kPartBytes, team);
+    const auto& on = slots.on;
+    auto gate_row = [&](long long q, bool here) {
+        return slots.row(static_cast<size_t>(p.gate_mode == kGateSample ? q / p.length : q) * channels, here);
     };
     auto fetch = [&](long long group, int ring) {
         if (group < groups) {
             const long long q = group * team.rows + team.row;
             const bool here = q < p.positions;
-            const size_t row = static_cast<size_t>(q) * channels;
-            F::fetch(slot(ring, 0), p.x, row, team, here);
-            if constexpr (MODE != kNoBlock) F::fetch(slot(ring, 1), p.y, row, team, here);
-            if constexpr (MODE == kFull) F::fetch(slot(ring, 2), p.gate, here ? gate_row(q) : 0, team, here);
+            const Row<NV> row = slots.row(static_cast<size_t>(q) * channels, here);
+            const unsigned k = ring * kTensors;
+            slots.fetch(k, p.x, row);
+            if constexpr (MODE != kNoBlock) slots.fetch(k + 1, p.y, row);
+            if constexpr (MODE == kFull) slots.fetch(k + 2, p.gate, p.gate_mode == kGateSample ? gate_row(q, here) : row);
         }
         copy_commit();
     };
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) fetch(block + k * blocks, k);
     const Weights<T, VEC, NV> weight_of(p, team, MODE != kNoBlock);
-    bool on[NV];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) on[j] = team.has(j);
     int turn = 0, ring = 0;
     for (long long group = block; group < groups; group += blocks) {
         const long long q = group * team.rows + team.row;
         const bool here = q < p.positions;
-        const size_t row = static_cast<size_t>(q) * channels;
+        const Row<NV> row = slots.row(static_cast<size_t>(q) * channels, here);
+        const unsigned slot = ring * kTensors;
         fetch(group + kAhead * blocks, ring == 0 ? kAhead : ring - 1);
         copy_wait<kAhead>();
         float2 r[N], st = make_float2(0.f, 1.f), st2 = st;
-        F::read(slot(ring, 0), p.x, row, team, here, r);
+        slots.read(slot, p.x, row, r);
         if constexpr (MODE != kNoBlock) {
             float2 h[N], a[N];
-            F::read(slot(ring, 1), p.y, row, team, here, h);
+            slots.read(slot + 1, p.y, row, h);
             if constexpr (MODE == kFull) {
-                F::read(slot(ring, 2), p.gate, here ? gate_row(q) : 0, team, here, a);
+                slots.read(slot + 2, p.gate, kCopied<typename F::E> ? row : gate_row(q, here), a);
                 activate_all(a, p.act);
             }
             if (p.post) st = statistics<VEC, NV>(p, team, h, on, turn);
@@ -321,7 +362,7 @@ __global__ void __launch_bounds__(kMaxThreads) token_forward_kernel(const __grid
                 const float2 z = fma2(fma2(h[i], rho, shift), weight_of.w[i], weight_of.b[i]);
                 r[i] = MODE == kPlain ? add2(r[i], z) : fma2(a[i], z, r[i]);
             }
-            F::store(p.r, row, team, here, r);
+            slots.store(p.r, row, r);
             clear_dead<VEC, NV>(r, on);
         }
         if (p.pre) {
@@ -331,14 +372,10 @@ __global__ void __launch_bounds__(kMaxThreads) token_forward_kernel(const __grid
             weight_pairs<T, VEC, NV>(p.pre_b, p, team, 0.f, b);
 #pragma unroll
             for (int i = 0; i < N; ++i) r[i] = fma2(fma2(r[i], rho, shift), weight_of.w2[i], b[i]);
-            F::store(p.n, row, team, here, r);
+            slots.store(p.n, row, r);
         }
-        if (p.stats && team.rank == 0 && team.me == 0 && here) {
-            p.stats[q] = st.x;
-            p.stats[p.positions + q] = st.y;
-            p.stats[2 * p.positions + q] = st2.x;
-            p.stats[3 * p.positions + q] = st2.y;
-        }
+        if (p.stats && team.rank == 0 && team.me == 0 && here)
+            reinterpret_cast<float4*>(p.stats)[q] = make_float4(st.x, st.y, st2.x, st2.y);
         ring = ring == kAhead ? 0 : ring + 1;
     }
     copy_wait<0>();
@@ -392,66 +429,69 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
     // the tensors' places in a ring slot
     constexpr int kX = 0, kDn = 1, kDr = 2, kY = 3, kGate = 4;
     extern __shared__ __align__(16) unsigned char dynamic[];
-    auto* part = reinterpret_cast<float2*>(dynamic);
+    auto* part = reinterpret_cast<float*>(dynamic);
     grid_dep_launch();
     Team<VEC, CL> team(tpr, columns, p.channels, part);
     const int channels = p.channels;
     const long long block = blockIdx.x / CL;  // the cluster
-    auto* slots = reinterpret_cast<typename F::E*>(dynamic + kPartBytes) + threadIdx.x;
-    auto slot = [&](int ring, int tensor) { return slots + (ring * kTensors + tensor) * NV * blockDim.x; };
+    const F slots(dynamic + kPartBytes, team);
+    const auto& on = slots.on;
     const long long first = tile_begin(p, block), last = tile_begin(p, block + 1);
-    const bool samples = p.tiles_per_sample != p.tiles;  // otherwise no division
-    struct At {
-        long long sample, q;
-        bool here;
+    // a tile's sample and first position in it
+    struct Cursor {
+        long long sample, l;
+        __device__ __forceinline__ void next(const Problem& p, int rows) {
+            l += rows;
+            if (l >= p.length) {
+                l = 0;
+                ++sample;
+            }
+        }
     };
-    auto at_of = [&](long long tile) {
-        const long long sample = samples ? tile / p.tiles_per_sample : 0;
-        const long long l = (tile - sample * p.tiles_per_sample) * team.rows + team.row;
-        return At{sample, sample * p.length + l, l < p.length};
-    };
+    Cursor ahead = {first / p.tiles_per_sample, first % p.tiles_per_sample * team.rows};
+    auto position = [&](const Cursor& c) { return c.sample * p.length + c.l + team.row; };
+    auto here_at = [&](const Cursor& c) { return c.l + team.row < p.length; };
+    auto row_at = [&](const Cursor& c) { return slots.row(static_cast<size_t>(position(c)) * channels, here_at(c)); };
+    auto gate_at = [&](const Cursor& c) { return slots.row(static_cast<size_t>(c.sample) * channels, here_at(c)); };
     auto fetch = [&](long long tile, int ring) {
         if (tile < last) {
-            const At at = at_of(tile);
-            const size_t row = static_cast<size_t>(at.q) * channels;
+            const Row<NV> row = row_at(ahead);
+            const unsigned k = ring * kTensors;
             if (p.dn) {
-                F::fetch(slot(ring, kX), p.x, row, team, at.here);
-                F::fetch(slot(ring, kDn), p.dn, row, team, at.here);
+                slots.fetch(k + kX, p.x, row);
+                slots.fetch(k + kDn, p.dn, row);
             }
-            if (p.dr) F::fetch(slot(ring, kDr), p.dr, row, team, at.here);
-            if constexpr (MODE != kNoBlock) F::fetch(slot(ring, kY), p.y, row, team, at.here);
-            if constexpr (MODE == kFull)
-                F::fetch(slot(ring, kGate), p.gate,
-                         p.gate_mode == kGateSample ? static_cast<size_t>(at.sample) * channels : row, team, at.here);
+            if (p.dr) slots.fetch(k + kDr, p.dr, row);
+            if constexpr (MODE != kNoBlock) slots.fetch(k + kY, p.y, row);
+            if constexpr (MODE == kFull) slots.fetch(k + kGate, p.gate, p.gate_mode == kGateSample ? gate_at(ahead) : row);
+            ahead.next(p, team.rows);
         }
         copy_commit();
     };
+    // the forward's statistics, a tile ahead too; zeros where there is no position
+    auto saved = [&](const Cursor& c, bool exists) {
+        return exists && here_at(c) ? reinterpret_cast<const float4*>(p.stats)[position(c)] : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    Cursor now = ahead;
+    float4 stats = saved(now, first < last);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) fetch(first + k, k);
     const Weights<T, VEC, NV> weight_of(p, team, MODE != kNoBlock);
     float2 dw2[N], db2[N], tah[N], ta[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) dw2[i] = db2[i] = tah[i] = ta[i] = both(0.f);
-    bool on[NV];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) on[j] = team.has(j);
     int turn = 0, ring = 0;
     for (long long tile = first; tile < last; ++tile) {
-        const At at = at_of(tile);
-        const size_t row = static_cast<size_t>(at.q) * channels;
-        const size_t gate_row = p.gate_mode == kGateSample ? static_cast<size_t>(at.sample) * channels : row;
-        float2 rho = both(0.f), shift = both(0.f), rho2 = both(0.f), shift2 = both(0.f);
-        if (at.here) {
-            rho = both(1.f);
-            if (p.post) {
-                rho = both(p.stats[p.positions + at.q]);
-                shift = both(-p.stats[at.q] * rho.x);
-            }
-            if (p.dn) {
-                rho2 = both(p.stats[3 * p.positions + at.q]);
-                shift2 = both(-p.stats[2 * p.positions + at.q] * rho2.x);
-            }
-        }
+        const Row<NV> row = row_at(now);
+        const bool here = here_at(now);
+        const Row<NV> gate_row = p.gate_mode == kGateSample ? gate_at(now) : row;
+        const long long sample = now.sample;
+        const unsigned slot = ring * kTensors;
+        const float2 rho = both(!p.post && here ? 1.f : p.post ? stats.y : 0.f);
+        const float2 shift = both(p.post ? -stats.x * stats.y : 0.f);
+        const float2 rho2 = both(p.dn ? stats.w : 0.f), shift2 = both(p.dn ? -stats.z * stats.w : 0.f);
+        now.next(p, team.rows);
+        stats = saved(now, tile + 1 < last);
         fetch(tile + kAhead, ring == 0 ? kAhead : ring - 1);
         copy_wait<kAhead>();
         // s: the sigmoid of the gate, or its plain value; the gate itself is read again where silu needs
@@ -461,23 +501,23 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
 #pragma unroll
             for (int i = 0; i < N; ++i) a[i] = s[i];
             if (p.act == kActSilu) {
-                F::read(slot(ring, kGate), p.gate, gate_row, team, at.here, a);
+                slots.read(slot + kGate, p.gate, gate_row, a);
 #pragma unroll
                 for (int i = 0; i < N; ++i) a[i] = mul2(a[i], s[i]);
             }
         };
         if constexpr (MODE != kNoBlock) {
-            F::read(slot(ring, kY), p.y, row, team, at.here, h);
+            slots.read(slot + kY, p.y, row, h);
 #pragma unroll
             for (int i = 0; i < N; ++i) h[i] = fma2(h[i], rho, shift);
             if constexpr (MODE == kFull) {
-                F::read(slot(ring, kGate), p.gate, gate_row, team, at.here, s);
+                slots.read(slot + kGate, p.gate, gate_row, s);
                 if (p.act != kActNone) activate_all(s, kActSigmoid);
             }
         }
         if (p.dn) {
-            F::read(slot(ring, kX), p.x, row, team, at.here, k);
-            F::read(slot(ring, kDn), p.dn, row, team, at.here, g);  // zeros where there is no channel
+            slots.read(slot + kX, p.x, row, k);
+            slots.read(slot + kDn, p.dn, row, g);  // zeros where there is no channel
             float2 a[N];
             if constexpr (MODE == kFull) gate_of(a);
             float2 s0 = both(0.f), s1 = both(0.f);
@@ -504,13 +544,13 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
             for (int i = 0; i < N; ++i) g[i] = both(0.f);
         }
         if (p.dr) {
-            F::read(slot(ring, kDr), p.dr, row, team, at.here, k);
+            slots.read(slot + kDr, p.dr, row, k);
 #pragma unroll
             for (int i = 0; i < N; ++i) g[i] = add2(g[i], k[i]);
         }
         clear_dead<VEC, NV>(g, on);
         // g: the gradient of r
-        if (p.dx) F::store(p.dx, row, team, at.here, g);
+        if (p.dx) slots.store(p.dx, row, g);
         if constexpr (MODE != kNoBlock) {
             float2 s0 = both(0.f), s1 = both(0.f), a[N];
             if constexpr (MODE == kFull) {
@@ -524,7 +564,7 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
                                                  : p.act == kActSigmoid ? mul2(s[i], rest) : both(1.f);
                         o[i] = mul2(mul2(g[i], fma2(h[i], weight_of.w[i], weight_of.b[i])), o[i]);
                     }
-                    F::store(p.dgate, row, team, at.here, o);
+                    slots.store(p.dgate, row, o);
                 }
             }
 #pragma unroll
@@ -545,13 +585,13 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
 #pragma unroll
                     for (int i = 0; i < N; ++i) k[i] = mul2(rho, add2(fma2(h[i], m4, k[i]), m3));
                 }
-                F::store(p.dy, row, team, at.here, k);
+                slots.store(p.dy, row, k);
             }
-            if (p.slots && (tile + 1 == last || (tile + 1) % p.tiles_per_sample == 0)) {
+            if (p.slots && (tile + 1 == last || now.l == 0)) {
                 // this ring slot has been read, and its next copies are kAhead positions away: the sums
                 // of several rows meet in the space behind the ring
-                float* meet = reinterpret_cast<float*>(slots - threadIdx.x + (kAhead + 1) * kTensors * NV * blockDim.x);
-                float* to = slot_of(p, block, at.sample);
+                float* meet = reinterpret_cast<float*>(dynamic + kPartBytes + (kAhead + 1) * kTensors * NV * slots.pitch);
+                float* to = slot_of(p, block, sample);
                 store_sums<VEC, NV>(p, team, meet, tah, to);
                 store_sums<VEC, NV>(p, team, meet, ta, to + channels);
 #pragma unroll
@@ -562,7 +602,7 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
     }
     copy_wait<0>();
     if (!p.sums) return;
-    float* meet = reinterpret_cast<float*>(slots - threadIdx.x + (kAhead + 1) * kTensors * NV * blockDim.x);
+    float* meet = reinterpret_cast<float*>(dynamic + kPartBytes + (kAhead + 1) * kTensors * NV * slots.pitch);
     float* out = p.partial + static_cast<size_t>(block) * kSums * channels;
     store_sums<VEC, NV>(p, team, meet, dw2, out + static_cast<size_t>(kDPreW) * channels);
     store_sums<VEC, NV>(p, team, meet, db2, out + static_cast<size_t>(kDPreB) * channels);

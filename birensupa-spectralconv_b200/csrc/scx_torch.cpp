@@ -249,7 +249,7 @@ Forward run_forward(const scx_residual_norm_config& c, const variable_list& in, 
     Forward f;
     if (in[1].defined()) f.r = at::empty_like(x);
     if (c.pre_norm) f.n = at::empty_like(x);
-    if (keep_stats) f.stats = at::empty({4, c.batch * c.length}, x.options().dtype(at::kFloat));
+    if (keep_stats) f.stats = at::empty({c.batch * c.length, 4}, x.options().dtype(at::kFloat));
     scx_residual_norm_tensors t = tensors_of(in);
     t.r = out(f.r);
     t.n = out(f.n);

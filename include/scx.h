@@ -368,7 +368,7 @@ int scx_adam_step(int n_tensors, void* const* params, const void* const* grads,
  * weights and scale vector then are ones, biases zeros (at most 262144 channels); y NULL: r = x (t.r is not written), n =
  * pre(x).  post_norm 0: z = y; pre_norm 0: no n.  The scale vector multiplies config.scale.
  * Statistics and sums are fp32, and n is computed from the unrounded r.  stats (may be NULL in
- * the forward): [4][batch*length] floats for the backward.  Outputs must not overlap the inputs or
+ * the forward): 4*batch*length floats for the backward, 16-byte aligned, in an order of the kernels' own.  Outputs must not overlap the inputs or
  * one another. */
 #define SCX_NORM_RMS 0
 #define SCX_NORM_LAYER 1
