@@ -110,9 +110,34 @@ __device__ __forceinline__ float2 sum_groups(float2 v) {
     return v;
 }
 
-// Joins two numbers per position and warp: f(thread's share, shares per position, read) runs on a few
-// threads per position, read(w) being warp w's numbers, and its result comes back to every thread's
-// positions in a and b.  Every thread of the block calls it.
+// A few threads per position add the warps' parts: SHARES of them, each every SHARES-th warp.
+template <int SHARES>
+struct Share {
+    int me;
+
+    // f over this share's warps, whole steps at once where there are several shares
+    template <typename F>
+    __device__ __forceinline__ void for_warps(int warps, F f) const {
+        if constexpr (SHARES == 1) {
+#pragma unroll 4
+            for (int w = 0; w < warps; ++w) f(w);
+        } else {
+#pragma unroll
+            for (int k = 0; k < kMaxWarps / SHARES; ++k)
+                if (k * SHARES + me < warps) f(k * SHARES + me);
+        }
+    }
+    // the sum over the shares of a position, 8 lanes apart
+    __device__ __forceinline__ float sum(float v) const {
+#pragma unroll
+        for (int o = 8; o < 8 * SHARES; o *= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    }
+};
+
+// Joins two numbers per position and warp: f(share, position, whether it exists and is this thread's to
+// store, read) runs on a few threads per position, read(w) being warp w's numbers, and its result comes
+// back to every thread's positions in a and b.  Every thread of the block calls it.
 template <int V, int EPT, int LC, typename F>
 __device__ __forceinline__ void join(Shared<V, EPT, LC>& sh, const Where& at, float2 (&a)[Pairs<V, EPT>::kSpots],
                                      float2 (&b)[Pairs<V, EPT>::kSpots], F f) {
@@ -130,15 +155,16 @@ __device__ __forceinline__ void join(Shared<V, EPT, LC>& sh, const Where& at, fl
     __syncthreads();
     // whole warps take part or not: f shuffles
     const int lane = static_cast<int>(threadIdx.x % 32);
-    auto one = [&](int q, int share, int shares) {
-        const bool here = q < S::kPos;
-        const float2 r = f(share, shares, here ? q : 0, here && share == 0, [&](int w) { return sh.part[w][here ? q : 0]; });
-        if (here && share == 0) sh.stat[q] = r;
+    auto one = [&](int q, auto share) {
+        const bool here = q < S::kPos, store = here && share.me == 0;
+        const float2* column = &sh.part[0][here ? q : 0];
+        const float2 r = f(share, q, store, [&](int w) { return column[w * S::kPitch]; });
+        if (store) sh.stat[q] = r;
     };
     if (S::kPos >= 8 && static_cast<int>(blockDim.x) >= 4 * S::kPos) {  // a warp: 8 positions x 4 shares
-        if (at.warp < S::kPos / 8) one(at.warp * 8 + lane % 8, lane / 8, 4);
+        if (at.warp < S::kPos / 8) one(at.warp * 8 + lane % 8, Share<4>{lane / 8});
     } else {
-        for (int q0 = at.warp * 32; q0 < S::kPos; q0 += at.warps * 32) one(q0 + lane, 0, 1);
+        for (int q0 = at.warp * 32; q0 < S::kPos; q0 += at.warps * 32) one(q0 + lane, Share<1>{0});
     }
     __syncthreads();
     const float2* from = &sh.stat[at.pos * V];
@@ -153,15 +179,6 @@ __device__ __forceinline__ void join(Shared<V, EPT, LC>& sh, const Where& at, fl
             b[s] = make_float2(v.y, v.w);
         }
     }
-}
-
-// Sums over the four shares of a position.
-__device__ __forceinline__ float sum_shares(float v, int shares) {
-    if (shares == 4) {
-        v += __shfl_xor_sync(0xffffffffu, v, 8);
-        v += __shfl_xor_sync(0xffffffffu, v, 16);
-    }
-    return v;
 }
 
 // Rho = 1 / sqrt(variance + eps) and -mean rho over the channels of a thread's positions, so that the
@@ -201,22 +218,21 @@ __device__ __forceinline__ void statistics(Shared<V, EPT, LC>& sh, const Problem
     P::sum(d, rho);
 #pragma unroll
     for (int q = 0; q < P::kSpots; ++q) rho[q] = sum_groups<LC>(rho[q]);
-    join<V, EPT, LC>(sh, at, shift, rho, [&](int share, int shares, int q, bool store, auto part) {
+    join<V, EPT, LC>(sh, at, shift, rho, [&](auto share, int q, bool store, auto part) {
         float mean = 0.f, sum = 0.f;
         if (layer) {
-            for (int w = share; w < at.warps; w += shares)
-                mean = fmaf(static_cast<float>(min(kPerWarp, p.channels - w * kPerWarp)), part(w).x, mean);
-            mean = sum_shares(mean, shares) * p.inv_c;
-            for (int w = share; w < at.warps; w += shares) {
+            auto count = [&](int w) { return static_cast<float>(min(kPerWarp, p.channels - w * kPerWarp)); };
+            share.for_warps(at.warps, [&](int w) { mean = fmaf(count(w), part(w).x, mean); });
+            mean = share.sum(mean) * p.inv_c;
+            share.for_warps(at.warps, [&](int w) {
                 const float2 e = part(w);
                 const float off = e.x - mean;
-                sum += fmaf(static_cast<float>(min(kPerWarp, p.channels - w * kPerWarp)) * off, off, e.y);
-            }
+                sum += fmaf(count(w) * off, off, e.y);
+            });
         } else {
-#pragma unroll 4
-            for (int w = share; w < at.warps; w += shares) sum += part(w).y;
+            share.for_warps(at.warps, [&](int w) { sum += part(w).y; });
         }
-        const float r = rsqrtf(fmaf(sum_shares(sum, shares), p.inv_c, p.eps));
+        const float r = rsqrtf(fmaf(share.sum(sum), p.inv_c, p.eps));
         if (store && keep != nullptr && q < live_pos) {
             keep[q] = mean;
             keep[p.positions + q] = r;
@@ -236,11 +252,10 @@ __device__ __forceinline__ void two_means(Shared<V, EPT, LC>& sh, const Problem&
         if (layer) m1[q] = sum_groups<LC>(m1[q]);
         m2[q] = sum_groups<LC>(m2[q]);
     }
-    join<V, EPT, LC>(sh, at, m1, m2, [&](int share, int shares, int, bool, auto part) {
+    join<V, EPT, LC>(sh, at, m1, m2, [&](auto share, int, bool, auto part) {
         float2 s = both(0.f);
-#pragma unroll 4
-        for (int w = share; w < at.warps; w += shares) s = add2(s, part(w));
-        return make_float2(layer ? -sum_shares(s.x, shares) * p.inv_c : 0.f, -sum_shares(s.y, shares) * p.inv_c);
+        share.for_warps(at.warps, [&](int w) { s = add2(s, part(w)); });
+        return make_float2(layer ? -share.sum(s.x) * p.inv_c : 0.f, -share.sum(s.y) * p.inv_c);
     });
 }
 
