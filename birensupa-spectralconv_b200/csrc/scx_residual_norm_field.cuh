@@ -501,7 +501,12 @@ __global__ void __launch_bounds__(MAXW * 32, MAXW <= 10 ? 2 : 1) field_backward_
     const Where at = where<V, EPT, LC>(p);
     constexpr int kTensors = backward_tensors(MODE);
     const F slots(dynamic + sizeof(sh), p, at);
-    const int first = static_cast<int>(tile_begin(p, blockIdx.x)), last = static_cast<int>(tile_begin(p, blockIdx.x + 1));
+    // Tiles in a row across the blocks, so that what is under way at one time lies together in DRAM's pages
+    // (a training pass of 16x64x129x129 in fp32: 308 us, with a run of tiles per block 330).  With a gate per
+    // sample a run of tiles per block all the same: its sums are kept by sample.
+    const int first = MODE == kSample ? static_cast<int>(tile_begin(p, blockIdx.x)) : blockIdx.x;
+    const int last = static_cast<int>(MODE == kSample ? tile_begin(p, blockIdx.x + 1) : p.tiles);
+    const int stride = MODE == kSample ? 1 : gridDim.x;
     Saved<V> ahead;
     auto fetch = [&](const TILE& t, bool exists, int turn) {
         if (exists) {
@@ -519,6 +524,7 @@ __global__ void __launch_bounds__(MAXW * 32, MAXW <= 10 ? 2 : 1) field_backward_
         copy_commit();
     };
     TILE t(p, first);
+    const TILE step(p, stride);
     fetch(t, first < last, 0);
     load_vectors<T>(sh, p, at.warps * EPT * LC);
     int turn = 0;
@@ -532,7 +538,7 @@ __global__ void __launch_bounds__(MAXW * 32, MAXW <= 10 ? 2 : 1) field_backward_
     auto of_channel = [&](int kind, int j) {
         return V == 1 ? (j % 2 ? sum[kind][j / 2].y : sum[kind][j / 2].x) : sum[kind][j % kAcc].x + sum[kind][j % kAcc].y;
     };
-    for (int tile = first; tile < last; ++tile, turn ^= 1) {
+    for (int tile = first; tile < last; tile += stride, turn ^= 1) {
         const Spots<EPT> spots = slots.spots(t.base(p, at), t.live(p, at));
         const int sample = t.sample;
         const unsigned slot = turn * kTensors;
@@ -545,8 +551,8 @@ __global__ void __launch_bounds__(MAXW * 32, MAXW <= 10 ? 2 : 1) field_backward_
             shift[s] = make_float2(-ahead.mean[s].x * rho[s].x, -ahead.mean[s].y * rho[s].y);
             shift2[s] = make_float2(-ahead.mean2[s].x * rho2[s].x, -ahead.mean2[s].y * rho2[s].y);
         }
-        t.next(p, 0, 1);
-        fetch(t, tile + 1 < last, turn ^ 1);
+        t.next(p, MODE == kSample ? 0 : step.sample, MODE == kSample ? 1 : step.index);
+        fetch(t, tile + stride < last, turn ^ 1);
         copy_wait<1>();
         float2 h[N], a[N], slope[N], k[N], g[N];
         if constexpr (MODE != kNoBlock) {
