@@ -110,21 +110,24 @@ __device__ __forceinline__ float2 sum_groups(float2 v) {
     return v;
 }
 
-// A few threads per position add the warps' parts: SHARES of them, each every SHARES-th warp.
-template <int SHARES>
+// A few threads per position add the warps' parts: SHARES of them, each every SHARES-th warp.  WHOLE: the
+// code of all steps at once, which is quicker by itself (training passes: 7x36x96x160 with a gate per sample
+// 47 us against 49, 8x128x128x128 154 against 159).  With a gate per element in fp32, which HBM bounds, a loop:
+// shorter code of a tile keeps the blocks' accesses apart (16x64x256x256: 559 us against 606).
+template <int SHARES, bool WHOLE>
 struct Share {
     int me;
 
-    // f over this share's warps, whole steps at once where there are several shares
+    // f over this share's warps
     template <typename F>
     __device__ __forceinline__ void for_warps(int warps, F f) const {
-        if constexpr (SHARES == 1) {
-#pragma unroll 4
-            for (int w = 0; w < warps; ++w) f(w);
-        } else {
+        if constexpr (WHOLE && SHARES > 1) {
 #pragma unroll
             for (int k = 0; k < kMaxWarps / SHARES; ++k)
                 if (k * SHARES + me < warps) f(k * SHARES + me);
+        } else {
+#pragma unroll 1
+            for (int w = me; w < warps; w += SHARES) f(w);
         }
     }
     // the sum over the shares of a position, 8 lanes apart
@@ -138,7 +141,7 @@ struct Share {
 // Joins two numbers per position and warp: f(share, position, whether it exists and is this thread's to
 // store, read) runs on a few threads per position, read(w) being warp w's numbers, and its result comes
 // back to every thread's positions in a and b.  Every thread of the block calls it.
-template <int V, int EPT, int LC, typename F>
+template <bool WHOLE, int V, int EPT, int LC, typename F>
 __device__ __forceinline__ void join(Shared<V, EPT, LC>& sh, const Where& at, float2 (&a)[Pairs<V, EPT>::kSpots],
                                      float2 (&b)[Pairs<V, EPT>::kSpots], F f) {
     using S = Shape<V, EPT, LC>;
@@ -162,9 +165,9 @@ __device__ __forceinline__ void join(Shared<V, EPT, LC>& sh, const Where& at, fl
         if (store) sh.stat[q] = r;
     };
     if (S::kPos >= 8 && static_cast<int>(blockDim.x) >= 4 * S::kPos) {  // a warp: 8 positions x 4 shares
-        if (at.warp < S::kPos / 8) one(at.warp * 8 + lane % 8, Share<4>{lane / 8});
+        if (at.warp < S::kPos / 8) one(at.warp * 8 + lane % 8, Share<4, WHOLE>{lane / 8});
     } else {
-        for (int q0 = at.warp * 32; q0 < S::kPos; q0 += at.warps * 32) one(q0 + lane, Share<1>{0});
+        for (int q0 = at.warp * 32; q0 < S::kPos; q0 += at.warps * 32) one(q0 + lane, Share<1, WHOLE>{0});
     }
     __syncthreads();
     const float2* from = &sh.stat[at.pos * V];
@@ -183,7 +186,7 @@ __device__ __forceinline__ void join(Shared<V, EPT, LC>& sh, const Where& at, fl
 
 // Rho = 1 / sqrt(variance + eps) and -mean rho over the channels of a thread's positions, so that the
 // normalised value is v rho - mean rho; `keep` (may be null) receives mean and rho per position.
-template <int V, int EPT, int LC>
+template <bool WHOLE, int V, int EPT, int LC>
 __device__ __forceinline__ void statistics(Shared<V, EPT, LC>& sh, const Problem& p,
                                            const float2 (&v)[Pairs<V, EPT>::kCount], const Where& at,
                                            float2 (&rho)[Pairs<V, EPT>::kSpots], float2 (&shift)[Pairs<V, EPT>::kSpots],
@@ -218,7 +221,7 @@ __device__ __forceinline__ void statistics(Shared<V, EPT, LC>& sh, const Problem
     P::sum(d, rho);
 #pragma unroll
     for (int q = 0; q < P::kSpots; ++q) rho[q] = sum_groups<LC>(rho[q]);
-    join<V, EPT, LC>(sh, at, shift, rho, [&](auto share, int q, bool store, auto part) {
+    join<WHOLE, V, EPT, LC>(sh, at, shift, rho, [&](auto share, int q, bool store, auto part) {
         float mean = 0.f, sum = 0.f;
         if (layer) {
             auto count = [&](int w) { return static_cast<float>(min(kPerWarp, p.channels - w * kPerWarp)); };
@@ -243,7 +246,7 @@ __device__ __forceinline__ void statistics(Shared<V, EPT, LC>& sh, const Problem
 
 // The negatives of the means over the channels of two products, given as sums over the thread's
 // channels per position; the first is zero in the RMS kind.
-template <int V, int EPT, int LC>
+template <bool WHOLE, int V, int EPT, int LC>
 __device__ __forceinline__ void two_means(Shared<V, EPT, LC>& sh, const Problem& p, const Where& at,
                                           float2 (&m1)[Pairs<V, EPT>::kSpots], float2 (&m2)[Pairs<V, EPT>::kSpots]) {
     const bool layer = p.kind == kLayer;
@@ -252,12 +255,15 @@ __device__ __forceinline__ void two_means(Shared<V, EPT, LC>& sh, const Problem&
         if (layer) m1[q] = sum_groups<LC>(m1[q]);
         m2[q] = sum_groups<LC>(m2[q]);
     }
-    join<V, EPT, LC>(sh, at, m1, m2, [&](auto share, int, bool, auto part) {
+    join<WHOLE, V, EPT, LC>(sh, at, m1, m2, [&](auto share, int, bool, auto part) {
         float2 s = both(0.f);
         share.for_warps(at.warps, [&](int w) { s = add2(s, part(w)); });
         return make_float2(layer ? -share.sum(s.x) * p.inv_c : 0.f, -share.sum(s.y) * p.inv_c);
     });
 }
+
+template <typename T, int MODE>
+constexpr bool kWhole = sizeof(T) == 2 || MODE != kFull;
 
 // Where a tile lies, for one thread; moved on by `step` tiles without a division.
 template <int V, int EPT, int LC>
@@ -420,11 +426,11 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) field_forward_kernel(const 
             slots.read(slot + 1, p.y, spots, h);
             if constexpr (MODE == kFull) slots.read(slot + 2, p.gate, spots, a);
             if (p.post) {
-                statistics<V, EPT, LC>(sh, p, h, at, rho, shift, p.stats ? p.stats + q0 : nullptr, live_pos);
+                statistics<kWhole<T, MODE>, V, EPT, LC>(sh, p, h, at, rho, shift, p.stats ? p.stats + q0 : nullptr, live_pos);
 #pragma unroll
                 for (int i = 0; i < P::kCount; ++i) h[i] = fma2(h[i], rho[P::spot(i)], shift[P::spot(i)]);
             }
-            if constexpr (MODE == kFull) activate_all(a, p.act);
+            if constexpr (MODE == kFull) activate_all<T>(a, p.act);
             if constexpr (MODE == kSample) sample_gate<T, V, EPT>(p, at, sample, a);
 #pragma unroll
             for (int i = 0; i < P::kCount; ++i) {
@@ -434,7 +440,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) field_forward_kernel(const 
             slots.store(p.r, spots, r);
         }
         if (!p.pre) continue;
-        statistics<V, EPT, LC>(sh, p, r, at, rho, shift, p.stats ? p.stats + 2 * p.positions + q0 : nullptr, live_pos);
+        statistics<kWhole<T, MODE>, V, EPT, LC>(sh, p, r, at, rho, shift, p.stats ? p.stats + 2 * p.positions + q0 : nullptr, live_pos);
 #pragma unroll
         for (int i = 0; i < P::kCount; ++i)
             r[i] = fma2(fma2(r[i], rho[P::spot(i)], shift[P::spot(i)]), P::channels(&sh.vec[kPreW][at.c0], i),
@@ -459,9 +465,9 @@ struct Saved {
         // V divides the length, so V positions' numbers of one kind are one aligned access
         const size_t q = static_cast<size_t>(t.sample) * p.length + t.l0() + at.pos * V, row = static_cast<size_t>(p.positions);
         auto read = [&](size_t from, float2 (&to)[kSpots]) {
-            const Vec<float, V> v = load_vec<float, V>(p.stats, from);
+            const float* v = p.stats + from;
 #pragma unroll
-            for (int s = 0; s < kSpots; ++s) to[s] = V == 1 ? both(v.w[0]) : make_float2(v.w[2 * s % V], v.w[(2 * s + 1) % V]);
+            for (int s = 0; s < kSpots; ++s) to[s] = V == 1 ? both(v[0]) : make_float2(v[2 * s % V], v[(2 * s + 1) % V]);
         };
 #pragma unroll
         for (int s = 0; s < kSpots; ++s) rho[s] = both(1.f);
@@ -561,7 +567,7 @@ __global__ void __launch_bounds__(MAXW * 32, MAXW <= 10 ? 2 : 1) field_backward_
             for (int i = 0; i < N; ++i) h[i] = fma2(h[i], rho[P::spot(i)], shift[P::spot(i)]);
             if constexpr (MODE == kFull) {
                 slots.read(slot + 4, p.gate, spots, a);
-                activate_all(a, slope, p.act);
+                activate_all<T>(a, slope, p.act);
             }
             if constexpr (MODE == kSample) sample_gate<T, V, EPT>(p, at, sample, a);
         }
@@ -584,7 +590,7 @@ __global__ void __launch_bounds__(MAXW * 32, MAXW <= 10 ? 2 : 1) field_backward_
             }
             P::sum(g, m1);
             P::sum(gk, m2);
-            two_means<V, EPT, LC>(sh, p, at, m1, m2);
+            two_means<kWhole<T, MODE>, V, EPT, LC>(sh, p, at, m1, m2);
 #pragma unroll
             for (int i = 0; i < N; ++i)
                 g[i] = mul2(rho2[P::spot(i)], add2(fma2(k[i], m2[P::spot(i)], g[i]), m1[P::spot(i)]));
@@ -622,7 +628,7 @@ __global__ void __launch_bounds__(MAXW * 32, MAXW <= 10 ? 2 : 1) field_backward_
                     float2 m1[kSpots], m2[kSpots];
                     P::sum(k, m1);
                     P::sum(kh, m2);
-                    two_means<V, EPT, LC>(sh, p, at, m1, m2);
+                    two_means<kWhole<T, MODE>, V, EPT, LC>(sh, p, at, m1, m2);
 #pragma unroll
                     for (int i = 0; i < N; ++i)
                         k[i] = mul2(rho[P::spot(i)], add2(fma2(h[i], m2[P::spot(i)], k[i]), m1[P::spot(i)]));

@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kMaxThreads) token_forward_kernel(const __grid
             slots.read(slot + 1, p.y, row, h);
             if constexpr (MODE == kFull) {
                 slots.read(slot + 2, p.gate, kCopied<typename F::E> ? row : gate_row(q, here), a);
-                activate_all(a, p.act);
+                activate_all<T>(a, p.act);
             }
             if (p.post) st = statistics<VEC, NV>(p, team, h, on, turn);
             const float2 rho = both(st.y), shift = both(-st.x * st.y);
@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
             for (int i = 0; i < N; ++i) h[i] = fma2(h[i], rho, shift);
             if constexpr (MODE == kFull) {
                 slots.read(slot + kGate, p.gate, gate_row, s);
-                if (p.act != kActNone) activate_all(s, kActSigmoid);
+                if (p.act != kActNone) activate_all<T>(s, kActSigmoid);
             }
         }
         if (p.dn) {
