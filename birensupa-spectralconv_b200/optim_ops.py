@@ -112,6 +112,9 @@ class FusedAdam(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
                                       decoupled_weight_decay=decoupled_weight_decay))
 
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_norm": self.max_norm, "last_norm": self.last_norm}
+
     def __setstate__(self, state):
         super().__setstate__(state)
         for group in self.param_groups:

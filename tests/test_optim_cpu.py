@@ -3,7 +3,9 @@ Python layer, and the host-side logic that needs no device."""
 
 from __future__ import annotations
 
+import copy
 import ctypes
+import pickle
 
 import pytest
 import torch
@@ -138,3 +140,11 @@ def test_state_dict_of_torch_adam_loads_and_keeps_float32_moments():
     state["param_groups"][0]["amsgrad"] = True
     with pytest.raises(RuntimeError, match="amsgrad"):
         ours.load_state_dict(state)
+
+
+def test_a_copied_or_pickled_optimizer_still_clips():
+    ours = optim_ops.FusedAdam([torch.nn.Parameter(torch.zeros(3))], lr=1e-3, max_norm=0.5, decoupled_weight_decay=True)
+    for other in (copy.deepcopy(ours), pickle.loads(pickle.dumps(ours))):
+        assert other.max_norm == 0.5 and other.last_norm is None
+        assert other.param_groups[0]["decoupled_weight_decay"] is True
+        other.step()  # no gradients: nothing to do, and nothing missing
