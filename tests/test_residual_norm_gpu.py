@@ -132,6 +132,32 @@ def test_the_sigmoid_over_its_range(cuda_device):
         assert torch.equal(torch.isnan(r)[~finite], torch.isnan(want)[~finite])
 
 
+@pytest.mark.parametrize("dim", [1, -1])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_the_sigmoid_of_every_two_byte_gate(dtype, dim, cuda_device):
+    """All 65536 gates, as above.  The exponent t = -g log2(e) of a two-byte gate is rounded once and log2(e) is
+    off by 0.22 roundings: 1.25 |g| roundings of exp(-g), of which exp(-g) / (1 + exp(-g)) reaches the sigmoid; r
+    is rounded once to the type, half a step of the value or of the numbers below the normal ones."""
+    bits = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16)
+    g = bits.view(dtype).view(16, 64, 64).to(cuda_device)
+    half = torch.finfo(dtype).eps / 2
+    for act in ("sigmoid", "silu"):
+        r, _ = residual_norm(torch.zeros_like(g), torch.ones_like(g), gate=g, gate_activation=act, post_norm=False,
+                             pre_norm=False, dim=dim)
+        wide = g.double()
+        s = torch.special.expit(wide)
+        want = s if act == "sigmoid" else wide * s
+        finite = torch.isfinite(want)
+        small = torch.where(s < 1.2e-38, want.abs(), 0 * s)
+        near = want.abs() * (1 + (11 + 1.25 * (-wide).clamp(0, 1e39)) * 2.0**-24)  # no 0 * inf
+        bound = near - want.abs() + near * half + torch.finfo(dtype).tiny * half + small
+        assert ((r.double() - want).abs() <= bound)[finite].all()
+        # infinities and NaN as they are: silu of -inf is -inf times 0
+        assert torch.equal(r[~finite].isnan(), want[~finite].isnan())
+        assert torch.equal(r.isinf(), want.isinf())
+
+
+
 @pytest.mark.parametrize("shape, dim", [((3, 19, 40), -1), ((2, 32, 8, 12), 1), ((1, 2, 3000), -1)], ids=str)
 @pytest.mark.parametrize("option", ["no_vectors", "narrow", "number", "no_post", "no_pre", "no_y", "only_dr", "only_dn",
                                     "frozen_vectors", "frozen_y", "frozen_x", "sample_frozen", "weights_only"])
