@@ -686,12 +686,13 @@ cudaError_t forward_in(const Problem& p, cudaStream_t s) {
     constexpr int VEC = 16 / static_cast<int>(sizeof(T));
     if (vectors_fit<T>(p)) {
         if (p.channels <= VEC * kMaxThreads) return forward_as<T, VEC, 1, 1, MODE>(p, s);
-        if (p.channels <= 2 * VEC * kMaxThreads) return forward_as<T, VEC, 1, 2, MODE>(p, s);
-        if (p.channels <= 4 * VEC * kMaxThreads) return forward_as<T, VEC, 1, 4, MODE>(p, s);
+        if (p.channels <= 2 * VEC * kMaxThreads) return forward_as<T, VEC, 2, 1, MODE>(p, s);
+        if (p.channels <= 4 * VEC * kMaxThreads) return forward_as<T, VEC, 2, 2, MODE>(p, s);
         return cudaErrorNotSupported;
     }
     if (p.channels <= 4 * kMaxThreads) return forward_as<T, 1, 4, 1, MODE>(p, s);
-    if (p.channels <= 16 * kMaxThreads) return forward_as<T, 1, 4, 4, MODE>(p, s);
+    if (p.channels <= 8 * kMaxThreads) return forward_as<T, 1, 8, 1, MODE>(p, s);
+    if (p.channels <= 16 * kMaxThreads) return forward_as<T, 1, 8, 2, MODE>(p, s);
     return cudaErrorNotSupported;
 }
 
