@@ -5,9 +5,9 @@
 // their weights, and in the backward their sums, in registers.  Statistics are sums over a
 // position's threads, by shuffles within a warp and through shared memory across warps.
 //
-// What a thread keeps bounds a block to 512 threads and 16 bytes of each tensor per thread.  Longer
-// positions (over 4096 channels of 2 bytes) are cut over a cluster of CL = 2 or 4 blocks, which
-// exchange their parts of each sum through distributed shared memory.
+// What a thread keeps bounds a block to 512 threads and 8 or 16 channels per thread.  Longer
+// positions are cut over a cluster of CL = 2 or 4 blocks, which exchange their parts of each sum through
+// distributed shared memory.
 #pragma once
 
 #include <algorithm>
@@ -406,7 +406,7 @@ __device__ void store_sums(const Problem& p, const TEAM& team, float* shared, co
         }
         return;
     }
-    constexpr int kPer = VEC < 4 ? VEC : 4;  // VEC >= 4 divides the channels, so `out` starts on 16 bytes
+    constexpr int kPer = VEC < 4 ? VEC : 4;  // VEC divides the channels, so `out` starts on a vector
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int c = team.channel(j);
@@ -421,11 +421,15 @@ __device__ void store_sums(const Problem& p, const TEAM& team, float* shared, co
     }
 }
 
+// As kAhead: five tensors of 32 bytes per thread leave shared memory for one position.
+template <int BYTES>
+constexpr int kBackwardAhead = BYTES > 16 ? 1 : kAhead;
+
 template <typename T, int VEC, int NV, int CL, int MODE>
 __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __grid_constant__ Problem p, int tpr,
                                                                      int columns) {
     using F = Slots<T, VEC, NV>;
-    constexpr int N = NV * VEC / 2, kTensors = backward_tensors(MODE);
+    constexpr int N = NV * VEC / 2, kTensors = backward_tensors(MODE), kDeep = kBackwardAhead<NV * sizeof(Vec<T, VEC>)>;
     // the tensors' places in a ring slot
     constexpr int kX = 0, kDn = 1, kDr = 2, kY = 3, kGate = 4;
     extern __shared__ __align__(16) unsigned char dynamic[];
@@ -475,7 +479,7 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
     Cursor now = ahead;
     float4 stats = saved(now, first < last);
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) fetch(first + k, k);
+    for (int k = 0; k < kDeep; ++k) fetch(first + k, k);
     const Weights<T, VEC, NV> weight_of(p, team, MODE != kNoBlock);
     float2 dw2[N], db2[N], tah[N], ta[N];
 #pragma unroll
@@ -492,8 +496,8 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
         const float2 rho2 = both(p.dn ? stats.w : 0.f), shift2 = both(p.dn ? -stats.z * stats.w : 0.f);
         now.next(p, team.rows);
         stats = saved(now, tile + 1 < last);
-        fetch(tile + kAhead, ring == 0 ? kAhead : ring - 1);
-        copy_wait<kAhead>();
+        fetch(tile + kDeep, ring == 0 ? kDeep : ring - 1);
+        copy_wait<kDeep>();
         // s: the sigmoid of the gate, or its plain value; the gate itself is read again where silu needs
         // it, since registers are what this kernel is short of
         float2 h[N], s[N], k[N], g[N];
@@ -588,9 +592,9 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
                 slots.store(p.dy, row, k);
             }
             if (p.slots && (tile + 1 == last || now.l == 0)) {
-                // this ring slot has been read, and its next copies are kAhead positions away: the sums
+                // this ring slot has been read, and its next copies are kDeep positions away: the sums
                 // of several rows meet in the space behind the ring
-                float* meet = reinterpret_cast<float*>(dynamic + kPartBytes + (kAhead + 1) * kTensors * NV * slots.pitch);
+                float* meet = reinterpret_cast<float*>(dynamic + kPartBytes + (kDeep + 1) * kTensors * NV * slots.pitch);
                 float* to = slot_of(p, block, sample);
                 store_sums<VEC, NV>(p, team, meet, tah, to);
                 store_sums<VEC, NV>(p, team, meet, ta, to + channels);
@@ -598,11 +602,11 @@ __global__ void __launch_bounds__(kMaxThreads) token_backward_kernel(const __gri
                 for (int i = 0; i < N; ++i) tah[i] = ta[i] = both(0.f);
             }
         }
-        ring = ring == kAhead ? 0 : ring + 1;
+        ring = ring == kDeep ? 0 : ring + 1;
     }
     copy_wait<0>();
     if (!p.sums) return;
-    float* meet = reinterpret_cast<float*>(dynamic + kPartBytes + (kAhead + 1) * kTensors * NV * slots.pitch);
+    float* meet = reinterpret_cast<float*>(dynamic + kPartBytes + (kDeep + 1) * kTensors * NV * slots.pitch);
     float* out = p.partial + static_cast<size_t>(block) * kSums * channels;
     store_sums<VEC, NV>(p, team, meet, dw2, out + static_cast<size_t>(kDPreW) * channels);
     store_sums<VEC, NV>(p, team, meet, db2, out + static_cast<size_t>(kDPreB) * channels);
@@ -657,7 +661,8 @@ cudaError_t forward_as(const Problem& p, cudaStream_t s) {
 template <typename T, int VEC, int NV, int CL, int MODE>
 cudaError_t backward_as(Problem& p, cudaStream_t s) {
     const Lay lay(p.channels, VEC, NV, CL);
-    const size_t smem = kPartBytes + (kAhead + 1) * backward_tensors(MODE) * NV * sizeof(Vec<T, VEC>) * lay.threads +
+    constexpr int kDeep = kBackwardAhead<NV * sizeof(Vec<T, VEC>)>;
+    const size_t smem = kPartBytes + (kDeep + 1) * backward_tensors(MODE) * NV * sizeof(Vec<T, VEC>) * lay.threads +
                         (lay.rows > 1 ? sizeof(float) * lay.threads * VEC * NV : 0);
     const void* kernel = reinterpret_cast<const void*>(token_backward_kernel<T, VEC, NV, CL, MODE>);
     int per_sm = 0;
@@ -671,25 +676,38 @@ cudaError_t backward_as(Problem& p, cudaStream_t s) {
     return launch<CL>(kernel, p.parts, lay.threads, smem, s, p, lay);
 }
 
-// Whether rows can be moved by 16-byte accesses: whole vectors per row, every base aligned.
-template <typename T>
+// Whether rows can be moved by vectors of VEC: whole ones per row, every base aligned, the weights for reads of
+// VEC fp32 values (of four, where VEC is larger).
+template <typename T, int VEC>
 bool vectors_fit(const Problem& p) {
-    const void* all[] = {p.x, p.y, p.gate_mode != kGateNone ? p.gate : nullptr, p.r, p.n, p.dr, p.dn, p.dx, p.dy,
-                         p.gate_mode == kGateFull ? p.dgate : nullptr, p.post_w, p.post_b, p.pre_w, p.pre_b, p.scale_w};
-    for (const void* a : all)
-        if (!aligned(a, 16)) return false;
-    return p.channels % (16 / static_cast<int>(sizeof(T))) == 0;
+    const void* rows[] = {p.x, p.y, p.gate_mode != kGateNone ? p.gate : nullptr, p.r, p.n, p.dr, p.dn, p.dx, p.dy,
+                          p.gate_mode == kGateFull ? p.dgate : nullptr};
+    const void* weights[] = {p.post_w, p.post_b, p.pre_w, p.pre_b, p.scale_w};
+    for (const void* a : rows)
+        if (!aligned(a, VEC * sizeof(T))) return false;
+    for (const void* a : weights)
+        if (!aligned(a, std::min<size_t>(VEC, 4) * sizeof(float))) return false;
+    return p.channels % VEC == 0;
 }
 
+// More per thread comes before a cluster: a position's sums within a block cost half of what a cluster's
+// exchange does (4096 tokens of 8192 bf16 channels: forward 48 us, over two blocks 91).  What the forward keeps
+// of 16 values fits its registers; the backward's sums and weights leave room for 8 with a gate, and for 16
+// without one (training pass of the same tokens 195 us, over two blocks 217; with a gate 304 and 265).
 template <typename T, int MODE>
 cudaError_t forward_in(const Problem& p, cudaStream_t s) {
     constexpr int VEC = 16 / static_cast<int>(sizeof(T));
-    if (vectors_fit<T>(p)) {
+    if (vectors_fit<T, VEC>(p)) {
         if (p.channels <= VEC * kMaxThreads) return forward_as<T, VEC, 1, 1, MODE>(p, s);
         if (p.channels <= 2 * VEC * kMaxThreads) return forward_as<T, VEC, 2, 1, MODE>(p, s);
         if (p.channels <= 4 * VEC * kMaxThreads) return forward_as<T, VEC, 2, 2, MODE>(p, s);
         return cudaErrorNotSupported;
     }
+    if constexpr (sizeof(T) == 2)
+        if (vectors_fit<T, 2>(p)) {
+            if (p.channels <= 8 * kMaxThreads) return forward_as<T, 2, 4, 1, MODE>(p, s);
+            if (p.channels <= 16 * kMaxThreads) return forward_as<T, 2, 4, 2, MODE>(p, s);
+        }
     if (p.channels <= 4 * kMaxThreads) return forward_as<T, 1, 4, 1, MODE>(p, s);
     if (p.channels <= 8 * kMaxThreads) return forward_as<T, 1, 8, 1, MODE>(p, s);
     if (p.channels <= 16 * kMaxThreads) return forward_as<T, 1, 8, 2, MODE>(p, s);
@@ -699,14 +717,28 @@ cudaError_t forward_in(const Problem& p, cudaStream_t s) {
 template <typename T, int MODE>
 cudaError_t backward_in(Problem& p, cudaStream_t s) {
     constexpr int VEC = 16 / static_cast<int>(sizeof(T));
-    if (vectors_fit<T>(p)) {
+    if (vectors_fit<T, VEC>(p)) {
         if (p.channels <= VEC * kMaxThreads) return backward_as<T, VEC, 1, 1, MODE>(p, s);
-        if (p.channels <= 2 * VEC * kMaxThreads) return backward_as<T, VEC, 1, 2, MODE>(p, s);
-        if (p.channels <= 4 * VEC * kMaxThreads) return backward_as<T, VEC, 1, 4, MODE>(p, s);
+        if constexpr (VEC == 4) {
+            if (p.channels <= 8 * kMaxThreads) return backward_as<T, VEC, 2, 1, MODE>(p, s);
+            if (p.channels <= 16 * kMaxThreads) return backward_as<T, VEC, 2, 2, MODE>(p, s);
+        } else {
+            if (p.channels <= 16 * kMaxThreads) {
+                if constexpr (MODE == kFull) return backward_as<T, VEC, 1, 2, MODE>(p, s);
+                else return backward_as<T, VEC, 2, 1, MODE>(p, s);
+            }
+            if (p.channels <= 32 * kMaxThreads) return backward_as<T, VEC, 1, 4, MODE>(p, s);
+        }
         return cudaErrorNotSupported;
     }
+    if constexpr (sizeof(T) == 2)
+        if (vectors_fit<T, 2>(p)) {
+            if (p.channels <= 8 * kMaxThreads) return backward_as<T, 2, 4, 1, MODE>(p, s);
+            if (p.channels <= 16 * kMaxThreads) return backward_as<T, 2, 4, 2, MODE>(p, s);
+        }
     if (p.channels <= 4 * kMaxThreads) return backward_as<T, 1, 4, 1, MODE>(p, s);
-    if (p.channels <= 16 * kMaxThreads) return backward_as<T, 1, 4, 4, MODE>(p, s);
+    if (p.channels <= 8 * kMaxThreads) return backward_as<T, 1, 8, 1, MODE>(p, s);
+    if (p.channels <= 16 * kMaxThreads) return backward_as<T, 1, 8, 2, MODE>(p, s);
     return cudaErrorNotSupported;
 }
 

@@ -86,7 +86,8 @@ def _run(t, dim, dr, dn, *, kind="rms", act="none", eps=1e-5, number=None, post=
 
 
 TOKENS = [(1, 1), (1, 1, 8), (2, 3, 7), (5, 33), (3, 17, 100), (1, 2, 4096), (2, 2, 5001), (4, 9, 1025), (7, 40, 64),
-          (1, 3, 16384), (1, 1, 20000), (33, 2, 48), (2, 700, 16), (3, 5, 8192), (2, 3, 2, 36), (2, 600, 4104), (1, 2, 12000), (2, 3, 2050), (1, 5, 7001)]
+          (1, 3, 16384), (1, 1, 20000), (33, 2, 48), (2, 700, 16), (3, 5, 8192), (2, 3, 2, 36), (2, 600, 4104), (1, 2, 12000), (2, 3, 2050), (1, 5, 7001),
+          (2, 350, 2100), (2, 350, 3001), (1, 500, 6004), (1, 500, 2304), (2, 300, 1002)]
 FIELDS = [(2, 4, 1, 1), (1, 5, 3, 5), (3, 32, 8, 16), (2, 36, 9, 7), (2, 200, 5, 13), (1, 64, 32, 32), (2, 32, 70),
           (4, 1, 31), (1, 513, 40), (2, 20, 12, 12, 4), (20, 32, 4), (1, 32, 64, 64), (3, 24, 100, 7), (2, 1100, 33), (1, 96, 36), (3, 40, 5, 8), (2, 300, 64), (1, 75, 41), (1, 130, 9)]
 SHAPES = [(s, -1) for s in TOKENS] + [(s, 1) for s in FIELDS]
@@ -233,6 +234,31 @@ def test_layouts_strides_and_offsets(cuda_device):
         out = residual_norm(t["x"], t["y"], gate=t["gate"], dim=dim, pre_weight=t["pre_weight"])
         (g,) = torch.autograd.grad(out, t["x"], (ones, ones))
         torch.testing.assert_close(leaf.grad, g, rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("weight_offset", [1, 2, 4])
+@pytest.mark.parametrize("offset", [1, 2, 6])
+@pytest.mark.parametrize("channels", [40, 1002])
+def test_two_byte_tokens_off_the_vector_alignment(channels, offset, weight_offset, cuda_device):
+    """Inputs, gradients and fp32 weights that start some elements into their buffers."""
+    t, dr, dn = _inputs((2, 33, channels), -1, torch.bfloat16, cuda_device, gate="full", seed=11)
+
+    def moved(v, by):
+        room = torch.empty(v.numel() + by, dtype=v.dtype, device=v.device)[by:].view(v.shape)
+        return room.copy_(v)
+
+    t = {k: moved(v, weight_offset if k in VECTORS else offset) for k, v in t.items()}
+    dr, dn = moved(dr, offset), moved(dn, offset)
+    leaves = {k: v.detach().requires_grad_(True) for k, v in t.items()}
+    assert all(v.data_ptr() == t[k].data_ptr() for k, v in leaves.items())
+    r, n = residual_norm(leaves["x"], leaves["y"], gate=leaves["gate"], gate_activation="silu", kind="layer", dim=-1,
+                         **{k: leaves[k] for k in VECTORS})
+    want = _expected(t, -1, dr, dn, kind="layer", act="silu", eps=1e-5, number=1.0, post=True, pre=True)
+    _compare("r", r, want["r"], t, -1)
+    _compare("n", n, want["n"], t, -1)
+    grads = torch.autograd.grad((r, n), list(leaves.values()), (dr, dn))
+    for k, got in zip(leaves, grads):
+        _compare("d_" + k, got, want["d_" + k], t, -1)
 
 
 def test_a_second_derivative_is_refused(cuda_device):
