@@ -726,12 +726,15 @@ cudaError_t forward_in(const Problem& p, cudaStream_t s) {
     if (vectors_fit<T, 4>(p)) {
         if (p.channels <= 64) return forward_as<T, 4, 2, 2, MODE>(p, s);
         if (p.channels <= 128) return forward_as<T, 4, 2, 4, MODE>(p, s);
+        if (p.channels <= 256) return forward_as<T, 4, 2, 8, MODE>(p, s);
         if (p.channels <= 512) return forward_as<T, 4, 2, 16, MODE>(p, s);
+        if (p.channels <= 1024) return forward_as<T, 4, 2, 32, MODE>(p, s);
         return cudaErrorNotSupported;
     }
     if (p.channels <= 128) return forward_as<T, 1, 8, 1, MODE>(p, s);
     if (p.channels <= 256) return forward_as<T, 1, 8, 2, MODE>(p, s);
     if (p.channels <= 512) return forward_as<T, 1, 8, 4, MODE>(p, s);
+    if (p.channels <= 1024) return forward_as<T, 1, 8, 8, MODE>(p, s);
     return cudaErrorNotSupported;
 }
 
@@ -742,13 +745,16 @@ cudaError_t backward_in(Problem& p, cudaStream_t s) {
         if (p.channels <= 40) return backward_as<T, 4, 2, 2, MODE, 10>(p, s);
         if (p.channels <= 64) return backward_as<T, 4, 2, 2, MODE>(p, s);
         if (p.channels <= 128) return backward_as<T, 4, 2, 4, MODE>(p, s);
+        if (p.channels <= 256) return backward_as<T, 4, 2, 8, MODE>(p, s);
         if (p.channels <= 512) return backward_as<T, 4, 2, 16, MODE>(p, s);
+        if (p.channels <= 1024) return backward_as<T, 4, 2, 32, MODE>(p, s);
         return cudaErrorNotSupported;
     }
     if (p.channels <= 64) return backward_as<T, 1, 8, 1, MODE, 8>(p, s);
     if (p.channels <= 128) return backward_as<T, 1, 8, 1, MODE>(p, s);
     if (p.channels <= 256) return backward_as<T, 1, 8, 2, MODE>(p, s);
     if (p.channels <= 512) return backward_as<T, 1, 8, 4, MODE>(p, s);
+    if (p.channels <= 1024) return backward_as<T, 1, 8, 8, MODE>(p, s);
     return cudaErrorNotSupported;
 }
 

@@ -89,7 +89,8 @@ TOKENS = [(1, 1), (1, 1, 8), (2, 3, 7), (5, 33), (3, 17, 100), (1, 2, 4096), (2,
           (1, 3, 16384), (1, 1, 20000), (33, 2, 48), (2, 700, 16), (3, 5, 8192), (2, 3, 2, 36), (2, 600, 4104), (1, 2, 12000), (2, 3, 2050), (1, 5, 7001),
           (2, 350, 2100), (2, 350, 3001), (1, 500, 6004), (1, 500, 2304), (2, 300, 1002)]
 FIELDS = [(2, 4, 1, 1), (1, 5, 3, 5), (3, 32, 8, 16), (2, 36, 9, 7), (2, 200, 5, 13), (1, 64, 32, 32), (2, 32, 70),
-          (4, 1, 31), (1, 513, 40), (2, 20, 12, 12, 4), (20, 32, 4), (1, 32, 64, 64), (3, 24, 100, 7), (2, 1100, 33), (1, 96, 36), (3, 40, 5, 8), (2, 300, 64), (1, 75, 41), (1, 130, 9)]
+          (4, 1, 31), (1, 513, 40), (2, 20, 12, 12, 4), (20, 32, 4), (1, 32, 64, 64), (3, 24, 100, 7), (2, 1100, 33), (1, 96, 36), (3, 40, 5, 8), (2, 300, 64), (1, 75, 41), (1, 130, 9),
+          (2, 256, 20, 20), (2, 768, 16, 20), (2, 1024, 300), (2, 700, 15, 17), (1, 1023, 333)]
 SHAPES = [(s, -1) for s in TOKENS] + [(s, 1) for s in FIELDS]
 GATES = [("none", "none"), ("sample", "sigmoid"), ("full", "silu")]
 
