@@ -721,15 +721,20 @@ bool vectors_fit(const Problem& p) {
     return p.length % V == 0;
 }
 
+// The more channels, the fewer positions a tile has: as many as 16 warps of 8 values per thread leave.  Two-byte
+// fields of more than 256 channels, whose vectors of 4 would be half a sector or less, go by single positions
+// and more channels per thread (2x768x128x128 bf16 training pass 664 us, by vectors 871; 512 channels 600 and
+// 653; 256 channels 507 and 462).
 template <typename T, int MODE>
 cudaError_t forward_in(const Problem& p, cudaStream_t s) {
     if (vectors_fit<T, 4>(p)) {
         if (p.channels <= 64) return forward_as<T, 4, 2, 2, MODE>(p, s);
         if (p.channels <= 128) return forward_as<T, 4, 2, 4, MODE>(p, s);
         if (p.channels <= 256) return forward_as<T, 4, 2, 8, MODE>(p, s);
-        if (p.channels <= 512) return forward_as<T, 4, 2, 16, MODE>(p, s);
-        if (p.channels <= 1024) return forward_as<T, 4, 2, 32, MODE>(p, s);
-        return cudaErrorNotSupported;
+        if constexpr (sizeof(T) == 4) {
+            if (p.channels <= 512) return forward_as<T, 4, 2, 16, MODE>(p, s);
+            if (p.channels <= 1024) return forward_as<T, 4, 2, 32, MODE>(p, s);
+        }
     }
     if (p.channels <= 128) return forward_as<T, 1, 8, 1, MODE>(p, s);
     if (p.channels <= 256) return forward_as<T, 1, 8, 2, MODE>(p, s);
@@ -746,9 +751,10 @@ cudaError_t backward_in(Problem& p, cudaStream_t s) {
         if (p.channels <= 64) return backward_as<T, 4, 2, 2, MODE>(p, s);
         if (p.channels <= 128) return backward_as<T, 4, 2, 4, MODE>(p, s);
         if (p.channels <= 256) return backward_as<T, 4, 2, 8, MODE>(p, s);
-        if (p.channels <= 512) return backward_as<T, 4, 2, 16, MODE>(p, s);
-        if (p.channels <= 1024) return backward_as<T, 4, 2, 32, MODE>(p, s);
-        return cudaErrorNotSupported;
+        if constexpr (sizeof(T) == 4) {
+            if (p.channels <= 512) return backward_as<T, 4, 2, 16, MODE>(p, s);
+            if (p.channels <= 1024) return backward_as<T, 4, 2, 32, MODE>(p, s);
+        }
     }
     if (p.channels <= 64) return backward_as<T, 1, 8, 1, MODE, 8>(p, s);
     if (p.channels <= 128) return backward_as<T, 1, 8, 1, MODE>(p, s);
