@@ -16,7 +16,7 @@
 // and backward: a thread per column of channels (no barriers, but two columns in registers leave 8
 // warps per SM: 284 us and 2.1 ms); every thread adding all warps' parts itself (one barrier instead
 // of two, but shared memory saturates: 452 and 558 us); 8-byte accesses, V = 2 and EPT = 4
-// (296 and 526 us).
+// (296 and 526 us).  This one: 245 and 313 us, 0.96 of the measured HBM rate over both.
 #pragma once
 
 #include <algorithm>

@@ -19,7 +19,7 @@ __device__ __forceinline__ void from_f32(__half& o, float v) { o = __float2half_
 
 // V values of type T.  Two-byte types are held as words of two, whose halves are the upper and lower bits
 // of two fp32 values (bf16) or convert together (fp16): arrays of the types themselves move as 16-bit
-// pieces (8192 x 2048 bf16 tokens with a gate, forward and backward: 139 us against 129 us).
+// pieces (a step from 139 to 129 us on 8192 x 2048 bf16 tokens with a gate, forward and backward).
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
     static constexpr bool kWordsOfTwo = sizeof(T) == 2 && V >= 2;

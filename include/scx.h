@@ -363,13 +363,13 @@ int scx_adam_step(int n_tensors, void* const* params, const void* const* grads,
  *   z = post(y),  r = x + scale act(gate) z,  n = pre(r)
  *   post, pre: (v - mean) / sqrt(mean((v - mean)^2) + eps) * weight + bias; kind RMS: mean = 0
  * Layouts: x, y, r, n (and a gate per element) are [batch][length][channels] (channels_last 1) or
- * [batch][channels][length] (0); a gate per sample is [batch][channels]; weights, biases and the
- * scale vector are [channels], of type weight_dtype (SCX_FLOAT32 or dtype).  Each may be NULL:
- * weights and scale vector then are ones, biases zeros (at most 262144 channels); y NULL: r = x (t.r is not written), n =
- * pre(x).  post_norm 0: z = y; pre_norm 0: no n.  The scale vector multiplies config.scale.
- * Statistics and sums are fp32, and n is computed from the unrounded r.  stats (may be NULL in
- * the forward): 4*batch*length floats for the backward, 16-byte aligned, in an order of the kernels' own.  Outputs must not overlap the inputs or
- * one another. */
+ * [batch][channels][length] (0), of at most 262144 channels; a gate per sample is
+ * [batch][channels]; weights, biases and the scale vector are [channels], of type weight_dtype
+ * (SCX_FLOAT32 or dtype).  Each may be NULL: weights and scale vector then are ones, biases zeros;
+ * y NULL: r = x (t.r is not written), n = pre(x).  post_norm 0: z = y; pre_norm 0: no n.  The scale
+ * vector multiplies config.scale.  Statistics and sums are fp32, and n is computed from the unrounded
+ * r.  stats (may be NULL in the forward): 4*batch*length floats for the backward, 16-byte aligned, in
+ * an order of the kernels' own.  Outputs must not overlap the inputs or one another. */
 #define SCX_NORM_RMS 0
 #define SCX_NORM_LAYER 1
 #define SCX_GATE_NONE 0
@@ -395,9 +395,9 @@ typedef struct {
 int scx_residual_norm_fwd(const scx_residual_norm_config* config, const scx_residual_norm_tensors* t,
                           scx_stream_t stream);
 /* Backward, from the forward's inputs and stats (t.r and t.n are not read); gradients of what the
- * forward did not have (y, a gate, a norm) are refused.  workspace: device
- * memory of scx_residual_norm_bwd_workspace_size() bytes, 16-byte aligned, in use until the
- * call's kernels end; 0 on an invalid or empty configuration, for which the call is refused. */
+ * forward did not have (y, a gate, a norm) are refused.  workspace: device memory of
+ * scx_residual_norm_bwd_workspace_size() bytes, 16-byte aligned, in use until the call's kernels end;
+ * 0 on an invalid or empty configuration, for which the call is refused. */
 size_t scx_residual_norm_bwd_workspace_size(const scx_residual_norm_config* config);
 int scx_residual_norm_bwd(const scx_residual_norm_config* config, const scx_residual_norm_tensors* t,
                           const scx_residual_norm_grads* g, void* workspace, size_t workspace_bytes,
