@@ -160,7 +160,8 @@ def test_the_sigmoid_of_every_two_byte_gate(dtype, dim, cuda_device):
 
 
 
-@pytest.mark.parametrize("shape, dim", [((3, 19, 40), -1), ((2, 32, 8, 12), 1), ((1, 2, 3000), -1)], ids=str)
+@pytest.mark.parametrize("shape, dim", [((3, 19, 40), -1), ((2, 32, 8, 12), 1), ((1, 2, 3000), -1), ((1, 9, 6000), -1),
+                                        ((1, 9, 5002), -1), ((2, 700, 12), 1)], ids=str)
 @pytest.mark.parametrize("option", ["no_vectors", "narrow", "number", "no_post", "no_pre", "no_y", "only_dr", "only_dn",
                                     "frozen_vectors", "frozen_y", "frozen_x", "sample_frozen", "weights_only"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
