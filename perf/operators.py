@@ -20,20 +20,14 @@ LR, BETA1, BETA2, ADAM_EPS, WEIGHT_DECAY = 2.0e-4, 0.9, 0.999, 1.0e-8, 1.0e-4
 NORM_EPS = 1.0e-5
 
 
-_modules = []
-
-
 def _package():
-    """The package's modules, imported once as a user's program does."""
-    if not _modules:
-        path = str(Path(__file__).resolve().parents[1] / "birensupa-spectralconv_b200")
-        if path not in sys.path:
-            sys.path.insert(0, path)
-        import optim_ops
-        import residual_norm_ops
+    path = str(Path(__file__).resolve().parents[1] / "birensupa-spectralconv_b200")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import optim_ops
+    import residual_norm_ops
 
-        _modules.extend((optim_ops, residual_norm_ops))
-    return _modules
+    return optim_ops, residual_norm_ops
 
 
 # --------------------------------------------------------------------------- cases
