@@ -49,6 +49,11 @@ int code_of(at::ScalarType t) {
     }
 }
 
+// Forward-mode derivatives do not pass through the kernels, and a tangent left out reads as zero.
+void check_no_tangent(const Tensor& t, const char* name) {
+    TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), name, " must not carry a tangent: there is no forward-mode derivative");
+}
+
 at::Device check_tensors(const Tensors& tensors, const char* name) {
     const at::Device device = tensors[0].device();
     for (const Tensor& t : tensors) {
@@ -57,6 +62,7 @@ at::Device check_tensors(const Tensors& tensors, const char* name) {
         TORCH_CHECK(code_of(t.scalar_type()) >= 0, name, " must be float32, bfloat16, float16 or complex64, got ",
                     t.scalar_type());
         TORCH_CHECK(t.device() == device, name, " must be on one device");
+        check_no_tangent(t, name);
     }
     return device;
 }
@@ -176,6 +182,10 @@ std::optional<Tensor> adam_step(const Tensors& params, const Tensors& given_grad
         TORCH_CHECK(t.scalar_type() == at::kFloat && t.numel() == 1, "steps must be single float32 values");
         TORCH_CHECK(g.device() == device && m.device() == device && v.device() == device && t.device() == device,
                     "gradients, moments and steps must be on the params' device");
+        check_no_tangent(g, "gradients");
+        check_no_tangent(m, "moments");
+        check_no_tangent(v, "moments");
+        check_no_tangent(t, "steps");
         TORCH_CHECK(!p.is_conj() && !m.is_conj() && !v.is_conj(), "params and moments must not be conjugate views");
         TORCH_CHECK(!p.is_neg() && !m.is_neg() && !v.is_neg(), "params and moments must not be negated views");
         TORCH_CHECK(dense(p) && same_layout(m, p) && same_layout(v, p),
@@ -351,6 +361,7 @@ std::pair<MaybeTensor, MaybeTensor> residual_norm(const Options& options, double
     bool wanted = false;
     for (Tensor& t : in) {
         if (!t.defined()) continue;
+        check_no_tangent(t, "inputs of residual_norm");
         t = t.contiguous();
         wanted = wanted || t.requires_grad();
     }

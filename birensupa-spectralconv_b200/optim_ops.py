@@ -5,8 +5,8 @@ The reference trains with ``torch.optim.Adam`` and does not clip (fno_ns/train_o
 these are what ``fno_train`` uses where a run asks for clipping or the fused step.  Gradients may be
 float32, bfloat16, float16 or complex64 (a spectral weight's, taken as its real and imaginary
 parts), in any mix and of any size.  Calls run on the current stream of the tensors' device,
-synchronise nothing and can be captured in a CUDA graph; results are bitwise repeatable.  A failed
-check raises RuntimeError.
+synchronise nothing and can be captured in a CUDA graph; results are bitwise repeatable.  Tensors with a
+forward-mode tangent are refused.  A failed check raises RuntimeError.
 """
 
 from __future__ import annotations

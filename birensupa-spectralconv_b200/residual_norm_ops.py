@@ -32,7 +32,8 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *, pre_weight:
                   post_bias: torch.Tensor | None = None, gate: torch.Tensor | None = None,
                   gate_activation: str = "none", scale: torch.Tensor | float | None = None, kind: str = "rms",
                   eps: float = 1e-5, dim: int = 1, post_norm: bool = True, pre_norm: bool = True):
-    """(r, n) of the formulas above; differentiable in every tensor.
+    """(r, n) of the formulas above; differentiable once in every tensor, in reverse mode (a tensor with a
+    forward-mode tangent is refused).
 
     x       the residual stream, a float32, bfloat16 or float16 CUDA tensor with its channels on
             ``dim`` (1, or -1 for the last)

@@ -20,6 +20,7 @@ import random
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 import optim_ops
 
@@ -474,3 +475,20 @@ def test_only_empty_tensors(cuda_device):
     steps = [torch.zeros((), device=cuda_device) for _ in empty]
     got = optim_ops.adam_step_(empty, empty, empty, empty, steps, lr=1.0, max_norm=1.0)
     assert float(got) == 0.0 and [float(s) for s in steps] == [1.0, 1.0]
+
+
+def test_forward_derivatives_are_refused(cuda_device):
+    t, one = torch.ones(5, device=cuda_device), torch.ones(5, device=cuda_device)
+    with fwAD.dual_level():
+        dual = fwAD.make_dual(t, one)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            optim_ops.grad_norm([one, dual])
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            optim_ops.clip_grads_([dual], 1.0)
+        step = torch.zeros((), device=cuda_device)
+        for k in range(4):
+            lists = [[torch.ones(5, device=cuda_device)] for _ in range(4)]
+            lists[k] = [dual]
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                optim_ops.adam_step_(*lists, [step], lr=1.0)
+    assert torch.equal(t, one)

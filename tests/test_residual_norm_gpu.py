@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from residual_norm_ops import residual_norm
 from residual_norm_reference import like, reference, rows_of, within
@@ -416,3 +417,18 @@ def test_offsets_past_32_bits(dim, shape, cuda_device):
     for a, b in zip(got[0][:4], got[1][:4]):
         assert torch.equal(torch.stack(ends(a.detach())), b.detach())
     torch.testing.assert_close(got[0][4], got[1][4], rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("leaf", [False, True])
+def test_a_forward_derivative_is_refused(leaf, cuda_device):
+    """A tangent that the kernels cannot carry must not be read as zero, in whatever input it comes and
+    whether gradients are recorded or not."""
+    t, _, _ = _inputs((3, 5, 8), -1, torch.float32, cuda_device, gate="full")
+    with fwAD.dual_level():
+        for k, v in t.items():
+            dual = {**t, k: fwAD.make_dual(v.clone().requires_grad_(leaf), torch.ones_like(v))}
+            x, y = dual.pop("x"), dual.pop("y")
+            for mode in (True, False):
+                with torch.set_grad_enabled(mode), pytest.raises(RuntimeError, match="forward-mode"):
+                    residual_norm(x, y, dim=-1, gate_activation="sigmoid", **dual)
+    residual_norm(t.pop("x"), t.pop("y"), dim=-1, **t)
