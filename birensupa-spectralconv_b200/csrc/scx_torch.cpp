@@ -110,9 +110,9 @@ struct Described {
     }
 };
 
-Tensor grad_norm(const Tensors& tensors) {
-    const at::Device device = check_tensors(tensors, "tensors");
-    Tensors flat = tensors;
+Tensor run_norm(at::TensorList tensors) {
+    const at::Device device = tensors[0].device();
+    Tensors flat = tensors.vec();
     for (Tensor& t : flat)
         if (!dense(t)) t = t.contiguous();
     const c10::cuda::CUDAGuard guard(device);
@@ -124,6 +124,41 @@ Tensor grad_norm(const Tensors& tensors) {
                                static_cast<float*>(norm.data_ptr()), ws.data_ptr(), bytes, stream_of(device)),
                  "scx_grad_norm");
     return norm;
+}
+
+// dN/dg = g / N (zero where N is), in torch operations, so that it can be differentiated again.  A norm that is
+// differentiated is part of a loss (a penalty on gradients), not of the training step that the kernels are for.
+struct GradNorm : torch::autograd::Function<GradNorm> {
+    static Tensor forward(AutogradContext* ctx, at::TensorList tensors) {
+        const Tensor norm = run_norm(tensors);
+        variable_list saved = tensors.vec();
+        saved.push_back(norm);
+        ctx->save_for_backward(std::move(saved));
+        return norm;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list saved = ctx->get_saved_variables();
+        const Tensor norm = saved.back();
+        saved.pop_back();
+        variable_list result(saved.size());
+        if (!grads[0].defined()) return result;
+        const Tensor factor = grads[0] / norm.masked_fill(norm == 0, 1.0);
+        for (size_t i = 0; i < saved.size(); ++i) {
+            if (!ctx->needs_input_grad(i)) continue;
+            const at::ScalarType type = saved[i].scalar_type();
+            const bool narrow = type == at::kBFloat16 || type == at::kHalf;  // rounded once, behind the product
+            result[i] = narrow ? (saved[i].to(at::kFloat) * factor).to(type) : saved[i] * factor;
+        }
+        return result;
+    }
+};
+
+Tensor grad_norm(const Tensors& tensors) {
+    check_tensors(tensors, "tensors");
+    bool wanted = false;
+    for (const Tensor& t : tensors) wanted = wanted || t.requires_grad();
+    return wanted && at::GradMode::is_enabled() ? GradNorm::apply(at::TensorList(tensors)) : run_norm(tensors);
 }
 
 Tensor clip_grads(const Tensors& grads, double max_norm) {

@@ -30,8 +30,9 @@ def _number(value, name: str) -> float:
 
 def grad_norm(tensors) -> torch.Tensor:
     """The 2-norm over all elements of all ``tensors`` (an iterable of CUDA tensors, or one), as a
-    0-d float32 tensor on their device.  The sum is held in 64 bits.  Without tensors: 0 on the
-    CPU, as torch.nn.utils.get_total_norm gives."""
+    0-d float32 tensor on their device.  The sum is held in 64 bits.  Differentiable, any number of
+    times (the gradient of zeros is zero).  Without tensors: 0 on the CPU, as
+    torch.nn.utils.get_total_norm gives."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not tensors:
         return torch.tensor(0.0)
@@ -40,9 +41,9 @@ def grad_norm(tensors) -> torch.Tensor:
 
 def clip_grads_(grads, max_norm: float) -> torch.Tensor:
     """Multiplies every tensor of ``grads`` in place by min(1, max_norm / (norm + 1e-6)), norm
-    their global 2-norm before clipping, which is returned (0-d float32 on their device).  A norm
-    that is not finite propagates as in torch.nn.utils.clip_grad_norm_.  No two tensors may share
-    memory."""
+    their global 2-norm before clipping, which is returned (0-d float32 on their device, detached).
+    A norm that is not finite propagates as in torch.nn.utils.clip_grad_norm_.  No two tensors may
+    share memory."""
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     max_norm = _number(max_norm, "max_norm")
     if not grads:

@@ -492,3 +492,54 @@ def test_forward_derivatives_are_refused(cuda_device):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 optim_ops.adam_step_(*lists, [step], lr=1.0)
     assert torch.equal(t, one)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16, torch.complex64])
+def test_the_norm_is_differentiable(dtype, cuda_device):
+    """dN/dg = g / N, per component of complex values: N is off by 1.01 u, and the quotient, the product and
+    the rounding to the type add one each."""
+    g = _gen(cuda_device, 10)
+    kinds = [(300, 7), (1,), (0,), (4096 + 3,)]
+    grads = [_randn(s, dtype, cuda_device, g).requires_grad_(k != 1) for k, s in enumerate(kinds)]
+    grads.append(_randn((6, 8), torch.float32, cuda_device, g).requires_grad_(True))
+    views = [*grads[:-1], grads[-1].t()[::2]]  # one that is not dense
+    total = optim_ops.grad_norm(views)
+    _check_norm(total, views)
+    wrt = [t for t in grads if t.requires_grad]
+    got = torch.autograd.grad(total, wrt, torch.full_like(total, -1.5))
+    n = _norm64(views)
+    for t, d in zip(wrt, got):
+        assert d.dtype == t.dtype
+        value = _f64(t)
+        if t is grads[-1]:
+            value[:, 1::2] = 0.0
+        want = -1.5 * value / n
+        bound = (4 * U32 + _u(t.dtype)) * want.abs() + torch.finfo(d.dtype).tiny
+        assert bool(((_f64(d) - want).abs() <= bound).all())
+    with torch.no_grad():
+        assert not optim_ops.grad_norm(views).requires_grad
+    zero = torch.zeros(5, device=cuda_device, requires_grad=True)
+    (d,) = torch.autograd.grad(optim_ops.grad_norm([zero]), zero)
+    assert torch.equal(d, torch.zeros_like(d))
+
+
+def test_a_penalty_on_the_gradient_norm(cuda_device):
+    """f = sum w^3 / 3 has the gradient w^2, N = |w^2| and dN/dw = 2 w^3 / N; then the second derivative of N
+    itself, v / N - g (g v) / N^3.  The first takes 4 roundings for w^2, at most 5 for N, 2 for their quotient and
+    5 more behind it: 24 u bounds them.  In the second the float32 sum g v adds chains of at most 40: 64 u of the
+    terms' magnitudes."""
+    g = _gen(cuda_device, 11)
+    w = _randn((1000,), torch.float32, cuda_device, g).requires_grad_(True)
+    (grad,) = torch.autograd.grad((w**3).sum() / 3, w, create_graph=True)
+    (got,) = torch.autograd.grad(optim_ops.grad_norm([grad]), w)
+    w64 = _f64(w)
+    want = 2 * w64**3 / w64.square().norm()
+    assert bool(((got.double() - want).abs() <= 24 * U32 * want.abs()).all())
+    v = _randn((1000,), torch.float32, cuda_device, g)
+    (first,) = torch.autograd.grad(optim_ops.grad_norm([w]), w, create_graph=True)
+    (second,) = torch.autograd.grad(first, w, v)
+    n, v64 = w64.norm(), v.double()
+    want = v64 / n - w64 * (w64 * v64).sum() / n**3
+    size = v64.abs() / n + w64.abs() * (w64 * v64).abs().sum() / n**3
+    assert bool(((second.double() - want).abs() <= 64 * U32 * size).all())
+
