@@ -543,3 +543,75 @@ def test_a_penalty_on_the_gradient_norm(cuda_device):
     size = v64.abs() / n + w64.abs() * (w64 * v64).abs().sum() / n**3
     assert bool(((second.double() - want).abs() <= 64 * U32 * size).all())
 
+
+
+LONG = [1, 4097, 2047, 4095, 8193, 2048, 12287, 4096, 2049, 8188, 8191, 3, 8192, 12288, 4100, 2052, 17_000_003, 8196, 0, 4099]
+
+
+def _long_list(dtype, dev, g, scale=1.0, square=False):
+    """Views with gaps between them of one buffer, each list's neighbours at other alignments: more than
+    16.8M float32 values, beside tensors around the counts that a block has in flight (1024 vectors of 4,
+    twice that, and 512)."""
+    wide = 2 if dtype == torch.complex64 else 1
+    sizes = [n if n < 1 << 20 else n // wide for n in LONG]
+    flat = torch.randn(wide * (sum(sizes) + len(sizes)), device=dev, generator=g) * scale
+    if square:
+        flat.square_()
+    buffer = torch.view_as_complex(flat.view(-1, 2)) if wide == 2 else flat
+    views, at = [], 0
+    for n in sizes:
+        views.append(buffer[at:at + n])
+        at += n + 1
+    return flat, views
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.complex64])
+def test_long_lists_norm(dtype, cuda_device):
+    """Ones in a run of the list at a time, zeros elsewhere: a vector that is lost or taken twice changes the
+    norm by more than 2^-19 of it."""
+    flat, views = _long_list(dtype, cuda_device, _gen(cuda_device, 12))
+    _check_norm(optim_ops.grad_norm(views), views)
+    edges = list(range(0, flat.numel(), 1_000_003)) + [flat.numel()]
+    for a, b in zip(edges, edges[1:]):
+        flat.zero_()
+        flat[a:b] = 1.0
+        _check_norm(optim_ops.grad_norm(views), views)
+    flat.fill_(math.nan)  # the gaps are not read
+    for v in views:
+        v.fill_(0.0)
+    assert float(optim_ops.grad_norm(views)) == 0.0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.complex64])
+def test_long_lists_clip(dtype, cuda_device):
+    flat, views = _long_list(dtype, cuda_device, _gen(cuda_device, 13))
+    before, rest = [_f64(v) for v in views], flat.clone()
+    limit = 0.37 * _norm64(views)
+    got = optim_ops.clip_grads_(views, limit)
+    assert abs(float(got) - limit / 0.37) <= 1.01 * U32 * float(got)
+    _check_clipped(views, before, limit)
+    for v in views:
+        v.zero_()
+    kept = flat != 0
+    assert int(kept.sum()) >= 15 and torch.equal(flat[kept], rest[kept])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.complex64])
+@pytest.mark.parametrize("clip", [False, True])
+def test_long_lists_adam(clip, dtype, cuda_device):
+    g = _gen(cuda_device, 14)
+    flats, lists = zip(*(_long_list(dtype, cuda_device, g, s, k == 3) for k, s in enumerate((0.3, 1.0, 0.1, 0.1))))
+    params, grads, m, v = lists
+    before = [tuple(_f64(t) for t in ts) for ts in zip(params, grads, m, v)]
+    rest = [f.clone() for f in flats]
+    steps = [torch.full((), 6.0, device=cuda_device) for _ in params]
+    n = _norm64(grads)
+    hyper = dict(lr=3e-3, betas=(0.9, 0.999), eps=1e-8)
+    optim_ops.adam_step_(params, grads, m, v, steps, max_norm=0.3 * n if clip else None, **hyper)
+    assert torch.equal(flats[1], rest[1]) and all(float(s) == 7.0 for s in steps)
+    _check_adam(params, m, v, before, step=7, wd=0.0, decoupled=False, c=0.3 * n / (n + 1e-6) if clip else 1.0, **hyper)
+    for k in (0, 2, 3):
+        for t in lists[k]:
+            t.zero_()
+        kept = flats[k] != 0
+        assert int(kept.sum()) >= 15 and torch.equal(flats[k][kept], rest[k][kept])
