@@ -473,10 +473,11 @@ Problem problem_of(const scx_residual_norm_config& c, const scx_residual_norm_te
     p.x = t.x;
     p.y = t.y;
     p.gate = t.gate;
-    p.post_w = t.post_weight;
-    p.post_b = t.post_bias;
-    p.pre_w = t.pre_weight;
-    p.pre_b = t.pre_bias;
+    // weights of a norm that is not taken are not read by any kernel, nor by the last sums
+    p.post_w = p.post ? t.post_weight : nullptr;
+    p.post_b = p.post ? t.post_bias : nullptr;
+    p.pre_w = p.pre ? t.pre_weight : nullptr;
+    p.pre_b = p.pre ? t.pre_bias : nullptr;
     p.scale_w = t.scale;
     p.r = t.r;
     p.n = t.n;

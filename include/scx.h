@@ -366,8 +366,8 @@ int scx_adam_step(int n_tensors, void* const* params, const void* const* grads,
  * [batch][channels][length] (0), of at most 262144 channels; a gate per sample is
  * [batch][channels]; weights, biases and the scale vector are [channels], of type weight_dtype
  * (SCX_FLOAT32 or dtype).  Each may be NULL: weights and scale vector then are ones, biases zeros;
- * y NULL: r = x (t.r is not written), n = pre(x).  post_norm 0: z = y; pre_norm 0: no n.  The scale
- * vector multiplies config.scale.  Statistics and sums are fp32, and n is computed from the unrounded
+ * y NULL: r = x (t.r is not written), n = pre(x).  post_norm 0: z = y; pre_norm 0: no n; the weights
+ * and biases of a norm that is not taken are not read.  The scale vector multiplies config.scale.  Statistics and sums are fp32, and n is computed from the unrounded
  * r.  stats (may be NULL in the forward): 4*batch*length floats for the backward, 16-byte aligned, in
  * an order of the kernels' own.  Outputs must not overlap the inputs or one another. */
 #define SCX_NORM_RMS 0

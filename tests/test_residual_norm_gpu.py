@@ -3,10 +3,13 @@ has the bounds and how they are derived), forward and backward, in both layouts.
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 
+import _scx
 from residual_norm_ops import residual_norm
 from residual_norm_reference import like, reference, rows_of, within
 
@@ -432,3 +435,44 @@ def test_a_forward_derivative_is_refused(leaf, cuda_device):
                 with torch.set_grad_enabled(mode), pytest.raises(RuntimeError, match="forward-mode"):
                     residual_norm(x, y, dim=-1, gate_activation="sigmoid", **dual)
     residual_norm(t.pop("x"), t.pop("y"), dim=-1, **t)
+
+
+@pytest.mark.parametrize("shape, dim", [((2, 33, 40), -1), ((2, 40, 33), 1), ((2, 20000, 3), 1)], ids=str)
+@pytest.mark.parametrize("gate_mode", [0, 1, 2])
+def test_weights_of_a_norm_that_is_not_taken_are_not_used(gate_mode, shape, dim, cuda_device):
+    """At the C ABI weights and biases may be given with post_norm or pre_norm 0: outputs and gradients are
+    those of a call without them."""
+    C, length = (shape[1], shape[2]) if dim == 1 else (shape[2], shape[1])
+    t, dr, dn = _inputs(shape, dim, torch.float32, cuda_device, gate=["none", "sample", "full"][gate_mode], seed=13)
+    for post, pre in ((0, 1), (1, 0), (0, 0)):
+        config = _scx.ResidualNormConfig(batch=shape[0], length=length, channels=C, channels_last=int(dim == -1), gate_mode=gate_mode,
+                                         gate_act=1, post_norm=post, pre_norm=pre, eps=1e-5, scale=0.5)
+        nbytes = _scx.lib.scx_residual_norm_bwd_workspace_size(ctypes.byref(config))
+        got = []
+        for given in (True, False):
+            r, n, dx, dy = (torch.zeros_like(t["x"]) for _ in range(4))
+            stats = torch.zeros(4 * shape[0] * length, device=cuda_device)
+            dscale = torch.zeros(C, device=cuda_device)
+            dgate = torch.zeros_like(t["gate"]) if gate_mode else None
+            ws = torch.zeros(nbytes, dtype=torch.uint8, device=cuda_device)
+            keep = {k: t[k].data_ptr() for k in ("post_weight", "post_bias") if post or given}
+            keep |= {k: t[k].data_ptr() for k in ("pre_weight", "pre_bias") if pre or given}
+            tensors = _scx.ResidualNormTensors(x=t["x"].data_ptr(), y=t["y"].data_ptr(), scale=t["scale"].data_ptr(), r=r.data_ptr(),
+                                               n=n.data_ptr(), stats=stats.data_ptr(), **keep,
+                                               gate=t["gate"].data_ptr() if gate_mode else None)
+            grads = _scx.ResidualNormGrads(dr=dr.data_ptr(), dn=dn.data_ptr() if pre else None, dx=dx.data_ptr(),
+                                           dy=dy.data_ptr(), d_scale=dscale.data_ptr(),
+                                           dgate=dgate.data_ptr() if gate_mode else None)
+            stream = torch.cuda.current_stream().cuda_stream
+            assert _scx.lib.scx_residual_norm_fwd(ctypes.byref(config), ctypes.byref(tensors), stream) == 0
+            assert _scx.lib.scx_residual_norm_bwd(ctypes.byref(config), ctypes.byref(tensors), ctypes.byref(grads),
+                                                  ws.data_ptr(), nbytes, stream) == 0
+            torch.cuda.synchronize()
+            got.append([r, n, dx, dy, dscale] + ([dgate] if gate_mode else []))
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+        want = _expected({**t, **({} if post else {"post_weight": None, "post_bias": None})}, dim, dr, dn if pre else None,
+                         kind="rms", act="sigmoid", eps=1e-5, number=0.5, post=bool(post), pre=bool(pre))
+        _compare("r", got[0][0], want["r"], t, dim)
+        _compare("d_scale", got[0][4], want["d_scale"], t, dim)
+        if gate_mode:
+            _compare("d_gate", got[0][5], want["d_gate"], t, dim)
