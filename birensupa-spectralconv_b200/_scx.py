@@ -23,6 +23,18 @@ if not LIB_PATH.exists():
 
 lib = ctypes.CDLL(str(LIB_PATH))
 
+
+def torch_binding():
+    """The module _scx_torch (optimizer operators, residual norm), which `make lib` alone does not build."""
+    try:
+        import _scx_torch
+    except ModuleNotFoundError as e:
+        raise ImportError(f"{PKG_DIR / '_scx_torch.so'} is missing: build it with `make -C {PKG_DIR}` "
+                          "(or __graft_entry__.build())") from e
+    return _scx_torch
+
+
+
 _i = ctypes.c_int
 _p = ctypes.c_void_p
 _sz = ctypes.c_size_t

@@ -28,7 +28,6 @@ import torch.nn.functional as F
 
 import _scx
 import spectral_conv_ext
-from residual_norm_ops import residual_norm
 from spectral_conv_ops import spectral_conv2d_autograd, spectral_conv2d_supa
 
 
@@ -345,6 +344,8 @@ class ResidualFNO2d(nn.Module):
         return _conv1x1(self.project[2], F.gelu(_conv1x1(self.project[0], n)))
 
     def _run_device(self, x: torch.Tensor, spectral) -> torch.Tensor:
+        from residual_norm_ops import residual_norm  # here: FNO2d and the host path need libscx.so alone
+
         def join(h, y=None, gate=None, **more):
             return residual_norm(h, y, gate=gate, gate_activation="none" if gate is None else "sigmoid", **more)
 

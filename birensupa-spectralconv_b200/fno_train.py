@@ -36,7 +36,6 @@ if str(PKG_DIR) not in sys.path:
     sys.path.insert(0, str(PKG_DIR))
 
 import fno_model  # noqa: E402
-import optim_ops  # noqa: E402
 import scx_data  # noqa: E402
 
 
@@ -64,6 +63,8 @@ def train(model: fno_model.FNO2d | fno_model.ResidualFNO2d, x_train, y_train, x_
           fused_adam: bool = False, log=print) -> dict:
     """Trains ``model`` (on the data's device) and returns a summary with the per-epoch losses, and
     with ``max_grad_norm`` the gradient norm of each epoch's last step."""
+    if fused_adam or max_grad_norm is not None:
+        import optim_ops  # needs the torch binding, which the recipe itself does not
     device = x_train.device
     g = torch.Generator(device=device)
     g.manual_seed(seed)

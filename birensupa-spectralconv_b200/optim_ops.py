@@ -15,10 +15,10 @@ import math
 
 import torch
 
-import _scx  # noqa: F401  (loads libscx.so, with its message where that is missing)
-import _scx_torch
+import _scx
 from spectral_conv_ext import _check
 
+_scx_torch = _scx.torch_binding()
 _dense, _overlaps_itself = _scx_torch.dense, _scx_torch.overlaps_itself
 
 

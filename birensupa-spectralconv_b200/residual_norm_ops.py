@@ -18,10 +18,10 @@ import math
 
 import torch
 
-import _scx  # noqa: F401  (loads libscx.so, with its message where that is missing)
-import _scx_torch
+import _scx
 from spectral_conv_ext import _check
 
+_scx_torch = _scx.torch_binding()
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _KINDS = {"rms": 0, "layer": 1}
 _ACTIVATIONS = {"none": 0, "sigmoid": 1, "silu": 2}
