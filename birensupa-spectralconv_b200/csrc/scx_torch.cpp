@@ -284,6 +284,9 @@ scx_residual_norm_tensors tensors_of(const variable_list& in) {
             data(in[6]), data(in[7]), nullptr,     nullptr,     nullptr};
 }
 
+// t with its values in memory as they read: in one run, and not behind a negation bit (contiguous() leaves that).
+Tensor plain(const Tensor& t) { return t.resolve_neg().contiguous(); }
+
 struct Forward {
     Tensor r, n, stats;
 };
@@ -352,8 +355,8 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
                     result[kBefore + i] = x.numel() ? at::empty_like(saved[i]) : at::zeros_like(saved[i]);
             if (x.numel()) {
                 const c10::cuda::CUDAGuard guard(x.device());
-                if (dr.defined()) dr = dr.contiguous();
-                if (dn.defined()) dn = dn.contiguous();
+                if (dr.defined()) dr = plain(dr);
+                if (dn.defined()) dn = plain(dn);
                 const scx_residual_norm_config c =
                     config_of(ctx->saved_data["options"].toIntVector(), ctx->saved_data["eps"].toDouble(),
                               ctx->saved_data["scale"].toDouble());
@@ -397,7 +400,7 @@ std::pair<MaybeTensor, MaybeTensor> residual_norm(const Options& options, double
     for (Tensor& t : in) {
         if (!t.defined()) continue;
         check_no_tangent(t, "inputs of residual_norm");
-        t = t.contiguous();
+        t = plain(t);
         wanted = wanted || t.requires_grad();
     }
     if (wanted && at::GradMode::is_enabled()) {

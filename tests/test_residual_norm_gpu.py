@@ -476,3 +476,21 @@ def test_weights_of_a_norm_that_is_not_taken_are_not_used(gate_mode, shape, dim,
         _compare("d_scale", got[0][4], want["d_scale"], t, dim)
         if gate_mode:
             _compare("d_gate", got[0][5], want["d_gate"], t, dim)
+
+
+@pytest.mark.parametrize("shape, dim", [((3, 5, 8), -1), ((2, 32, 4, 4), 1), ((1, 1), -1)], ids=str)
+def test_negated_views(shape, dim, cuda_device):
+    """Tensors whose sign is a bit of the view (as the imaginary part of a conjugate has) and not of the
+    values in memory, among the inputs and the incoming gradients."""
+    t, dr, dn = _inputs(shape, dim, torch.float32, cuda_device, gate="full", seed=12)
+    flipped = {k: torch._neg_view(-v) for k, v in t.items()}
+    assert all(v.is_neg() and torch.equal(v, t[k]) for k, v in flipped.items())
+    got = []
+    for s, d, e in ((t, dr, dn), (flipped, torch._neg_view(-dr), torch._neg_view(-dn))):
+        leaves = {k: v.detach().requires_grad_(True) for k, v in s.items()}
+        outs = residual_norm(leaves["x"], leaves["y"], gate=leaves["gate"], gate_activation="sigmoid", dim=dim,
+                             **{k: leaves[k] for k in VECTORS})
+        got.append([*outs, *torch.autograd.grad(outs, list(leaves.values()), (d, e))])
+        with torch.no_grad():
+            got[-1] += residual_norm(s["x"], s["y"], dim=dim)
+    assert all(torch.equal(a, b) for a, b in zip(*got))
