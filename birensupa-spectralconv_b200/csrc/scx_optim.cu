@@ -297,11 +297,13 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ 
 __device__ __forceinline__ void adam_one(float& p, float g, float& m, float& v, float c, float2 k,
                                          const AdamScalars& s) {
     g *= c;
-    if (!s.decoupled) g = fmaf(s.weight_decay, p, g);
+    if (!s.decoupled && s.weight_decay != 0.f) g = fmaf(s.weight_decay, p, g);  // no 0 * inf from an infinite p
     m = fmaf(s.beta1, m, s.rest1 * g);
     v = fmaf(s.beta2, v, s.rest2 * g * g);
-    // the decay joins the update before p is rounded: lr * wd alone is often below half a step of p
-    p -= fmaf(s.shrink, p, k.x * m / fmaf(sqrtf(v), k.y, s.eps));
+    const float move = k.x * m / fmaf(sqrtf(v), k.y, s.eps);
+    // the decay joins the update before p is rounded: lr * wd alone is often below half a step of p.  An infinite p
+    // has no decay to take, and stays.
+    p -= isinf(p) ? move : fmaf(s.shrink, p, move);
 }
 
 template <int DEEP, typename T>

@@ -615,3 +615,31 @@ def test_long_lists_adam(clip, dtype, cuda_device):
             t.zero_()
         kept = flats[k] != 0
         assert int(kept.sum()) >= 15 and torch.equal(flats[k][kept], rest[k][kept])
+
+
+@pytest.mark.parametrize("decay, decoupled", [(0.0, False), (0.0, True), (0.01, True)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rate_on_device", [False, True])
+def test_infinite_parameters_stay_as_in_torch(rate_on_device, dtype, decay, decoupled, cuda_device):
+    """A parameter held at an infinity (a masked entry) keeps it, and its moments are those of its gradient.
+    The others agree to the roundings: in float32 3 updates of 0.125 by 24 u and 6 of p; in bfloat16 torch's moments
+    are rounded too, 3 updates by 2^-6 and 6 halves of a step 2^-7 of p."""
+    p = torch.linspace(-1.0, 1.0, 40, device=cuda_device).to(dtype)
+    p[3], p[20], p[38] = -math.inf, math.inf, -math.inf
+    grad = torch.randn(40, device=cuda_device, generator=_gen(cuda_device, 15)).to(dtype)
+    grad[20] = 0.0
+    ours, ref = torch.nn.Parameter(p.clone()), torch.nn.Parameter(p.clone())
+    ours.grad, ref.grad = grad.clone(), grad.clone()
+    lr = torch.full((), 0.125, device=cuda_device) if rate_on_device else 0.125
+    kind = torch.optim.AdamW if decoupled else torch.optim.Adam
+    opt = optim_ops.FusedAdam([ours], lr=lr, weight_decay=decay, decoupled_weight_decay=decoupled)
+    opt_ref = kind([ref], lr=0.125, weight_decay=decay)
+    for _ in range(3):
+        opt.step()
+        opt_ref.step()
+    for k in (3, 20, 38):
+        assert float(ours.detach()[k]) == float(ref.detach()[k]) == float(p[k])
+    assert bool(torch.isfinite(opt.state[ours]["exp_avg"]).all()) and bool(torch.isfinite(opt.state[ours]["exp_avg_sq"]).all())
+    rest = torch.isfinite(p)
+    torch.testing.assert_close(ours.detach()[rest], ref.detach()[rest], rtol=0.0,
+                               atol=1e-5 if dtype == torch.float32 else 0.05)
