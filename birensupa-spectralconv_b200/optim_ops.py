@@ -99,7 +99,7 @@ class FusedAdam(torch.optim.Optimizer):
     """Adam (AdamW with ``decoupled_weight_decay``) on ``adam_step_``: one call per parameter
     group, with ``max_norm`` clipping the gradients by the global norm over all groups on their
     way into the update (``p.grad`` is not changed).  ``last_norm`` is that norm, a 0-d tensor on
-    the device, after a step.
+    the device, after a step (without any gradient 0 on the CPU, as ``clip_grad_norm_`` gives).
 
     State and options carry torch.optim.Adam's names, so state dicts go both ways (``step`` on the
     device, as torch's ``fused`` and ``capturable`` forms keep it; moments are float32 for bfloat16
@@ -160,6 +160,8 @@ class FusedAdam(torch.optim.Optimizer):
             if params:
                 work.append((group, params))
         total = None
+        if not work:
+            self.last_norm = None if self.max_norm is None else torch.tensor(0.0)
         if self.max_norm is not None and len(work) > 1:
             total = grad_norm([p.grad for _, params in work for p in params])
         for group, params in work:

@@ -148,3 +148,10 @@ def test_a_copied_or_pickled_optimizer_still_clips():
         assert other.max_norm == 0.5 and other.last_norm is None
         assert other.param_groups[0]["decoupled_weight_decay"] is True
         other.step()  # no gradients: nothing to do, and nothing missing
+
+
+def test_a_step_without_gradients_leaves_no_old_norm():
+    ours = optim_ops.FusedAdam([torch.nn.Parameter(torch.zeros(3))], lr=1e-3, max_norm=0.5)
+    ours.last_norm = torch.tensor(7.0)
+    ours.step()
+    assert float(ours.last_norm) == 0.0

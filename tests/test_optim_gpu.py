@@ -643,3 +643,14 @@ def test_infinite_parameters_stay_as_in_torch(rate_on_device, dtype, decay, deco
     rest = torch.isfinite(p)
     torch.testing.assert_close(ours.detach()[rest], ref.detach()[rest], rtol=0.0,
                                atol=1e-5 if dtype == torch.float32 else 0.05)
+
+
+def test_the_last_norm_is_of_the_last_step(cuda_device):
+    p = torch.nn.Parameter(torch.ones(4, device=cuda_device))
+    opt = optim_ops.FusedAdam([p], lr=1e-2, max_norm=1.0)
+    p.grad = torch.full_like(p, 2.0)
+    opt.step()
+    assert float(opt.last_norm) == 4.0
+    opt.zero_grad()
+    opt.step()  # without a gradient: as clip_grad_norm_ gives then
+    assert float(opt.last_norm) == 0.0
