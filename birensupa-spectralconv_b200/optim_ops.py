@@ -104,7 +104,8 @@ class FusedAdam(torch.optim.Optimizer):
     State and options carry torch.optim.Adam's names, so state dicts go both ways (``step`` on the
     device, as torch's ``fused`` and ``capturable`` forms keep it; moments are float32 for bfloat16
     and float16 parameters, and stay so through load_state_dict).  ``lr`` may be a 0-d float32 CUDA
-    tensor, which a captured step reads at each replay."""
+    tensor, which a captured step reads at each replay.  A parameter's first step, which makes its
+    state, is refused in a capture."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0, *,
                  decoupled_weight_decay: bool = False, max_norm: float | None = None):
@@ -154,6 +155,9 @@ class FusedAdam(torch.optim.Optimizer):
             for p in params:
                 state = self.state[p]
                 if not state:
+                    _check(not torch.cuda.is_current_stream_capturing(),
+                           "a parameter's first step has to run before it is captured: its zero moments and count "
+                           "would be made again at every replay")
                     state["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
                     state["exp_avg"] = self._moment(p)
                     state["exp_avg_sq"] = self._moment(p)

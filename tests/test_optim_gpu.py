@@ -654,3 +654,23 @@ def test_the_last_norm_is_of_the_last_step(cuda_device):
     opt.zero_grad()
     opt.step()  # without a gradient: as clip_grad_norm_ gives then
     assert float(opt.last_norm) == 0.0
+
+
+def test_a_first_step_is_not_captured(cuda_device):
+    """Its zero moments and count would be made again at every replay."""
+    p = torch.nn.Parameter(torch.ones(4, device=cuda_device))
+    p.grad = torch.ones_like(p)
+    opt = optim_ops.FusedAdam([p], lr=0.5)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="before it is captured"):
+        with torch.cuda.graph(graph):
+            opt.step()
+    assert not opt.state[p] and bool((p.detach() == 1.0).all())
+    del graph
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    graph.replay()
+    graph.replay()
+    assert float(opt.state[p]["step"]) == 3.0
