@@ -155,7 +155,7 @@ class FusedAdam(torch.optim.Optimizer):
             for p in params:
                 state = self.state[p]
                 if not state:
-                    _check(not torch.cuda.is_current_stream_capturing(),
+                    _check(not (p.is_cuda and torch.cuda.is_current_stream_capturing()),
                            "a parameter's first step has to run before it is captured: its zero moments and count "
                            "would be made again at every replay")
                     state["step"] = torch.zeros((), dtype=torch.float32, device=p.device)

@@ -155,3 +155,10 @@ def test_a_step_without_gradients_leaves_no_old_norm():
     ours.last_norm = torch.tensor(7.0)
     ours.step()
     assert float(ours.last_norm) == 0.0
+
+
+def test_a_step_on_the_host_is_refused():
+    p = torch.nn.Parameter(torch.ones(2))
+    p.grad = torch.ones(2)
+    with pytest.raises(RuntimeError, match="params must be CUDA"):
+        optim_ops.FusedAdam([p]).step()
