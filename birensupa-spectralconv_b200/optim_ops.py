@@ -130,18 +130,28 @@ class FusedAdam(torch.optim.Optimizer):
         new = torch.zeros_like(p, dtype=kind, memory_format=torch.preserve_format, requires_grad=False)
         return new if value is None else new.copy_(value)
 
-    @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
-        super().load_state_dict(state_dict)
-        # the base class casts moments to their parameter's type: take them over from the source
+        # the base class casts moments to their parameter's type: they are taken over from the source, which is
+        # what the caller's hooks have made of it, before the caller's own hooks on the result
+        source = []
+        hooks = [self.register_load_state_dict_pre_hook(lambda _, given: source.append(given)),
+                 self.register_load_state_dict_post_hook(lambda _: self._keep_moments(source[-1]), prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    @torch.no_grad()
+    def _keep_moments(self, state_dict) -> None:
         ours = [p for g in self.param_groups for p in g["params"]]
         theirs = [i for g in state_dict["param_groups"] for i in g["params"]]
         for p, i in zip(ours, theirs):
             saved = state_dict["state"].get(i)
             if saved:
-                self.state[p] = {"step": torch.as_tensor(saved["step"]).to(p.device, torch.float32, copy=True),
-                                 "exp_avg": self._moment(p, saved["exp_avg"]),
-                                 "exp_avg_sq": self._moment(p, saved["exp_avg_sq"])}
+                self.state[p].update(step=torch.as_tensor(saved["step"]).to(p.device, torch.float32, copy=True),
+                                     exp_avg=self._moment(p, saved["exp_avg"]),
+                                     exp_avg_sq=self._moment(p, saved["exp_avg_sq"]))
 
     @torch.no_grad()
     def step(self, closure=None):

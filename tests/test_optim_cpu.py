@@ -162,3 +162,25 @@ def test_a_step_on_the_host_is_refused():
     p.grad = torch.ones(2)
     with pytest.raises(RuntimeError, match="params must be CUDA"):
         optim_ops.FusedAdam([p]).step()
+
+
+def test_load_state_dict_hooks_see_and_change_what_is_loaded():
+    p = torch.nn.Parameter(torch.zeros(3, dtype=torch.bfloat16))
+    ours = optim_ops.FusedAdam([p], lr=1e-3)
+    m = torch.full((3,), 1.0 + 2.0**-20)
+    groups = [{"lr": 5e-4, "betas": (0.8, 0.9), "eps": 1e-7, "weight_decay": 0.1, "params": [0]}]
+    state = {"state": {0: {"step": 7, "exp_avg": m, "exp_avg_sq": m * m, "note": 5}}, "param_groups": groups}
+    other = {"state": {0: {"step": 9, "exp_avg": 2 * m, "exp_avg_sq": m, "note": 5}}, "param_groups": groups}
+    seen = []
+    before = ours.register_load_state_dict_pre_hook(lambda opt, given: other)
+    after = ours.register_load_state_dict_post_hook(lambda opt: seen.append(opt.state[p]["exp_avg"].clone()))
+    ours.load_state_dict(state)
+    got = ours.state[p]
+    assert torch.equal(got["exp_avg"], 2 * m) and torch.equal(got["exp_avg_sq"], m) and float(got["step"]) == 9.0
+    assert got["note"] == 5 and got["exp_avg"].dtype == torch.float32
+    assert len(seen) == 1 and torch.equal(seen[0], 2 * m)
+    before.remove()
+    after.remove()
+    ours.load_state_dict(state)
+    assert torch.equal(ours.state[p]["exp_avg"], m) and len(seen) == 1
+    assert not ours._optimizer_load_state_dict_pre_hooks and not ours._optimizer_load_state_dict_post_hooks
