@@ -9,6 +9,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -54,7 +55,11 @@ void check_no_tangent(const Tensor& t, const char* name) {
     TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), name, " must not carry a tangent: there is no forward-mode derivative");
 }
 
+// A trace would record the outputs' allocation and not the kernels that fill them.
+void check_not_traced() { TORCH_CHECK(!torch::jit::tracer::isTracing(), "the call cannot be traced"); }
+
 at::Device check_tensors(const Tensors& tensors, const char* name) {
+    check_not_traced();
     const at::Device device = tensors[0].device();
     for (const Tensor& t : tensors) {
         TORCH_CHECK(t.is_cuda(), name, " must be CUDA tensors");
@@ -394,6 +399,7 @@ std::pair<MaybeTensor, MaybeTensor> residual_norm(const Options& options, double
                                                   const MaybeTensor& post_w, const MaybeTensor& post_b,
                                                   const MaybeTensor& pre_w, const MaybeTensor& pre_b,
                                                   const MaybeTensor& scale_w) {
+    check_not_traced();
     variable_list in = {x};
     for (const MaybeTensor* t : {&y, &gate, &post_w, &post_b, &pre_w, &pre_b, &scale_w}) in.push_back(t->value_or(Tensor()));
     bool wanted = false;

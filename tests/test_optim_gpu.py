@@ -674,3 +674,11 @@ def test_a_first_step_is_not_captured(cuda_device):
     graph.replay()
     graph.replay()
     assert float(opt.state[p]["step"]) == 3.0
+
+
+def test_tracing_is_refused(cuda_device):
+    """A trace would keep the outputs' allocation and not the kernels."""
+    x = torch.randn(8, device=cuda_device)
+    for call in (lambda a: optim_ops.grad_norm([a]), lambda a: optim_ops.clip_grads_([a.clone()], 1.0)):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(call, x, check_trace=False)

@@ -494,3 +494,10 @@ def test_negated_views(shape, dim, cuda_device):
         with torch.no_grad():
             got[-1] += residual_norm(s["x"], s["y"], dim=dim)
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_tracing_is_refused(cuda_device):
+    """A trace would keep the outputs' allocation and not the kernel that fills them."""
+    x, y = torch.randn(2, 3, 8, device=cuda_device)
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(lambda a, b: residual_norm(a, b, dim=-1), (x, y), check_trace=False)
