@@ -402,6 +402,13 @@ bool disjoint(std::vector<Span>& spans) {
     return true;
 }
 
+// Whether `one` shares memory with any of sorted, disjoint spans.
+bool meets(const std::vector<Span>& spans, const Span& one) {
+    const auto at = std::upper_bound(spans.begin(), spans.end(), one.begin,
+                                     [](uintptr_t begin, const Span& s) { return begin < s.end; });
+    return at != spans.end() && at->begin < one.end;
+}
+
 bool valid_tensor(const void* p, long long count, int dtype) {
     return count >= 0 && dtype >= kF32 && dtype <= kF16 && count <= (1LL << 40) &&
            (count == 0 || (p != nullptr && reinterpret_cast<uintptr_t>(p) % element_size(dtype) == 0));
@@ -587,6 +594,9 @@ cudaError_t adam(int n, const AdamLists& l, float* const* steps, double lr, cons
         spans.push_back(span_of(l.v[i], c * 4));
     }
     if (!disjoint(spans)) return cudaErrorInvalidValue;
+    for (int i = 0; i < n; ++i)  // a gradient is read while other blocks write
+        if (l.counts[i] > 0 && meets(spans, span_of(l.g[i], l.counts[i] * static_cast<long long>(element_size(l.dtypes[i])))))
+            return cudaErrorInvalidValue;
     const AdamScalars sc = {static_cast<float>(beta1), static_cast<float>(1.0 - beta1), static_cast<float>(beta2),
                             static_cast<float>(1.0 - beta2), static_cast<float>(eps), static_cast<float>(weight_decay),
                             decoupled ? static_cast<float>(lr * weight_decay) : 0.f, decoupled ? 1 : 0};

@@ -66,7 +66,7 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     with ``decoupled``).
 
     params       float32, bfloat16, float16 or complex64 CUDA tensors, dense, none sharing memory
-    grads        like params (type and shape), left as they are
+    grads        like params (type and shape), left as they are; none shares memory with what is written
     exp_avgs, exp_avg_sqs   the moments: float32 (complex64 for complex params), whatever the
                  params' type, of the params' shape and strides
     steps        0-d float32 CUDA tensors, one per parameter, counted up by the call (so a replayed

@@ -348,7 +348,7 @@ int scx_grad_clip(int n_tensors, void* const* tensors, const long long* counts, 
  * type is, and p is computed in fp32 and rounded once.  steps: one float in device memory per
  * tensor (so a replayed graph advances).  lr_device: NULL, or one float in device memory that
  * is read in place of lr.  Host arrays and addresses as above; params, moments and steps must
- * not overlap one another.  workspace: scx_adam_workspace_size() bytes, 16-byte aligned. */
+ * not overlap one another, nor a gradient.  workspace: scx_adam_workspace_size() bytes, 16-byte aligned. */
 size_t scx_adam_workspace_size(int n_tensors);
 int scx_adam_step(int n_tensors, void* const* params, const void* const* grads,
                   float* const* exp_avgs, float* const* exp_avg_sqs, float* const* steps,
@@ -367,9 +367,10 @@ int scx_adam_step(int n_tensors, void* const* params, const void* const* grads,
  * [batch][channels]; weights, biases and the scale vector are [channels], of type weight_dtype
  * (SCX_FLOAT32 or dtype).  Each may be NULL: weights and scale vector then are ones, biases zeros;
  * y NULL: r = x (t.r is not written), n = pre(x).  post_norm 0: z = y; pre_norm 0: no n; the weights
- * and biases of a norm that is not taken are not read.  The scale vector multiplies config.scale.  Statistics and sums are fp32, and n is computed from the unrounded
- * r.  stats (may be NULL in the forward): 4*batch*length floats for the backward, 16-byte aligned, in
- * an order of the kernels' own.  Outputs must not overlap the inputs or one another. */
+ * and biases of a norm that is not taken are not read.  The scale vector multiplies config.scale.
+ * Statistics and sums are fp32, and n is computed from the unrounded r.  stats (may be NULL in the
+ * forward): 4*batch*length floats for the backward, 16-byte aligned, in an order of the kernels'
+ * own.  Outputs must not overlap the inputs or one another. */
 #define SCX_NORM_RMS 0
 #define SCX_NORM_LAYER 1
 #define SCX_GATE_NONE 0

@@ -184,3 +184,9 @@ def test_load_state_dict_hooks_see_and_change_what_is_loaded():
     ours.load_state_dict(state)
     assert torch.equal(ours.state[p]["exp_avg"], m) and len(seen) == 1
     assert not ours._optimizer_load_state_dict_pre_hooks and not ours._optimizer_load_state_dict_post_hooks
+
+
+@pytest.mark.parametrize("address", [1024, 1000, 1052, 4096, 4124, 5116, 6144, 6116])
+def test_adam_refuses_gradients_in_what_it_writes(address):
+    """32 bytes at `address`, against params at 1024, moments at 4096 and 5120 and the count at 6144."""
+    assert _adam(g=_ptrs(address)) == INVALID

@@ -682,3 +682,17 @@ def test_tracing_is_refused(cuda_device):
     for call in (lambda a: optim_ops.grad_norm([a]), lambda a: optim_ops.clip_grads_([a.clone()], 1.0)):
         with pytest.raises(RuntimeError, match="traced"):
             torch.jit.trace(call, x, check_trace=False)
+
+
+def test_adam_lists_beside_one_another(cuda_device):
+    """Parameter, gradient and moments one behind the other in one buffer, in either order."""
+    for order in ((0, 1, 2, 3), (3, 2, 1, 0), (1, 0, 3, 2)):
+        flat = torch.randn(4 * 1001, device=cuda_device, generator=_gen(cuda_device, 16)).abs()
+        lists = [[flat[1001 * k:1001 * (k + 1)]] for k in order]
+        before = [tuple(_f64(t[0]) for t in lists)]
+        step = torch.zeros((), device=cuda_device)
+        hyper = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8)
+        optim_ops.adam_step_(*lists, [step], **hyper)
+        _check_adam(lists[0], lists[2], lists[3], before, step=1, wd=0.0, decoupled=False, c=1.0, **hyper)
+        with pytest.raises(RuntimeError):
+            optim_ops.adam_step_(lists[0], [flat[500:1501]], lists[2], lists[3], [step], **hyper)
