@@ -11,7 +11,7 @@
 // device, keeps nothing, and can be captured: a table of up to kBigTable tensors goes into the
 // 32 KB of parameters a launch may carry, and longer lists take several launches.
 //
-// Work is cut into units of kUnit bytes of the widest tensor type, numbered through the whole
+// Work is cut into units of kUnit (1024) elements, whatever their type, numbered through the whole
 // list; a block takes one contiguous range of units, so neighbouring blocks do not depend on how
 // the tensors' sizes fall, and walks it tensor by tensor.
 //
@@ -229,8 +229,9 @@ __device__ void scale_piece(T* __restrict__ p, long long n, float c) {
 }
 
 // Per-block partial sums of squares.  In an Adam step block 0 also advances the tensors' step
-// counts and leaves (lr / (1 - b1^t), 1 / sqrt(1 - b2^t)) of each in `corrections`.  AHEAD for long lists
-// (67M fp32 values: 43 us, 47 us without; 2.4M: 7.4 us and 6.2 us without).
+// counts and leaves (lr / (1 - b1^t), 1 / sqrt(1 - b2^t)) of each in `corrections`.  AHEAD for lists of
+// more than kManyUnits (67M fp32 values: 43 us, 47 us without; 2.4M: 7.4 us and 6.2 us without; the limit lies
+// between the two lengths that were measured).
 template <int N, bool STEPS, bool AHEAD>
 __global__ void __launch_bounds__(kThreads) square_sum_kernel(const __grid_constant__ ReadTable<N> t,
                                                               const __grid_constant__ StepTable<STEPS ? N : 1> steps,
@@ -356,7 +357,7 @@ __device__ void adam_piece(T* __restrict__ p, const T* __restrict__ g, float* __
 
 // DEEP vectors of each tensor in flight per thread: two for long lists, whose stream they fill (67M values:
 // 352 us, 373 us with one); one for short ones, where twice the blocks fit an SM (2.4M: 19 us, 21 us
-// with two).
+// with two); the limit as above.
 template <int N, int DEEP>
 __global__ void __launch_bounds__(kThreads) adam_kernel(const __grid_constant__ AdamTable<N> t,
                                                         const float2* corrections, const double* partial, int parts,

@@ -112,7 +112,9 @@ __device__ __forceinline__ float within(float v, float bound) {
 // the difference comes exactly from a fused product, with log2(e) in two parts, so that the error
 // does not grow with g.  Relative error below 8 roundings down to g = -87, where the result leaves
 // the normal numbers and is zero.  For gates of two bytes 2^t alone: the rounding of t costs |g| 2^-24, at
-// most 2^-17.5, a ninetieth of fp16's own (8192x2048 bf16 tokens 107.3 us, with the correction 110.6).
+// most 2^-17.5, a ninetieth of fp16's own (8192x2048 bf16 tokens 107.3 us, with the correction 110.6).  The fp32 sums
+// over positions take it in too: as an absolute error that is 1.25 |g| s (1 - s) 2^-24, below a third of a
+// rounding of one.
 template <typename T>
 __device__ __forceinline__ float2 sigmoid2(float2 g) {
     constexpr float kLog2e = 1.44269504f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.69314718f;

@@ -112,8 +112,8 @@ __device__ __forceinline__ float2 sum_groups(float2 v) {
 
 // A few threads per position add the warps' parts: SHARES of them, each every SHARES-th warp.  WHOLE: the
 // code of all steps at once, which is quicker by itself (training passes: 7x36x96x160 with a gate per sample
-// 47 us against 49, 8x128x128x128 154 against 159).  With a gate per element in fp32, which HBM bounds, a loop:
-// shorter code of a tile keeps the blocks' accesses apart (16x64x256x256: 559 us against 606).
+// 47 us against 49, 8x128x128x128 154 against 159).  With a gate per element in fp32, which HBM bounds, a loop
+// (16x64x256x256: 559 us against 606; measured on that shape alone; what makes the difference is not known).
 template <int SHARES, bool WHOLE>
 struct Share {
     int me;
@@ -494,7 +494,9 @@ __device__ __forceinline__ float sum_positions(float v) {
 __host__ __device__ constexpr int backward_tensors(int mode) { return mode == kFull ? 5 : 4; }
 
 // MAXW: the most warps it is launched with.  Up to 10 the registers are held to what lets two blocks
-// share an SM (36 channels of 7 x 96 x 160 with a gate per sample: 30 us against 40 us).
+// share an SM (36 channels of 7 x 96 x 160 with a gate per sample: 30 us against 40 us).  With a gate per element
+// that spills 52 to 56 bytes of the 10 warps' kernel, as the forward's two blocks per SM do up to 80 of the kernels
+// by single values.
 template <typename T, int V, int EPT, int LC, int MODE, int MAXW>
 __global__ void __launch_bounds__(MAXW * 32, MAXW <= 10 ? 2 : 1) field_backward_kernel(const __grid_constant__ Problem p) {
     using F = Slots<T, V, EPT>;

@@ -692,8 +692,9 @@ bool vectors_fit(const Problem& p) {
 
 // More per thread comes before a cluster: a position's sums within a block cost half of what a cluster's
 // exchange does (4096 tokens of 8192 bf16 channels: forward 48 us, over two blocks 91).  What the forward keeps
-// of 16 values fits its registers; the backward's sums and weights leave room for 8 with a gate, and for 16
-// without one (training pass of the same tokens 195 us, over two blocks 217; with a gate 304 and 265).
+// of 16 values fits its registers (all but 28 bytes in fp16 with a gate).  The backward's sums and weights do not: of 16 two-byte values it spills 416
+// bytes without a gate, and is still the quicker there (training pass of the same tokens 195 us, over two blocks
+// 217); with a gate it is not (304 and 265), and 8 values per thread are kept.
 template <typename T, int MODE>
 cudaError_t forward_in(const Problem& p, cudaStream_t s) {
     constexpr int VEC = 16 / static_cast<int>(sizeof(T));
