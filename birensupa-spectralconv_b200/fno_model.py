@@ -311,8 +311,8 @@ class ResidualFNO2d(nn.Module):
     ``gate``: "none", "element" (a 1x1 convolution of n) or "sample" (a linear map of n's mean over
     the positions).  ``norm``: "rms" or "layer".  The layer kernels are ``residual_norm``'s, forward
     and backward, and the spectral convolutions the library's; 1x1 convolutions and GELU run as torch
-    operations in full float32.  Interfaces as FNO2d's: ``forward_device``, ``forward_autograd``,
-    ``forward(x, use_supa)``."""
+    operations in full float32.  Interfaces as FNO2d's: ``forward_device`` and ``forward_autograd``, of a model on
+    x's device, ``forward(x, use_supa)``, ``prepare_supa_eval``."""
 
     def __init__(self, modes1: int = 12, modes2: int = 12, width: int = 32, n_layers: int = 4, in_channels: int = 10,
                  out_channels: int = 1, gate: str = "element", norm: str = "rms", scale: float = 0.5):
@@ -358,6 +358,10 @@ class ResidualFNO2d(nn.Module):
         return self._run_device(x, lambda sc, n: spectral_conv2d_autograd(n, sc.weights1, sc.weights2, sc.modes1,
                                                                           sc.modes2))
 
+    def prepare_supa_eval(self) -> None:
+        """Moves every parameter to the current CUDA device."""
+        self.to(torch.device("cuda", torch.cuda.current_device()))
+
     @torch.no_grad()
     def forward_device(self, x: torch.Tensor) -> torch.Tensor:
         """Forward on x's CUDA device, [B, T, H, W] to [B, out_channels, H, W]."""
@@ -366,11 +370,13 @@ class ResidualFNO2d(nn.Module):
         return self._run_device(x, lambda sc, n: sc(n))
 
     def forward(self, x: torch.Tensor, use_supa: bool = True) -> torch.Tensor:
-        """As FNO2d's: on the CUDA device with a host result, or (``use_supa=False``) in torch
-        operations on the host."""
+        """As FNO2d's: on the CUDA device with a host result (weights held elsewhere are copied for the
+        call), or (``use_supa=False``) in torch operations on the host."""
         if use_supa:
             device = x.device if x.is_cuda else torch.device("cuda", torch.cuda.current_device())
-            return self.forward_device(x.to(device=device, dtype=torch.float32)).cpu()
+            x = x.to(device=device, dtype=torch.float32)
+            away = {k: p.detach().to(device) for k, p in self.named_parameters() if p.device != device}
+            return torch.func.functional_call(self, away, (x,)) if away else self.forward_device(x).cpu()
         return self._run(x.cpu(), lambda sc, n: sc(n, use_supa=False), _residual_norm_host)
 
 

@@ -152,3 +152,22 @@ def test_a_captured_training_step(cuda_device):
         graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(_real(p), _real(q)) for p, q in zip(model.parameters(), eager.parameters()))
+
+
+@pytest.mark.parametrize("gate", ["element", "sample"])
+def test_a_model_on_the_host_runs_on_the_device(gate, cuda_device):
+    """model(x) as FNO2d's: weights held on the host are copied for the call and stay where they are."""
+    model = _model(gate)
+    there = copy.deepcopy(model).to(cuda_device)
+    x = torch.randn(2, 10, 32, 32)
+    want = there.forward_device(x.to(cuda_device)).cpu()
+    for given in (x, x.to(cuda_device)):
+        got = model(given)
+        assert not got.is_cuda and torch.equal(got, want)
+    assert all(not p.is_cuda for p in model.parameters())
+    with torch.no_grad():
+        model.first_weight.mul_(2.0)
+        there.first_weight.mul_(2.0)
+    assert torch.equal(model(x), there.forward_device(x.to(cuda_device)).cpu())
+    model.prepare_supa_eval()
+    assert all(p.is_cuda for p in model.parameters()) and torch.equal(model(x), there(x))
